@@ -6,6 +6,7 @@
 #include "kda_common.cuh"
 #include "kda_cp.cuh"
 #include "kda_plan.cuh"
+#include "kda_serving.cuh"
 
 namespace {
 
@@ -409,9 +410,19 @@ const char* kda_error_string(int code) {
   }
 }
 
-size_t kda_abi_struct_bytes(int which) { return which == 0 ? sizeof(KdaPrefillArgs) : (which == 1 ? sizeof(KdaSegmentArgs) : 0); }
+size_t kda_abi_struct_bytes(int which) {
+  switch (which) {
+    case 0: return sizeof(KdaPrefillArgs);
+    case 1: return sizeof(KdaSegmentArgs);
+    case 2: return sizeof(KdaConvArgs);
+    case 3: return sizeof(KdaScanArgs);
+    case 4: return sizeof(KdaStepArgs);
+    case 5: return sizeof(KdaPoolArgs);
+    default: return 0;
+  }
+}
 
-const char* kda_version(void) { return "kda_b200 4 sm_100a"; }
+const char* kda_version(void) { return "kda_b200 5 sm_100a"; }
 
 int kda_prefill_plan_counts(const KdaPrefillArgs* a, int32_t* counts, void* stream_) {
   if (a == nullptr || counts == nullptr || a->workspace == nullptr || a->H <= 0 || a->N < 1) return KDA_ERR_ARG;
@@ -432,6 +443,202 @@ int kda_debug_configure(int64_t wait_limit_us, int32_t flags, void* prof_counter
   g_debug_flags = flags;
   g_prof = reinterpret_cast<unsigned long long*>(prof_counters);
   return KDA_OK;
+}
+
+}  // extern "C"
+
+// ---- the operators around the prefill (kernels: kda_conv.cu, kda_sscan.cu, kda_step.cu, kda_pool.cu)
+namespace {
+
+bool known_type(int type) { return type >= KDA_TYPE_BF16 && type <= KDA_TYPE_FP32; }
+
+// whether every pointer lies at a whole value of `type`
+template <typename... P>
+bool whole(int type, const P*... p) {
+  const uintptr_t size = type == KDA_TYPE_FP32 ? 4 : 2;
+  return (((reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0) && ...);
+}
+bool whole_table(const void* p, int is64) { return (reinterpret_cast<uintptr_t>(p) & (is64 ? 7 : 3)) == 0; }
+
+int check_sequences(const KdaSequences& s, bool step) {
+  if (s.N < 0 || s.T < 0 || s.n_slots < 0) return KDA_ERR_ARG;
+  if (s.T > 0x7fffffffLL) return KDA_ERR_LIMIT;
+  if (!whole_table(s.cu_seqlens, s.cu_is64) || !whole_table(s.slots, s.slots_is64) || !whole_table(s.status, 0)) return KDA_ERR_ARG;
+  if (step) return s.N == s.T && (s.slots != nullptr || s.n_slots >= s.N) ? KDA_OK : KDA_ERR_ARG;
+  if (s.N < 1 || (s.cu_seqlens == nullptr && s.N != 1)) return KDA_ERR_ARG;
+  return s.slots != nullptr || s.n_slots >= s.N ? KDA_OK : KDA_ERR_ARG;
+}
+
+kda::SeqTable seq_table(const KdaSequences& s) {
+  kda::SeqTable t;
+  t.cu = s.cu_seqlens; t.slots = s.slots; t.status = s.status; t.T = s.T; t.n_slots = s.n_slots;
+  t.cu_is64 = s.cu_is64; t.slots_is64 = s.slots_is64; t.N = s.N;
+  return t;
+}
+
+int launched(cudaError_t e) { return e == cudaSuccess ? KDA_OK : cuda_fail(e); }
+
+int conv_launch(const KdaConvArgs* a, bool step, void* stream) {
+  if (a == nullptr || a->C < 1 || a->W < 2 || a->W > 4 || !known_type(a->type) || !known_type(a->weight_type)) return KDA_ERR_ARG;
+  const int rc = check_sequences(a->seq, step);
+  if (rc != KDA_OK) return rc;
+  if (!a->weight || (a->seq.T > 0 && (!a->x || !a->out || a->ldx < a->C || a->ldo < a->C))) return KDA_ERR_ARG;
+  if (!whole(a->type, a->x, a->out, a->src, a->dst) || !whole(a->weight_type, a->weight, a->bias)) return KDA_ERR_ARG;
+  const int64_t rows = (int64_t)(a->W - 1) * a->C;
+  if ((a->src && a->src_slot_stride < rows) || (a->dst && a->dst_slot_stride < rows)) return KDA_ERR_ARG;
+  if (step && a->seq.T > 0 && (!a->dst || a->src != a->dst || a->src_slot_stride != a->dst_slot_stride)) return KDA_ERR_ARG;
+  kda::ConvParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x; p.weight = a->weight; p.bias = a->bias; p.out = a->out; p.src = a->src; p.dst = a->dst;
+  p.seq = seq_table(a->seq);
+  p.ldx = a->ldx; p.ldo = a->ldo; p.src_stride = a->src_slot_stride; p.dst_stride = a->dst_slot_stride;
+  p.C = a->C; p.W = a->W; p.silu = a->silu != 0; p.weight_type = a->weight_type; p.zero_pad = a->seq.zero_rest != 0;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return launched(step ? kda::launch_conv_step(p, a->type, s) : kda::launch_conv(p, a->type, s));
+}
+
+int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
+  if (a == nullptr || a->Dm < 1 || a->Ns < 1 || a->groups < 1 || a->Dm % a->groups || !known_type(a->type)) return KDA_ERR_ARG;
+  if (a->Ns > KDA_SCAN_MAX_STATE) return KDA_ERR_LIMIT;
+  const int rc = check_sequences(a->seq, step);
+  if (rc != KDA_OK) return rc;
+  if (!a->A) return KDA_ERR_ARG;
+  if (!whole(a->type, a->u, a->dt, a->B, a->C, a->z, a->out) || !whole(KDA_TYPE_FP32, a->A, a->D, a->dt_bias, a->src, a->dst)) return KDA_ERR_ARG;
+  const int64_t gn = (int64_t)a->groups * a->Ns, rows = (int64_t)a->Dm * a->Ns;
+  if (a->seq.T > 0) {
+    if (!a->u || !a->dt || !a->B || !a->C || !a->out) return KDA_ERR_ARG;
+    if (a->ldu < a->Dm || a->lddt < a->Dm || a->ldo < a->Dm || (a->z && a->ldz < a->Dm) || a->ldb < gn || a->ldc < gn) return KDA_ERR_ARG;
+  }
+  if ((a->src && a->src_slot_stride < rows) || (a->dst && a->dst_slot_stride < rows)) return KDA_ERR_ARG;
+  if (step && a->seq.T > 0 && (!a->dst || a->src != a->dst || a->src_slot_stride != a->dst_slot_stride)) return KDA_ERR_ARG;
+  kda::ScanParams p;
+  memset(&p, 0, sizeof(p));
+  p.u = a->u; p.dt = a->dt; p.B = a->B; p.C = a->C; p.z = a->z; p.out = a->out;
+  p.A = a->A; p.D = a->D; p.dt_bias = a->dt_bias; p.src = a->src; p.dst = a->dst;
+  p.seq = seq_table(a->seq);
+  p.ldu = a->ldu; p.lddt = a->lddt; p.ldb = a->ldb; p.ldc = a->ldc; p.ldz = a->ldz; p.ldo = a->ldo;
+  p.src_stride = a->src_slot_stride; p.dst_stride = a->dst_slot_stride;
+  p.Dm = a->Dm; p.Ns = a->Ns; p.groups = a->groups; p.softplus = a->softplus != 0; p.zero_pad = a->seq.zero_rest != 0;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return launched(step ? kda::launch_sscan_step(p, a->type, s) : kda::launch_sscan(p, a->type, s));
+}
+
+// The parts of the argument block that a call uses, checked; fills the kernels' parameters.
+int pool_params(const KdaPoolArgs* a, bool used, bool src, bool copies, kda::PoolPlan& p, kda::PoolRows& r) {
+  if (a == nullptr || a->slots < 1 || a->n < 0) return KDA_ERR_ARG;
+  if (a->slots > 0x7fffffffLL || a->n > 0x3fffffffLL) return KDA_ERR_LIMIT;
+  if ((used && !a->used) || (src && a->n > 0 && !a->src)) return KDA_ERR_ARG;
+  if (!whole_table(a->src, a->src_is64) || !whole_table(a->dst, a->dst_is64) || !whole_table(a->status, 0) || !whole_table(a->slots_out, 0) ||
+      !whole_table(a->remap, 0)) return KDA_ERR_ARG;
+  memset(&p, 0, sizeof(p));
+  memset(&r, 0, sizeof(r));
+  if (copies) {
+    if (a->n_pools < 0 || a->n_pools > KDA_MAX_POOLS) return KDA_ERR_ARG;
+    for (int k = 0; k < a->n_pools; k++) {
+      if (!a->base[k] || a->bytes[k] < 1 || a->stride[k] < a->bytes[k]) return KDA_ERR_ARG;
+      r.base[k] = reinterpret_cast<unsigned char*>(a->base[k]);
+      r.stride[k] = a->stride[k];
+      r.bytes[k] = a->bytes[k];
+    }
+    if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 3)) return KDA_ERR_ARG;
+    if (a->workspace_bytes < kda_pool_workspace_bytes(a->n, a->slots)) return KDA_ERR_WORKSPACE;
+  }
+  r.n = a->n_pools;
+  r.slots = a->slots;
+  p.used = a->used; p.src = a->src; p.dst = a->dst; p.src_is64 = a->src_is64; p.dst_is64 = a->dst_is64; p.n = a->n;
+  p.slots_out = a->slots_out; p.remap = a->remap; p.moves = reinterpret_cast<int*>(a->workspace); p.status = a->status; p.P = a->slots;
+  return KDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kda_short_conv_launch(const KdaConvArgs* a, void* stream) { return conv_launch(a, false, stream); }
+int kda_short_conv_step_launch(const KdaConvArgs* a, void* stream) { return conv_launch(a, true, stream); }
+
+size_t kda_selective_scan_workspace_bytes(int64_t T, int32_t N, int32_t Dm, int32_t Ns) {
+  (void)T; (void)N; (void)Dm; (void)Ns;
+  return 0;
+}
+int kda_selective_scan_launch(const KdaScanArgs* a, void* stream) { return scan_launch(a, false, stream); }
+int kda_selective_scan_step_launch(const KdaScanArgs* a, void* stream) { return scan_launch(a, true, stream); }
+
+int kda_step_launch(const KdaStepArgs* a, void* stream) {
+  if (a == nullptr || a->H < 1) return KDA_ERR_ARG;
+  if (a->frontend != KDA_FRONTEND_RAW && a->frontend != KDA_FRONTEND_PLAIN) return KDA_ERR_ARG;
+  const int rc = check_sequences(a->seq, true);
+  if (rc != KDA_OK) return rc;
+  const bool raw = a->frontend == KDA_FRONTEND_RAW;
+  if (raw && (!a->A_log || !a->dt_bias)) return KDA_ERR_ARG;
+  if (!whole(KDA_TYPE_BF16, a->q, a->k, a->v, a->out) || !whole(raw ? KDA_TYPE_BF16 : KDA_TYPE_FP32, a->g, a->beta)) return KDA_ERR_ARG;
+  if (!whole(KDA_TYPE_FP32, a->A_log, a->dt_bias)) return KDA_ERR_ARG;
+  const int64_t hd = (int64_t)a->H * KDA_HEAD_DIM;
+  if (a->seq.T > 0) {
+    if (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->out) return KDA_ERR_ARG;
+    if (a->ldq < hd || a->ldk < hd || a->ldv < hd || a->ldg < hd || a->ldo < hd || a->ldbeta < a->H) return KDA_ERR_ARG;
+    if (!a->pool || !aligned16(a->pool) || (a->slot_stride & 3) || a->slot_stride < hd * KDA_HEAD_DIM) return KDA_ERR_ARG;
+  }
+  kda::StepParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = reinterpret_cast<const __nv_bfloat16*>(a->q);
+  p.k = reinterpret_cast<const __nv_bfloat16*>(a->k);
+  p.v = reinterpret_cast<const __nv_bfloat16*>(a->v);
+  p.g = a->g; p.beta = a->beta;
+  p.out = reinterpret_cast<__nv_bfloat16*>(a->out);
+  p.A_log = a->A_log; p.dt_bias = a->dt_bias; p.pool = a->pool;
+  p.seq = seq_table(a->seq);
+  p.ldq = a->ldq; p.ldk = a->ldk; p.ldv = a->ldv; p.ldg = a->ldg; p.ldbeta = a->ldbeta; p.ldo = a->ldo; p.slot_stride = a->slot_stride;
+  p.scale = a->scale; p.lower_bound = a->lower_bound; p.H = a->H; p.raw = raw; p.zero_pad = a->seq.zero_rest != 0;
+  return launched(kda::launch_kda_step(p, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t kda_pool_workspace_bytes(int64_t n, int64_t P) {
+  if (n < 0 || P < 1) return 0;
+  return sizeof(int) * (size_t)(4 + (3 * n > P + 2 ? 3 * n : P + 2));   // pairs and free slots of n entries, or P / 2 moves
+}
+
+int kda_pool_copy_launch(const KdaPoolArgs* a, void* stream) {
+  kda::PoolPlan p;
+  kda::PoolRows r;
+  const int rc = pool_params(a, false, true, true, p, r);
+  if (rc != KDA_OK) return rc;
+  if (a->n == 0) return KDA_OK;
+  if (!a->dst) return KDA_ERR_ARG;
+  return launched(kda::launch_pool_copy(p, r, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int kda_pool_fork_launch(const KdaPoolArgs* a, void* stream) {
+  kda::PoolPlan p;
+  kda::PoolRows r;
+  const int rc = pool_params(a, true, true, true, p, r);
+  if (rc != KDA_OK) return rc;
+  if (a->n == 0) return KDA_OK;
+  if (!a->slots_out) return KDA_ERR_ARG;
+  return launched(kda::launch_pool_fork(p, r, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int kda_pool_free_launch(const KdaPoolArgs* a, void* stream) {
+  kda::PoolPlan p;
+  kda::PoolRows r;
+  const int rc = pool_params(a, true, true, false, p, r);
+  if (rc != KDA_OK) return rc;
+  if (a->n == 0) return KDA_OK;
+  return launched(kda::launch_pool_free(p, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+int kda_pool_compact_launch(const KdaPoolArgs* a, void* stream) {
+  kda::PoolPlan p;
+  kda::PoolRows r;
+  const int rc = pool_params(a, true, false, true, p, r);
+  if (rc != KDA_OK) return rc;
+  if (!a->remap || a->n_tables < 0 || a->n_tables > KDA_MAX_TABLES) return KDA_ERR_ARG;
+  p.n_tables = a->n_tables;
+  for (int t = 0; t < a->n_tables; t++) {
+    if (a->table_n[t] < 0 || (a->table_n[t] > 0 && !a->tables[t]) || !whole_table(a->tables[t], a->table_is64[t])) return KDA_ERR_ARG;
+    p.tables[t] = a->tables[t]; p.table_n[t] = a->table_n[t]; p.table_is64[t] = a->table_is64[t];
+  }
+  return launched(kda::launch_pool_compact(p, r, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

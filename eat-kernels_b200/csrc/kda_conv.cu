@@ -1,0 +1,212 @@
+// Short causal convolution over packed sequences, depthwise:
+//   y[t, c] = act(b[c] + sum_j w[c, j] x[t - (W - 1) + j, c])
+// Rows in front of a sequence are the W - 1 history rows of its slot; its last W - 1 rows become the new history.
+#include "kda_serving.cuh"
+
+namespace kda {
+
+namespace {
+
+constexpr int CONV_THREADS = 128;
+
+__device__ __forceinline__ float weight_at(const void* p, int type, long long i) {
+  if (type == TYPE_BF16) return to_float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  if (type == TYPE_FP16) return to_float(reinterpret_cast<const __half*>(p)[i]);
+  return reinterpret_cast<const float*>(p)[i];
+}
+
+template <int VEC, int W>
+__device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (&w)[W][VEC], float (&b)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++) {
+#pragma unroll
+    for (int j = 0; j < W; j++) w[j][i] = weight_at(p.weight, p.weight_type, (long long)(c + i) * W + j);
+    b[i] = p.bias != nullptr ? weight_at(p.bias, p.weight_type, c + i) : 0.0f;
+  }
+}
+
+// VEC channels a thread, a tile of tokens a block.  A sequence's first W - 1 tokens belong to the tile that holds its start,
+// even where they reach into the next tile: only that tile reads the slot's history, and it writes the new one after that,
+// so the pool is updated in place by one launch.  Bound by memory: the window slides in registers, a tile re-reads W - 1
+// rows of the tile before it (out of L2).
+template <typename T, int VEC, int W>
+__global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const ConvParams p) {
+  constexpr int HW = W - 1;
+  using P = Pack<T, VEC>;
+  const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
+  const long long t0 = (long long)(blockIdx.x / cblocks) * p.tile;
+  const long long t1 = min(t0 + p.tile, p.seq.T);
+  const bool last = t1 == p.seq.T;
+  const int c = ((int)(blockIdx.x % cblocks) * CONV_THREADS + (int)threadIdx.x) * VEC;
+  const bool mine = c < p.C;
+  const T* x = reinterpret_cast<const T*>(p.x) + c;
+  T* out = reinterpret_cast<T*>(p.out) + c;
+  const T* src = reinterpret_cast<const T*>(p.src) + c;
+  T* dst = reinterpret_cast<T*>(p.dst) + c;
+  const int N = p.seq.N;
+  P zero;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) zero.v[i] = from_float<T>(0.0f);
+
+  const bool rejected = cu_rejected(p.seq);
+  float w[W][VEC], b[VEC];
+  if (mine) load_weights<VEC, W>(p, c, w, b);
+
+  auto run = [&](long long from, long long to, float (&win)[HW][VEC]) {
+#pragma unroll 4
+    for (long long t = from; t < to; t++) {
+      float cur[VEC], y[VEC];
+      unpack(*reinterpret_cast<const P*>(x + t * p.ldx), cur);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        float acc = b[i];
+#pragma unroll
+        for (int j = 0; j < HW; j++) acc = fmaf(w[j][i], win[j][i], acc);
+        acc = fmaf(w[HW][i], cur[i], acc);
+        y[i] = p.silu ? silu<T>(acc) : acc;
+#pragma unroll
+        for (int j = 0; j + 1 < HW; j++) win[j][i] = win[j + 1][i];
+        win[HW - 1][i] = cur[i];
+      }
+      *reinterpret_cast<P*>(out + t * p.ldo) = pack<T, VEC>(y);
+    }
+  };
+
+  // the first sequence that starts in this tile, and the one that reaches into it
+  int lo = 0, hi = N + 1;
+  if (!rejected) {
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (cu_at(p.seq, mid) >= t0) hi = mid; else lo = mid + 1;
+    }
+  }
+  if (!rejected && mine && lo > 0 && lo <= N) {
+    const long long begin = cu_at(p.seq, lo - 1), end = cu_at(p.seq, lo);
+    const long long from = max(t0, begin + HW), to = min(end, t1);
+    if (from < to) {
+      float win[HW][VEC];
+#pragma unroll
+      for (int j = 0; j < HW; j++) unpack(*reinterpret_cast<const P*>(x + (from - HW + j) * p.ldx), win[j]);
+      run(from, to, win);
+    }
+  }
+  // sequences that start here, empty ones among them (behind a rejected layout all are empty and the first tile has them)
+  for (int s = rejected ? (t0 == 0 ? 0 : N) : lo; s < N; s++) {
+    const long long begin = rejected ? 0 : cu_at(p.seq, s), end = rejected ? 0 : cu_at(p.seq, s + 1);
+    if (!rejected && begin >= t1 && !(last && begin == t1)) break;
+    const long long slot = claim_slot(p.seq, s);
+    if (!mine) continue;
+    P hist[HW];
+#pragma unroll
+    for (int j = 0; j < HW; j++)
+      hist[j] = p.src != nullptr && slot >= 0 ? *reinterpret_cast<const P*>(src + slot * p.src_stride + (long long)j * p.C) : zero;
+    if (p.dst != nullptr && slot >= 0) {
+      const long long len = end - begin;
+#pragma unroll
+      for (int j = 0; j < HW; j++) {
+        P row = zero;
+        if (len >= HW - j) row = *reinterpret_cast<const P*>(x + (end - HW + j) * p.ldx);
+#pragma unroll
+        for (int h = 0; h < HW; h++)
+          if (h == len + j) row = hist[h];
+        *reinterpret_cast<P*>(dst + slot * p.dst_stride + (long long)j * p.C) = row;
+      }
+    }
+    float win[HW][VEC];
+#pragma unroll
+    for (int j = 0; j < HW; j++) unpack(hist[j], win[j]);
+    run(begin, min(end, max(t1, begin + HW)), win);
+  }
+  if ((rejected || p.zero_pad) && mine)
+    for (long long t = rejected ? t0 : max(t0, cu_at(p.seq, N)); t < t1; t++) *reinterpret_cast<P*>(out + t * p.ldo) = zero;
+}
+
+// One token a row, VEC channels a thread: the window is the slot's history and the token.
+template <typename T, int VEC, int W>
+__global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const ConvParams p) {
+  constexpr int HW = W - 1;
+  using P = Pack<T, VEC>;
+  const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
+  const int row = blockIdx.x / cblocks;
+  const int c = ((int)(blockIdx.x % cblocks) * CONV_THREADS + (int)threadIdx.x) * VEC;
+  const long long slot = claim_row(p.seq, row);
+  if (c >= p.C) return;
+  P* out = reinterpret_cast<P*>(reinterpret_cast<T*>(p.out) + row * p.ldo + c);
+  float y[VEC];
+  if (slot == -2) {
+#pragma unroll
+    for (int i = 0; i < VEC; i++) y[i] = 0.0f;
+    if (p.zero_pad) *out = pack<T, VEC>(y);
+    return;
+  }
+  float w[W][VEC];
+  load_weights<VEC, W>(p, c, w, y);
+  T* pool = reinterpret_cast<T*>(p.dst) + slot * p.dst_stride + c;
+  const P cur = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + row * p.ldx + c);
+  P hist[HW];
+  if (slot >= 0) {
+#pragma unroll
+    for (int j = 0; j < HW; j++) hist[j] = *reinterpret_cast<const P*>(pool + (long long)j * p.C);
+#pragma unroll
+    for (int j = 0; j + 1 < HW; j++) *reinterpret_cast<P*>(pool + (long long)j * p.C) = hist[j + 1];
+    *reinterpret_cast<P*>(pool + (long long)(HW - 1) * p.C) = cur;
+#pragma unroll
+    for (int j = 0; j < HW; j++) {
+      float f[VEC];
+      unpack(hist[j], f);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) y[i] = fmaf(w[j][i], f[i], y[i]);
+    }
+  }
+  float f[VEC];
+  unpack(cur, f);
+#pragma unroll
+  for (int i = 0; i < VEC; i++) {
+    y[i] = fmaf(w[HW][i], f[i], y[i]);
+    if (p.silu) y[i] = silu<T>(y[i]);
+  }
+  *out = pack<T, VEC>(y);
+}
+
+// 16-byte accesses where every row starts on 16 bytes, single values elsewhere.
+template <typename T>
+bool wide(const ConvParams& p) {
+  constexpr int VEC = 16 / sizeof(T);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.src) |
+                       reinterpret_cast<uintptr_t>(p.dst);
+  return (at & 15) == 0 && ((p.C | p.ldx | p.ldo | p.src_stride | p.dst_stride) & (VEC - 1)) == 0;
+}
+
+template <typename T, int VEC>
+cudaError_t launch_width(const ConvParams& p, bool step, cudaStream_t stream) {
+  const long long cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
+  const long long rows = step ? p.seq.T : (p.seq.T > 0 ? (p.seq.T + p.tile - 1) / p.tile : 1);
+  const long long blocks = cblocks * rows;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (blocks == 0) return cudaSuccess;
+  const dim3 grid((unsigned)blocks);
+  if (p.W == 2) step ? kda_short_conv_step_kernel<T, VEC, 2><<<grid, CONV_THREADS, 0, stream>>>(p) : kda_short_conv_kernel<T, VEC, 2><<<grid, CONV_THREADS, 0, stream>>>(p);
+  if (p.W == 3) step ? kda_short_conv_step_kernel<T, VEC, 3><<<grid, CONV_THREADS, 0, stream>>>(p) : kda_short_conv_kernel<T, VEC, 3><<<grid, CONV_THREADS, 0, stream>>>(p);
+  if (p.W == 4) step ? kda_short_conv_step_kernel<T, VEC, 4><<<grid, CONV_THREADS, 0, stream>>>(p) : kda_short_conv_kernel<T, VEC, 4><<<grid, CONV_THREADS, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_type(ConvParams p, bool step, cudaStream_t stream) {
+  p.tile = 32;
+  if (wide<T>(p)) return launch_width<T, 16 / sizeof(T)>(p, step, stream);
+  return launch_width<T, 1>(p, step, stream);
+}
+
+cudaError_t launch_any(const ConvParams& p, int type, bool step, cudaStream_t stream) {
+  if (type == TYPE_BF16) return launch_type<__nv_bfloat16>(p, step, stream);
+  if (type == TYPE_FP16) return launch_type<__half>(p, step, stream);
+  return launch_type<float>(p, step, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_conv(ConvParams p, int type, cudaStream_t stream) { return launch_any(p, type, false, stream); }
+cudaError_t launch_conv_step(ConvParams p, int type, cudaStream_t stream) { return launch_any(p, type, true, stream); }
+
+}  // namespace kda

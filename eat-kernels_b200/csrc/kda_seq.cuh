@@ -1,0 +1,103 @@
+// What the operators around the KDA prefill share on the device: the caller's sequence and slot tables, read where they lie
+// and checked by whoever uses them, and the token types.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace kda {
+
+constexpr int SEQ_BAD_CU = 1, SEQ_BAD_SLOT = 2, SEQ_POOL_FULL = 32;      // KDA_STATUS_* of these operators
+
+// Sequences of a packed batch and the slots of their states.  Without `cu` there is one sequence [0, T) (a step: T sequences
+// of one token); without `slots` sequence i uses slot i.
+struct SeqTable {
+  const void* cu;
+  const void* slots;
+  int* status;
+  long long T, n_slots;
+  int cu_is64, slots_is64, N;
+};
+
+__device__ __forceinline__ long long table_at(const void* p, int is64, long long i) {
+  return is64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+__device__ __forceinline__ long long cu_at(const SeqTable& s, long long i) {
+  return s.cu != nullptr ? table_at(s.cu, s.cu_is64, i) : (i == 0 ? 0 : s.T);
+}
+
+__device__ __forceinline__ void report(int* status, int bits) {
+  if (status != nullptr) atomicOr(status, bits);
+}
+
+// Called by the whole block: is cu_seqlens not 0-based, decreasing or beyond T?  Every block looks for itself (N + 1 entries
+// out of L2, one pass of a block up to its number of threads) instead of waiting for a planner launch in front.
+__device__ __forceinline__ bool cu_rejected(const SeqTable& s) {
+  if (s.cu == nullptr) return false;
+  int bad = 0;
+  for (int i = threadIdx.x; i <= s.N; i += blockDim.x) {
+    const long long c0 = cu_at(s, i), c1 = i < s.N ? cu_at(s, i + 1) : c0;
+    if (c0 < 0 || c0 > s.T || c1 < c0 || (i == 0 && c0 != 0)) bad = 1;
+  }
+  const bool rejected = __syncthreads_or(bad) != 0;
+  if (rejected && threadIdx.x == 0) report(s.status, SEQ_BAD_CU);
+  return rejected;
+}
+
+// Called by the whole block: the slot of sequence i, or -1 where its entry is out of range or repeats an earlier one (the
+// first claim keeps the slot, as in the prefill's planner).
+__device__ __forceinline__ long long claim_slot(const SeqTable& s, int i) {
+  if (s.slots == nullptr) return i;
+  const long long d = table_at(s.slots, s.slots_is64, i);
+  int bad = d < 0 || d >= s.n_slots;
+  for (int j = threadIdx.x; j < i && !bad; j += blockDim.x)
+    if (table_at(s.slots, s.slots_is64, j) == d) bad = 1;
+  if (__syncthreads_or(bad) == 0) return d;
+  if (threadIdx.x == 0) report(s.status, SEQ_BAD_SLOT);
+  return -1;
+}
+
+// The same for a row of a step, where a negative entry stands for a row of padding: -2.
+__device__ __forceinline__ long long claim_row(const SeqTable& s, int i) {
+  if (s.slots != nullptr && table_at(s.slots, s.slots_is64, i) < 0) return -2;
+  return claim_slot(s, i);
+}
+
+// ---- token types
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// VEC consecutive values of a row: one access of VEC * sizeof(T) bytes, aligned to that.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& p, float (&f)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++) f[i] = to_float(p.v[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC]) {
+  Pack<T, VEC> p;
+#pragma unroll
+  for (int i = 0; i < VEC; i++) p.v[i] = from_float<T>(f[i]);
+  return p;
+}
+
+// x / (1 + e^-x): the approximate exponential and quotient are off by some 2^-21, which 16-bit outputs do not show; 32-bit
+// ones take the exact functions.
+template <typename T>
+__device__ __forceinline__ float silu(float x) {
+  if constexpr (sizeof(T) == 4) return x / (1.0f + expf(-x));
+  return __fdividef(x, 1.0f + __expf(-x));
+}
+
+}  // namespace kda

@@ -16,6 +16,9 @@ cu_seqlens [N+1] int32/int64 or None (one sequence).  Gate, beta sigmoid and q/k
 `chunk_kda` is the plain, pre-activated call (g = fp32 log-decay, beta in (0,1), q/k already normalised, state
 key-first [N, H, K, V]).
 
+The operators around it in a recurrent layer (short convolution, selective scan, the single-token steps) are in `serving.py`, the
+upkeep of the slot pools in `pool.py`.
+
 All compute goes through the C ABI of libkda_b200.so (include/kda_b200.h); this module only checks arguments,
 owns output / workspace tensors and passes raw device pointers.  There is no CPU or eager fallback.
 """
@@ -32,7 +35,9 @@ D = 128
 CHUNK = 32
 LOWER_BOUND = -5.0   # the reference fixes the gate's lower bound (kda/b200/csrc/w3/base/kernel.py:723)
 
-__all__ = ["kda_prefill", "run", "prepare", "status_bits", "chunk_kda", "prepare_plain"]
+__all__ = ["kda_prefill", "run", "prepare", "status_bits", "chunk_kda", "prepare_plain",
+           "short_conv", "short_conv_step", "selective_scan", "selective_scan_step", "kda_step", "kda_step_plain",
+           "pool_copy", "pool_fork", "pool_free", "pool_compact"]
 
 
 def default_kernel():
@@ -46,7 +51,10 @@ def _err(msg):
 
 
 def _byte_interval(t):
-    """[lo, hi) of the bytes a tensor's elements can touch (its extreme elements under its strides), or None when empty."""
+    """[lo, hi) of the bytes a tensor's elements can touch (its extreme elements under its strides), or None when empty.  A pair
+    is such an interval already."""
+    if isinstance(t, tuple):
+        return t
     if t is None or not torch.is_tensor(t) or t.numel() == 0:
         return None
     reach = 0
@@ -414,3 +422,8 @@ def chunk_kda(q, k, v, g, beta, scale=None, initial_state=None, output_final_sta
     res = _prepare_plain(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens, serving)()
     o = res[0].reshape(shape)
     return (o if dt == torch.bfloat16 else o.to(dt), *res[1:])
+
+
+from .pool import pool_compact, pool_copy, pool_fork, pool_free  # noqa: E402
+from .serving import (kda_step, kda_step_plain, selective_scan, selective_scan_step, short_conv,  # noqa: E402
+                      short_conv_step)

@@ -15,7 +15,11 @@ KERNEL_TCGEN05, KERNEL_MMA_SYNC, KERNEL_TCGEN05_TWO_TASK = 0, 1, 2
 MAX_CUT_PIECES = 128
 EXPORTS = ["kda_prefill_workspace_bytes", "kda_prefill_workspace_bytes_cuts", "kda_prefill_workspace_clear_bytes", "kda_prefill_launch", "kda_prefill_plan_counts", "kda_prefill_launch_noalloc", "kda_segment_launch", "kda_scan_launch", "kda_scan_strided_launch",
            "kda_fixup_launch", "kda_fixup_tiles_launch", "kda_segment_tiles", "kda_state_rows_copy", "kda_error_string", "kda_abi_struct_bytes", "kda_version",
-           "kda_debug_configure"]
+           "kda_debug_configure", "kda_short_conv_launch", "kda_short_conv_step_launch", "kda_selective_scan_workspace_bytes",
+           "kda_selective_scan_launch", "kda_selective_scan_step_launch", "kda_step_launch", "kda_pool_workspace_bytes",
+           "kda_pool_copy_launch", "kda_pool_fork_launch", "kda_pool_free_launch", "kda_pool_compact_launch"]
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+SCAN_MAX_STATE, MAX_POOLS, MAX_TABLES = 128, 8, 8
 
 
 class KdaPrefillArgs(C.Structure):
@@ -52,6 +56,58 @@ class KdaSegmentArgs(C.Structure):
     ]
 
 
+class KdaSequences(C.Structure):
+    _fields_ = [
+        ("cu_seqlens", C.c_void_p), ("slots", C.c_void_p), ("n_slots", C.c_int64), ("T", C.c_int64), ("status", C.c_void_p),
+        ("cu_is64", C.c_int32), ("slots_is64", C.c_int32), ("N", C.c_int32), ("zero_rest", C.c_int32),
+    ]
+
+
+class KdaConvArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("out", C.c_void_p), ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("ldx", C.c_int64), ("ldo", C.c_int64), ("src_slot_stride", C.c_int64), ("dst_slot_stride", C.c_int64),
+        ("seq", KdaSequences),
+        ("C", C.c_int32), ("W", C.c_int32), ("type", C.c_int32), ("weight_type", C.c_int32), ("silu", C.c_int32),
+    ]
+
+
+class KdaScanArgs(C.Structure):
+    _fields_ = [
+        ("u", C.c_void_p), ("dt", C.c_void_p), ("B", C.c_void_p), ("C", C.c_void_p), ("z", C.c_void_p), ("out", C.c_void_p),
+        ("A", C.c_void_p), ("D", C.c_void_p), ("dt_bias", C.c_void_p), ("src", C.c_void_p), ("dst", C.c_void_p),
+        ("ldu", C.c_int64), ("lddt", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64), ("ldz", C.c_int64),
+        ("ldo", C.c_int64), ("src_slot_stride", C.c_int64), ("dst_slot_stride", C.c_int64),
+        ("seq", KdaSequences),
+        ("Dm", C.c_int32), ("Ns", C.c_int32), ("groups", C.c_int32), ("type", C.c_int32), ("softplus", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class KdaStepArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
+        ("out", C.c_void_p), ("A_log", C.c_void_p), ("dt_bias", C.c_void_p), ("pool", C.c_void_p),
+        ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("ldg", C.c_int64), ("ldbeta", C.c_int64),
+        ("ldo", C.c_int64), ("slot_stride", C.c_int64),
+        ("seq", KdaSequences),
+        ("scale", C.c_float), ("lower_bound", C.c_float), ("frontend", C.c_int32), ("H", C.c_int32),
+    ]
+
+
+class KdaPoolArgs(C.Structure):
+    _fields_ = [
+        ("base", C.c_void_p * MAX_POOLS), ("stride", C.c_int64 * MAX_POOLS), ("bytes", C.c_int64 * MAX_POOLS),
+        ("slots", C.c_int64), ("n_pools", C.c_int32), ("n_tables", C.c_int32), ("used", C.c_void_p), ("src", C.c_void_p),
+        ("dst", C.c_void_p), ("n", C.c_int64), ("src_is64", C.c_int32), ("dst_is64", C.c_int32), ("slots_out", C.c_void_p),
+        ("remap", C.c_void_p), ("tables", C.c_void_p * MAX_TABLES), ("table_n", C.c_int64 * MAX_TABLES),
+        ("table_is64", C.c_int32 * MAX_TABLES), ("status", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+STRUCTS = [KdaPrefillArgs, KdaSegmentArgs, KdaConvArgs, KdaScanArgs, KdaStepArgs, KdaPoolArgs]
 _lib = None
 
 
@@ -101,7 +157,16 @@ def lib():
         L.kda_debug_configure.restype = C.c_int
         L.kda_abi_struct_bytes.argtypes = [C.c_int]
         L.kda_abi_struct_bytes.restype = C.c_size_t
-        if (L.kda_abi_struct_bytes(0) != C.sizeof(KdaPrefillArgs) or L.kda_abi_struct_bytes(1) != C.sizeof(KdaSegmentArgs)):
+        for name, block in (("short_conv", KdaConvArgs), ("short_conv_step", KdaConvArgs), ("selective_scan", KdaScanArgs),
+                            ("selective_scan_step", KdaScanArgs), ("step", KdaStepArgs), ("pool_copy", KdaPoolArgs),
+                            ("pool_fork", KdaPoolArgs), ("pool_free", KdaPoolArgs), ("pool_compact", KdaPoolArgs)):
+            entry = getattr(L, f"kda_{name}_launch")
+            entry.argtypes, entry.restype = [C.POINTER(block), C.c_void_p], C.c_int
+        L.kda_selective_scan_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+        L.kda_selective_scan_workspace_bytes.restype = C.c_size_t
+        L.kda_pool_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
+        L.kda_pool_workspace_bytes.restype = C.c_size_t
+        if any(L.kda_abi_struct_bytes(i) != C.sizeof(block) for i, block in enumerate(STRUCTS)):
             raise RuntimeError("libkda_b200.so and the Python binding disagree on the argument struct layout: rebuild")
         _lib = L
     return _lib

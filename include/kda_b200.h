@@ -231,10 +231,134 @@ int kda_fixup_tiles_launch(void* out, const void* tiles, int64_t n_tiles, int64_
 int kda_state_rows_copy(void* dst, int64_t dst_row_stride, int32_t dst_is_bf16, const float* src,
                         int64_t src_row_stride, const int32_t* idx, int32_t n_rows, int32_t H, void* stream);
 
+/* ---- the operators around the prefill in a recurrent layer.  No counterpart in the reference, which stops at the prefill.
+ * Token tensors are packed as there: [T] rows of one token, ld* = elements between consecutive rows (>= the row), values of a
+ * row consecutive.  16-byte alignment is not needed, but rows that all start on 16 bytes are read fastest.  Written buffers
+ * may not overlap anything else (a state buffer may be source and destination at once).  One kernel launch each. */
+enum { KDA_TYPE_BF16 = 0, KDA_TYPE_FP16 = 1, KDA_TYPE_FP32 = 2 };
+
+/* Further bits of `status` in these calls, which OR them in (the caller clears it): KDA_STATUS_BAD_CU (every sequence taken as
+ * empty, all output rows zero), KDA_STATUS_BAD_SLOT (out of range or a repeat of an earlier entry: that sequence starts from
+ * zeros and its state is not stored), and */
+enum { KDA_STATUS_POOL_FULL = 32 };   /* kda_pool_fork: no slot was left for some entry */
+
+/* Sequences of a batch and the slots of their states. */
+typedef struct KdaSequences {
+  const void* cu_seqlens;  /* device int32/int64 [N+1], or NULL: one sequence [0, T].  Unused in a step: row i is sequence i */
+  const void* slots;       /* device int32/int64 [N], or NULL: sequence i uses slot i.  In a step a negative entry stands for
+                              a row of padding: nothing of it is read, computed or stored */
+  int64_t n_slots;         /* slots of the state buffers (range check; >= N without a table) */
+  int64_t T;               /* token rows; at most 2^31 - 1 */
+  int32_t* status;         /* device int32, or NULL */
+  int32_t cu_is64, slots_is64;
+  int32_t N;               /* sequences; T in a step */
+  int32_t zero_rest;       /* output rows that no sequence owns (behind the last one; padding): 1 = zeros, 0 = left as they are */
+} KdaSequences;
+
+/* Depthwise causal convolution: out[t][c] = act(bias[c] + sum_j weight[c][j] x[t - (W-1) + j][c]), rows in front of a sequence
+ * = its slot's W-1 history rows, which its last W-1 rows replace. */
+typedef struct KdaConvArgs {
+  const void* x;           /* [T][C] */
+  const void* weight;      /* [C][W], packed */
+  const void* bias;        /* [C] of the weight's type, or NULL */
+  void* out;               /* [T][C] */
+  const void* src;         /* [slot][W-1][C] of x's type, oldest row first; NULL = zeros */
+  void* dst;               /* NULL = not stored; may be src.  A step needs src == dst */
+  int64_t ldx, ldo, src_slot_stride, dst_slot_stride;
+  KdaSequences seq;
+  int32_t C, W;            /* W = 2, 3 or 4 */
+  int32_t type, weight_type;   /* KDA_TYPE_*: of x, out and history; of weight and bias */
+  int32_t silu;            /* 1: act(y) = y / (1 + exp(-y)) */
+} KdaConvArgs;
+int kda_short_conv_launch(const KdaConvArgs* args, void* stream);
+int kda_short_conv_step_launch(const KdaConvArgs* args, void* stream);
+
+/* Selective state space scan, per channel d with state values h[0..Ns-1] (fp32):
+ *   s = dt + dt_bias (softplus of it with `softplus`);  h[n] = exp(s A[d][n]) h[n] + s u B[g][n];
+ *   out = (sum_n C[g][n] h[n] + D[d] u) (times z / (1 + exp(-z)) with z),   g = d / (Dm / groups) */
+typedef struct KdaScanArgs {
+  const void *u, *dt;      /* [T][Dm] */
+  const void *B, *C;       /* [T][groups][Ns], packed rows */
+  const void* z;           /* [T][Dm] or NULL */
+  void* out;               /* [T][Dm]; all of one type */
+  const float* A;          /* [Dm][Ns], packed */
+  const float* D;          /* [Dm] or NULL */
+  const float* dt_bias;    /* [Dm] or NULL */
+  const float* src;        /* [slot][Dm][Ns]; NULL = zeros */
+  float* dst;              /* NULL = not stored; may be src.  A step needs src == dst */
+  int64_t ldu, lddt, ldb, ldc, ldz, ldo, src_slot_stride, dst_slot_stride;
+  KdaSequences seq;
+  int32_t Dm, Ns, groups;  /* Ns <= KDA_SCAN_MAX_STATE; groups divides Dm */
+  int32_t type, softplus;
+  void* workspace;         /* kda_selective_scan_workspace_bytes(..) bytes, 16-byte aligned; contents need not survive, but
+                              concurrent calls must not share it.  May be NULL where that is 0.  Unused in a step */
+  size_t workspace_bytes;
+} KdaScanArgs;
+#define KDA_SCAN_MAX_STATE 128
+size_t kda_selective_scan_workspace_bytes(int64_t T, int32_t N, int32_t Dm, int32_t Ns);
+int kda_selective_scan_launch(const KdaScanArgs* args, void* stream);
+int kda_selective_scan_step_launch(const KdaScanArgs* args, void* stream);
+
+/* One token of the KDA recurrence for each row; front-ends as in kda_prefill_launch, the state value first with the raw one and
+ * key first with the plain one (no L2 norm of q, k there).  Token tensors need no alignment; the pool 16-byte aligned, its slot
+ * stride a multiple of 4. */
+typedef struct KdaStepArgs {
+  const void *q, *k, *v;   /* bf16 [T][H][128] */
+  const void *g, *beta;    /* [T][H][128], [T][H]: bf16 (raw) or fp32 (plain) */
+  void* out;               /* bf16 [T][H][128] */
+  const float* A_log;      /* [H]      raw front-end only */
+  const float* dt_bias;    /* [H*128]  raw front-end only */
+  float* pool;             /* [slot][H][128][128], updated in place */
+  int64_t ldq, ldk, ldv, ldg, ldbeta, ldo, slot_stride;
+  KdaSequences seq;
+  float scale, lower_bound;
+  int32_t frontend, H;
+} KdaStepArgs;
+int kda_step_launch(const KdaStepArgs* args, void* stream);
+
+/* Upkeep of pools that share one table of slots (states, convolution histories, ...).  Row s of pool k: bytes [base[k] +
+ * s * stride[k], + bytes[k]).  Two launches (kda_pool_free_launch: one); nothing is read on the host. */
+#define KDA_MAX_POOLS 8
+#define KDA_MAX_TABLES 8
+typedef struct KdaPoolArgs {
+  void* base[KDA_MAX_POOLS];
+  int64_t stride[KDA_MAX_POOLS], bytes[KDA_MAX_POOLS];
+  int64_t slots;           /* P, of every pool; at most 2^31 - 1 */
+  int32_t n_pools;
+  int32_t n_tables;        /* compact: tables to rewrite */
+  uint8_t* used;           /* device [P]: 0 = free (not for copy) */
+  const void* src;         /* device [n]: copy: source slots, negative = zeros; fork: parents, negative = none (zeros); free: slots,
+                              negative = padding */
+  const void* dst;         /* device [n]: copy: destination slots, negative = padding */
+  int64_t n;               /* entries of src / dst */
+  int32_t src_is64, dst_is64;
+  int32_t* slots_out;      /* fork: device [n], the new slots (-1: none) */
+  int32_t* remap;          /* compact: device [P], where each slot went (-1: was free) */
+  void* tables[KDA_MAX_TABLES];        /* compact: device slot tables, int32/int64, rewritten in place (negative: left alone) */
+  int64_t table_n[KDA_MAX_TABLES];
+  int32_t table_is64[KDA_MAX_TABLES];
+  int32_t* status;         /* device int32, or NULL */
+  void* workspace;         /* kda_pool_workspace_bytes(n, P) bytes, 4-byte aligned (not for free) */
+  size_t workspace_bytes;
+} KdaPoolArgs;
+size_t kda_pool_workspace_bytes(int64_t n, int64_t P);
+/* dst[i] <- src[i].  Entries out of range, and destinations that an earlier entry names or any entry reads, are left out
+ * (KDA_STATUS_BAD_SLOT). */
+int kda_pool_copy_launch(const KdaPoolArgs* args, void* stream);
+/* Each entry, in order, takes the lowest free slot, marks it used and fills it with its parent's rows.  A parent that is out of
+ * range or was not in use before the call: no slot, KDA_STATUS_BAD_SLOT.  None left: KDA_STATUS_POOL_FULL. */
+int kda_pool_fork_launch(const KdaPoolArgs* args, void* stream);
+/* Marks slots free.  One that is out of range, free already or named before: KDA_STATUS_BAD_SLOT. */
+int kda_pool_free_launch(const KdaPoolArgs* args, void* stream);
+/* With m slots in use, moves those behind the first m, in order, into the holes among them: `used` becomes m ones and P - m
+ * zeros.  Entries of a table that name no slot in use become -1 (KDA_STATUS_BAD_SLOT). */
+int kda_pool_compact_launch(const KdaPoolArgs* args, void* stream);
+
 /* Text of a KDA_ERR_* code; for KDA_ERR_LAUNCH the last CUDA error string seen by this thread. */
 const char* kda_error_string(int code);
 
-/* sizeof(KdaPrefillArgs) (which = 0) or sizeof(KdaSegmentArgs) (which = 1) as the library was compiled: lets a foreign
+/* sizeof of KdaPrefillArgs (which = 0), KdaSegmentArgs (1), KdaConvArgs (2), KdaScanArgs (3), KdaStepArgs (4) or KdaPoolArgs (5)
+ * as the library was compiled: lets a foreign
  * binding check its struct layout before the first call. */
 size_t kda_abi_struct_bytes(int which);
 

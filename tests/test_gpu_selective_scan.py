@@ -1,0 +1,299 @@
+"""selective_scan and selective_scan_step against the definition in 64 bits, with a running error bound: types, state sizes, groups,
+odd channels, strides, lengths from none to long, tables that are wrong, padding, captured calls."""
+import math
+
+import pytest
+import torch
+
+from serving_testlib import DEV, assert_within, cu_of, generator, randn, scan64
+
+pytestmark = pytest.mark.gpu
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+
+def make(gen, T, Dm, Ns, G, dtype, gate=True, slow=False):
+    A = -torch.arange(1, Ns + 1, device=DEV) * torch.exp(randn(gen, Dm, Ns, scale=0.3))
+    step = torch.exp(torch.rand(Dm, generator=gen, device=DEV) * math.log(100.0) + math.log(1e-4 if slow else 1e-3))
+    return dict(u=randn(gen, 1, T, Dm, dtype=dtype), dt=randn(gen, 1, T, Dm, dtype=dtype, scale=0.5), A=A, B=randn(gen, 1, T, G, Ns, dtype=dtype),
+                C=randn(gen, 1, T, G, Ns, dtype=dtype), D=randn(gen, Dm), z=randn(gen, 1, T, Dm, dtype=dtype) if gate else None,
+                dt_bias=step + torch.log(-torch.expm1(-step)))
+
+
+def at(a, rows):
+    return {n: t[:, rows] if t is not None and n in ("u", "dt", "B", "C", "z") else t for n, t in a.items()}
+
+
+def check(a, init, lens, y, final, softplus=True, what=""):
+    t = 0
+    for i, n in enumerate(lens):
+        s = at(a, slice(t, t + n))
+        want, bound, h, E = scan64(s["u"][0], s["dt"][0], a["A"], s["B"][0], s["C"][0], a["D"], s["z"][0] if s["z"] is not None else None,
+                                   a["dt_bias"], init[i], softplus)
+        assert_within(y[0, t:t + n], want, bound, f"{what} sequence {i}")
+        assert_within(final[i], h, E, f"{what} state {i}")
+        t += n
+
+
+@pytest.mark.parametrize("dtype,Dm,Ns,G,lens,gate", [
+    (BF, 256, 16, 1, [77], True), (BF, 200, 16, 2, [1, 0, 33, 64, 65, 2], True), (HF, 129, 13, 1, [40, 0, 3], False), (F, 64, 4, 4, [1], True),
+    (F, 96, 8, 1, [130, 31], False), (BF, 64, 32, 2, [70, 5], True), (F, 36, 64, 1, [50], True), (HF, 24, 128, 3, [35, 1], True),
+    (F, 1, 16, 1, [300], True), (BF, 1000, 16, 1, [1] * 20, True), (F, 33, 1, 1, [0, 9, 0], True), (F, 40, 100, 1, [20], False)])
+@pytest.mark.parametrize("pooled", [False, True])
+def test_prompts(dtype, Dm, Ns, G, lens, gate, pooled):
+    import kda_b200
+    gen, N = generator(Dm + Ns), len(lens)
+    a = make(gen, sum(lens), Dm, Ns, G, dtype, gate)
+    if pooled:
+        pool = randn(gen, N + 3, Dm, Ns)
+        slots = torch.randperm(N + 3, generator=torch.Generator().manual_seed(3))[:N].to(DEV)
+        before, status = pool.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+        y, got = kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu_of(lens), ssm_state_indices=slots, status=status)
+        assert got is pool and int(status) == 0
+        check(a, before[slots], lens, y, pool[slots])
+        rest = [i for i in range(N + 3) if i not in slots.tolist()]
+        assert torch.equal(pool[rest], before[rest])
+    else:
+        init = randn(gen, N, Dm, Ns)
+        keep = init.clone()
+        y, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of(lens, torch.int32))
+        assert torch.equal(init, keep)
+        check(a, init, lens, y, final)
+        y, final = kda_b200.selective_scan(**a, cu_seqlens=cu_of(lens))
+        check(a, torch.zeros_like(init), lens, y, final)
+
+
+@pytest.mark.parametrize("Dm,T,dtype", [(16, 5000, F), (512, 3000, HF), (96, 2049, BF), (7, 4097, F)])
+@pytest.mark.parametrize("slow", [False, True])
+def test_long_axes_on_few_channels(Dm, T, dtype, slow):
+    import kda_b200
+    gen = generator(T)
+    a = make(gen, T, Dm, 16, 1, dtype, True, slow)
+    lens = [T - 700, 1, 0, 699]
+    init = randn(gen, 4, Dm, 16)
+    y, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of(lens))
+    check(a, init, lens, y, final)
+    y, final = kda_b200.selective_scan(**a, initial_state=init[:1])
+    check(a, init[:1], [T], y, final)
+
+
+@pytest.mark.parametrize("leave", ["D", "z", "dt_bias", "all"])
+def test_what_may_be_left_out(leave):
+    import kda_b200
+    gen = generator(12)
+    a = make(gen, 50, 72, 16, 1, BF)
+    for n in ("D", "z", "dt_bias"):
+        if leave in (n, "all"):
+            a[n] = None
+    y, final = kda_b200.selective_scan(**a)
+    check(a, torch.zeros(1, 72, 16, device=DEV), [50], y, final)
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_step_sizes_as_given_growing_states_and_hard_decays(step):
+    """Without the softplus a step may be negative (the state grows); step sizes and rates whose decay underflows; none at all."""
+    import kda_b200
+    gen = generator(13)
+    a = make(gen, 40, 48, 16, 1, F)
+    a["dt"] = a["dt"] * 0.3
+    a["dt_bias"] = None
+    a["A"][:4] = -1e4
+    a["dt"][:, 10:14] = 0.0
+    init = randn(gen, 40 if step else 1, 48, 16)
+    if step:
+        pool = init.clone()
+        y, _ = kda_b200.selective_scan_step(**{n: a[n] for n in ("u", "dt", "A", "B", "C", "D", "z", "dt_bias")}, pool=pool, dt_softplus=False)
+        keep = torch.ones(48, dtype=torch.bool, device=DEV)
+        keep[:4] = False                                              # those overflow where the step is negative
+        part = {n: (t[..., keep] if n in ("u", "dt", "z") else t[keep] if n in ("A", "D") else t) if t is not None else None for n, t in a.items()}
+        check(part, init[:, keep], [1] * 40, y[..., keep], pool[:, keep], False)
+        return
+    a["dt"][..., :4] = a["dt"][..., :4].abs()
+    y, final = kda_b200.selective_scan(**a, initial_state=init, dt_softplus=False)
+    check(a, init, [40], y, final, False)
+
+
+def test_large_and_small_step_logits():
+    """softplus over its whole range: e^x far below fp32's step at one, x itself far above."""
+    import kda_b200
+    gen = generator(14)
+    a = make(gen, 64, 32, 16, 1, F)
+    a["dt"] = torch.linspace(-80.0, 40.0, 64 * 32, device=DEV).view(1, 64, 32)[:, torch.randperm(64, generator=torch.Generator().manual_seed(1)).to(DEV)]
+    a["dt_bias"] = None
+    y, final = kda_b200.selective_scan(**a)
+    check(a, torch.zeros(1, 32, 16, device=DEV), [64], y, final)
+
+
+@pytest.mark.parametrize("off", [0, 1, 8])
+def test_views_are_read_and_written_in_place(off):
+    import kda_b200
+    gen, lens = generator(15), [40, 25]
+    a = make(gen, 65, 256, 16, 1, BF)
+    wide = randn(gen, 1, 65, 1200, dtype=BF)
+    a["u"], a["z"], a["dt"] = wide[:, :, off:off + 256], wide[:, :, 300 + off:556 + off], wide[:, :, 600 + off:856 + off] * 0.5
+    xbc = randn(gen, 1, 65, 1, 50, dtype=BF)
+    a["B"], a["C"] = xbc[..., off:off + 16], xbc[..., 20 + off:36 + off]
+    target = torch.full((1, 70, 512), 7.0, dtype=BF, device=DEV)
+    y, final = kda_b200.selective_scan(**a, cu_seqlens=cu_of(lens), out=target[:, 2:67, off:off + 256])
+    check(a, torch.zeros(2, 256, 16, device=DEV), lens, y, final)
+    rest = target.clone()
+    rest[:, 2:67, off:off + 256] = 7.0
+    assert bool((rest == 7.0).all())
+
+
+def test_rows_behind_the_last_sequence():
+    import kda_b200
+    gen, lens = generator(16), [10, 60]
+    a = make(gen, 100, 136, 16, 1, BF)
+    for n in ("u", "dt", "B", "C", "z"):
+        a[n][:, 70:] = float("nan")
+    y, final = kda_b200.selective_scan(**a, cu_seqlens=cu_of(lens))
+    check(a, torch.zeros(2, 136, 16, device=DEV), lens, y, final)
+    assert bool((y[:, 70:] == 0).all())
+    out = torch.full_like(y, 3.0)
+    kda_b200.selective_scan(**a, cu_seqlens=cu_of(lens), out=out)
+    assert torch.equal(out[:, :70], y[:, :70]) and bool((out[:, 70:] == 3.0).all())
+
+
+def test_a_neighbour_that_is_not_a_number_stays_there():
+    import kda_b200
+    gen, lens = generator(17), [32, 33, 31]
+    a = make(gen, 96, 40, 16, 1, F)
+    pool = randn(gen, 5, 40, 16)
+    for n in ("u", "dt", "B", "C", "z"):
+        a[n][:, :32] = float("nan")
+    pool[[0, 2]] = float("inf")
+    before, slots = pool.clone(), torch.tensor([0, 3, 1], device=DEV)
+    y, _ = kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu_of(lens), ssm_state_indices=slots)
+    check(at(a, slice(32, 96)), before[slots[1:]], lens[1:], y[:, 32:], pool[slots[1:]])
+    assert bool(torch.isinf(pool[2]).all()) and torch.equal(pool[4], before[4])
+
+
+@pytest.mark.parametrize("bad", [[0, 40, 30, 60], [1, 20, 40, 60], [0, 20, 40, 61]])
+def test_a_rejected_layout(bad):
+    import kda_b200
+    gen = generator(18)
+    a = make(gen, 60, 64, 16, 1, BF)
+    pool = randn(gen, 3, 64, 16)
+    before, status, out = pool.clone(), torch.zeros(1, dtype=torch.int32, device=DEV), torch.full((1, 60, 64), 3.0, dtype=BF, device=DEV)
+    cu = torch.tensor(bad, device=DEV)
+    kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu, ssm_state_indices=torch.arange(3, device=DEV), out=out, status=status)
+    assert int(status) == 1 and bool((out == 0).all()) and torch.equal(pool, before)
+    _, final = kda_b200.selective_scan(**a, initial_state=before, cu_seqlens=cu)
+    assert torch.equal(final, before)
+
+
+def test_slots_out_of_range_or_named_twice():
+    import kda_b200
+    gen, n = generator(19), 6
+    a = make(gen, 5 * n, 64, 16, 1, F)
+    pool = randn(gen, n, 64, 16)
+    before, status = pool.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    slots = torch.tensor([0, n, -1, 0, 4, 5], device=DEV, dtype=torch.int32)
+    y, _ = kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu_of([5] * n), ssm_state_indices=slots, status=status)
+    assert int(status) == 2 and torch.equal(pool[1:4], before[1:4])
+    init = before.clone()
+    init[1:4] = 0
+    _, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of([5] * n))
+    final[[0, 4, 5]] = pool[[0, 4, 5]]
+    check(a, init, [5] * n, y, final)
+
+
+@pytest.mark.parametrize("dtype,Dm,Ns,G,rows", [(BF, 4096, 16, 1, 3), (F, 1000, 16, 1, 1), (HF, 72, 13, 2, 40), (BF, 64, 64, 1, 7), (F, 24, 128, 3, 5),
+                                                (BF, 100, 8, 4, 9), (F, 3, 1, 1, 2), (HF, 256, 32, 1, 300)])
+@pytest.mark.parametrize("pad", [0, 2])
+def test_single_tokens(dtype, Dm, Ns, G, rows, pad):
+    import kda_b200
+    gen, N = generator(rows + Dm), rows + pad
+    a = make(gen, N, Dm, Ns, G, dtype)
+    pool = randn(gen, N + 2, Dm, Ns)
+    before = pool.clone()
+    slots = torch.randperm(N + 2, generator=torch.Generator().manual_seed(3))[:N].to(torch.int32).to(DEV)
+    if pad:
+        slots[1 if rows > 1 else 0] = -1
+        slots[-1] = -7
+        a["u"][0, -1] = float("nan")
+    live = [i for i in range(N) if int(slots[i]) >= 0]
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    y, got = kda_b200.selective_scan_step(**a, pool=pool, ssm_state_indices=slots, status=status)
+    assert got is pool and int(status) == 0
+    ids = slots[live].long()
+    some = live[:12]
+    check(at(a, some), before[ids[:12]], [1] * len(some), y[:, some], pool[ids[:12]])
+    whole = before.clone()
+    y2, final = kda_b200.selective_scan(**at(a, live), initial_state=whole[ids].contiguous(), cu_seqlens=cu_of([1] * len(live)))
+    torch.testing.assert_close(y[:, live].float(), y2.float(), rtol=2 ** -7, atol=1e-4)
+    torch.testing.assert_close(pool[ids], final, rtol=1e-5, atol=1e-5)
+    dead = [i for i in range(N) if i not in live]
+    assert bool((y[0, dead] == 0).all())
+    rest = [i for i in range(N + 2) if i not in ids.tolist()]
+    assert torch.equal(pool[rest], before[rest])
+    out, again = torch.full_like(y, 3.0), before.clone()
+    kda_b200.selective_scan_step(**a, pool=again, ssm_state_indices=slots, out=out)
+    assert torch.equal(out[0, live], y[0, live]) and bool((out[0, dead] == 3.0).all()) and torch.equal(again, pool)
+
+
+def test_single_tokens_with_a_slot_named_twice():
+    import kda_b200
+    gen = generator(20)
+    a, pool = make(gen, 4, 64, 16, 1, F), randn(gen, 3, 64, 16)
+    before, status = pool.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    y, _ = kda_b200.selective_scan_step(**a, pool=pool, ssm_state_indices=torch.tensor([2, 0, 2, 3], device=DEV), status=status)
+    assert int(status) == 2 and torch.equal(pool[1], before[1])
+    init = torch.stack([before[2], before[0], torch.zeros_like(before[0]), torch.zeros_like(before[0])])
+    _, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of([1] * 4))
+    check(a, init, [1] * 4, y, torch.stack([pool[2], pool[0], final[2], final[3]]))
+
+
+def test_captured_calls_follow_their_tables():
+    import kda_b200
+    gen, N, T = generator(21), 6, 90
+    a, pool = make(gen, T, 96, 16, 1, BF), randn(gen, 9, 96, 16)
+    tok = make(gen, N, 96, 16, 1, BF)
+    tok["A"], tok["D"], tok["dt_bias"] = a["A"], a["D"], a["dt_bias"]
+    cu, slots, step_slots = cu_of([15] * N), torch.arange(N, device=DEV), torch.arange(N, device=DEV)
+    kda_b200.selective_scan(**a, initial_state=pool.clone(), cu_seqlens=cu, ssm_state_indices=slots)
+    torch.cuda.synchronize()
+    prompt, token = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(prompt):
+        y, _ = kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu, ssm_state_indices=slots)
+    with torch.cuda.graph(token):
+        ys, _ = kda_b200.selective_scan_step(**tok, pool=pool, ssm_state_indices=step_slots)
+    for lens, ids in (([15] * N, [0, 1, 2, 3, 4, 5]), ([1, 0, 40, 2, 30, 0], [8, 2, 7, 1, 0, 5]), ([90, 0, 0, 0, 0, 0], [3, 4, 5, 6, 7, 8])):
+        cu.copy_(cu_of(lens))
+        slots.copy_(torch.tensor(ids))
+        step_slots.copy_(torch.tensor(ids[:4] + [-1, -1]))
+        a["u"].normal_()
+        before = pool.clone()
+        prompt.replay()
+        check(a, before[slots], lens, y, pool[slots])
+        middle = pool.clone()
+        token.replay()
+        check(at(tok, slice(0, 4)), middle[slots[:4]], [1] * 4, ys[:, :4], pool[slots[:4]])
+        assert bool((ys[:, 4:] == 0).all())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z, final = kda_b200.selective_scan(**a, cu_seqlens=cu)
+    side.synchronize()
+    check(a, torch.zeros(N, 96, 16, device=DEV), [90, 0, 0, 0, 0, 0], z, final)
+
+
+def test_offsets_behind_32_bits():
+    import kda_b200
+    Dm, T = 8192, 270_000
+    gen = generator(22)
+    a = make(gen, 40, Dm, 16, 1, BF)
+    far = {n: torch.zeros(1, T, *t.shape[2:], dtype=BF, device=DEV) for n, t in a.items() if n in ("u", "dt", "B", "C")}
+    for n in far:
+        far[n][:, -40:] = a[n]
+    big = dict(a, **far, z=None)
+    lens = [T - 40, 40]
+    y, final = kda_b200.selective_scan(**big, cu_seqlens=cu_of(lens))
+    check(dict(a, z=None), torch.zeros(1, Dm, 16, device=DEV), [40], y[:, -40:], final[1:])
+    assert bool((y[:, :100] == 0).all())
+    del big, far, y
+    pool = torch.zeros(17_000, Dm, 16, device=DEV)                   # slots up to 2.2e9 values
+    tok = at(a, slice(0, 2))
+    y, _ = kda_b200.selective_scan_step(**tok, pool=pool, ssm_state_indices=torch.tensor([16_999, 3], device=DEV))
+    check(tok, torch.zeros(2, Dm, 16, device=DEV), [1, 1], y, pool[[16_999, 3]])
+    assert int((pool != 0).any(-1).any(-1).sum()) == 2
