@@ -518,6 +518,15 @@ int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
   p.seq = seq_table(a->seq);
   p.ldu = a->ldu; p.lddt = a->lddt; p.ldb = a->ldb; p.ldc = a->ldc; p.ldz = a->ldz; p.ldo = a->ldo;
   p.src_stride = a->src_slot_stride; p.dst_stride = a->dst_slot_stride;
+  if (!step) {
+    p.piece = (int)kda::sscan_piece(a->seq.T, a->seq.N, a->Dm, a->Ns);
+    if (p.piece > 0) {
+      if (!a->workspace || !aligned16(a->workspace)) return KDA_ERR_ARG;
+      if (a->workspace_bytes < kda_selective_scan_workspace_bytes(a->seq.T, a->seq.N, a->Dm, a->Ns)) return KDA_ERR_WORKSPACE;
+      p.ws_state = reinterpret_cast<float*>(a->workspace);
+      p.ws_sum = p.ws_state + (a->seq.T / p.piece + a->seq.N) * rows;
+    }
+  }
   p.Dm = a->Dm; p.Ns = a->Ns; p.groups = a->groups; p.softplus = a->softplus != 0; p.zero_pad = a->seq.zero_rest != 0;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return launched(step ? kda::launch_sscan_step(p, a->type, s) : kda::launch_sscan(p, a->type, s));
@@ -558,8 +567,10 @@ int kda_short_conv_launch(const KdaConvArgs* a, void* stream) { return conv_laun
 int kda_short_conv_step_launch(const KdaConvArgs* a, void* stream) { return conv_launch(a, true, stream); }
 
 size_t kda_selective_scan_workspace_bytes(int64_t T, int32_t N, int32_t Dm, int32_t Ns) {
-  (void)T; (void)N; (void)Dm; (void)Ns;
-  return 0;
+  if (T < 0 || N < 1 || Dm < 1 || Ns < 1 || Ns > KDA_SCAN_MAX_STATE) return 0;
+  const long long piece = kda::sscan_piece(T, N, Dm, Ns);
+  if (piece == 0) return 0;
+  return sizeof(float) * (size_t)(T / piece + N) * Dm * (Ns + 1);
 }
 int kda_selective_scan_launch(const KdaScanArgs* a, void* stream) { return scan_launch(a, false, stream); }
 int kda_selective_scan_step_launch(const KdaScanArgs* a, void* stream) { return scan_launch(a, true, stream); }

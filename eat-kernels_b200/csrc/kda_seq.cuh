@@ -92,12 +92,15 @@ __device__ __forceinline__ Pack<T, VEC> pack(const float (&f)[VEC]) {
   return p;
 }
 
-// x / (1 + e^-x): the approximate exponential and quotient are off by some 2^-21, which 16-bit outputs do not show; 32-bit
+// x / (1 + e^-x): the approximate exponential and reciprocal are off by some 2^-21, which 16-bit outputs do not show; 32-bit
 // ones take the exact functions.
 template <typename T>
 __device__ __forceinline__ float silu(float x) {
   if constexpr (sizeof(T) == 4) return x / (1.0f + expf(-x));
-  return __fdividef(x, 1.0f + __expf(-x));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return x * r;
 }
 
 }  // namespace kda

@@ -3,45 +3,54 @@
 //
 // What bounds it: one exponential a token, channel and state value, 16 a clock and SM in the special-function unit, which is
 // two to three times the time of the tokens' bytes.  So everything else is kept away from that unit and from the instruction
-// stream of the warps that feed it:
-//   * a block has four scan warps, one a scheduler, and four helper warps.  The helpers load the tokens, work out the step
-//     sizes, s u, D u and the gate, and write the outputs; the scan warps only see shared memory.  Two stages of tokens
-//     between them, handed over by named barriers.
-//   * a channel's state lies over L lanes, S values each; the products run two values an instruction.  Sums over the lanes are
-//     taken for L tokens at once, each step of the exchange halving the tokens a lane holds (L - 1 exchanges for L tokens).
+// stream and the shared memory of the warps that feed it:
+//   * a block has eight scan warps and four helper warps.  The helpers load the tokens, work out the step sizes, s u, D u and
+//     the gate, and write the outputs; the scan warps only see shared memory.  Two stages of tokens between them, handed over
+//     by named barriers.  A warp by itself issues every third cycle at best (fp32 multiply-adds that do not depend on one
+//     another: 2.7 cycles), so a state is spread over as many warps as keep their instruction count.
+//   * shared memory holds time rows: a lane takes four tokens in one access, and all products but the chain itself run two
+//     tokens an instruction, without a value copied to make a pair.
+//   * a channel's state lies over L lanes, S values each.  Sums over the lanes are taken for a group of tokens at once, each
+//     step of the exchange halving the tokens that a lane holds.
 #include "kda_serving.cuh"
 
 namespace kda {
 
 namespace {
 
-constexpr int SCAN_LANES = 128;          // scan threads of a block, and as many helpers
-constexpr int SCAN_THREADS = 2 * SCAN_LANES;
-constexpr int TILE = 32;                 // tokens a stage
+constexpr int SCAN_LANES = 256;          // scan threads of a block
+constexpr int HELPERS = 128;
+constexpr int SCAN_THREADS = SCAN_LANES + HELPERS;
+constexpr int STEP_LANES = 128;          // threads of a single token's block
+constexpr int TILE = 16;                 // tokens a stage
+constexpr int QUADS = TILE / 4;
 constexpr float LOG2E_F = 1.4426950408889634f;
 
-// Polynomials by minimax (Remez exchange) of the relative error, coefficients rounded to fp32: 1.8e-7 off with the roundings.
-__device__ __forceinline__ float log1p_unit(float e) {     // log(1 + e), e in [0, 1]
-  float p = 0.0052326940931379795f;
-  p = fmaf(p, e, -0.02950523979961872f);
-  p = fmaf(p, e, 0.07822595536708832f);
-  p = fmaf(p, e, -0.13663245737552643f);
-  p = fmaf(p, e, 0.19106006622314453f);
-  p = fmaf(p, e, -0.2484298199415207f);
-  p = fmaf(p, e, 0.3331909775733948f);
-  p = fmaf(p, e, -0.4999949336051941f);
-  p = fmaf(p, e, 0.9999999403953552f);
-  return p * e;
+// log(1 + e) / e for e in [0, 1]: minimax polynomial (Remez exchange) of the relative error, coefficients rounded to fp32;
+// 1.8e-7 off with its roundings.
+__host__ __device__ constexpr float log1p_coef(int k) {
+  constexpr float c[9] = {0.9999999403953552f,  -0.4999949336051941f,  0.3331909775733948f,  -0.2484298199415207f, 0.19106006622314453f,
+                          -0.13663245737552643f, 0.07822595536708832f, -0.02950523979961872f, 0.0052326940931379795f};
+  return c[k];
 }
 __device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; below 2^-126 zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// max(x, 0) + log(1 + exp(-|x|)); NaN stays
+// max(x, 0) + log(1 + exp(-|x|)); NaN stays, by the second term
 __device__ __forceinline__ float softplus(float x) {
   const float e = exp2_fast(-fabsf(x) * LOG2E_F);
-  return x != x ? x : fmaxf(x, 0.0f) + log1p_unit(e);
+  float q = log1p_coef(8);
+#pragma unroll
+  for (int k = 7; k >= 0; k--) q = fmaf(q, e, log1p_coef(k));
+  return fmaxf(x, 0.0f) + q * e;
+}
+
+// A in powers of two; finite, since -inf times a step of zero (behind the last token) would be NaN
+__device__ __forceinline__ float decay_rate(float a) {
+  a *= LOG2E_F;
+  return a < -3.0e38f ? -3.0e38f : a;
 }
 
 // two fp32 values an instruction
@@ -63,224 +72,471 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
+// of two values, the polynomial for both at once
+__device__ __forceinline__ F2 softplus2(float x, float y) {
+  const F2 e = f2(exp2_fast(-fabsf(x) * LOG2E_F), exp2_fast(-fabsf(y) * LOG2E_F));
+  F2 q = f2(log1p_coef(8), log1p_coef(8));
+#pragma unroll
+  for (int k = 7; k >= 0; k--) q = fma2(q, e, f2(log1p_coef(k), log1p_coef(k)));
+  float p0, p1;
+  split(mul2(q, e), p0, p1);
+  return f2(fmaxf(x, 0.0f) + p0, fmaxf(y, 0.0f) + p1);
+}
+
 __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(SCAN_THREADS) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(SCAN_THREADS) : "memory"); }
-enum { BAR_FULL = 1, BAR_DONE = 3 };     // + stage
+enum { BAR_FULL = 1, BAR_DONE = 3, BAR_HELPERS = 5 };     // FULL, DONE: + stage
 
-template <int S>
-struct Values {
-  float v[S];
+// Tokens as they lie in memory, on their way to the helpers: rows of time, for DEPTH tiles.
+template <typename T, int L, int S>
+struct RawShared {
+  static constexpr int DEPTH = sizeof(T) == 4 ? 3 : 4;                   // what lets two blocks share an SM
+
+  // rows of whole 16 bytes; 16-bit rows four apart fall into different halves of the banks
+  static constexpr int XS = SCAN_LANES / L + 8, NS = L * S + 8;
+  T x[DEPTH][3][TILE][XS];                           // u, dt, z
+  T bc[DEPTH][2][TILE][NS];
 };
-// S consecutive values of shared memory, in one access
-template <int S>
-__device__ __forceinline__ Values<S> load_values(const float* p) {
-  Values<S> r;
-  if constexpr (S == 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    r.v[0] = f.x; r.v[1] = f.y; r.v[2] = f.z; r.v[3] = f.w;
-  } else if constexpr (S == 2) {
-    const float2 f = *reinterpret_cast<const float2*>(p);
-    r.v[0] = f.x; r.v[1] = f.y;
-  } else {
-    r.v[0] = *p;
-  }
-  return r;
-}
 
 template <int L, int S>
 struct ScanShared {
   static constexpr int CB = SCAN_LANES / L;          // channels of a block
+  static_assert(CB >= 8 && L * S <= 128, "layouts");
   static constexpr int NP = L * S;                   // state values, padded
-  static constexpr int YS = CB + CB / 4;             // row of outputs: L rows of a warp's channels fall into different banks
-  float2 step[2][TILE][CB];                          // s, s u
-  float b[2][TILE][NP], c[2][TILE][NP];
-  float y[2][TILE][YS];                              // D u, then the outputs without the gate
-  float gate[2][TILE][CB];
+  // a row of time, both stages: eight rows' 16 bytes at one time fall into different banks
+  static constexpr int R = 2 * TILE + 4;
+  float step[CB][R], input[CB][R];                   // s, s u
+  float y[CB][R];                                    // sums of C h
+  float skip[CB][R], gate[CB][R];                    // D u, silu(z)
+  float b[NP][R], c[NP][R];
 };
 
 struct Work {                                        // a block's share
   int group, d0, channels;                           // group of channels, first channel, how many
-  long long begin, end;                              // tokens
+  int seq, piece, pieces, at;                        // sequence, which of its pieces, how many it has, piece of the launch
+  int tokens;
+  long long begin;                                   // first token
 };
 
-// The helpers' half: tokens in, outputs out.
-template <typename T, int L, int S>
-__device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanShared<L, S>& sh, int tid) {
-  using Sh = ScanShared<L, S>;
-  constexpr int CB = Sh::CB, NP = Sh::NP, E = TILE * CB / SCAN_LANES, EB = TILE * NP / SCAN_LANES;
-  constexpr int ROWS = SCAN_LANES / CB;              // tokens that the helpers cover at a time
-  const int c = tid % CB, row = tid / CB;
-  const bool mine = c < w.channels;
-  const int d = w.d0 + (mine ? c : 0);
-  const float skip = p.D != nullptr ? p.D[d] : 0.0f, bias = p.dt_bias != nullptr ? p.dt_bias[d] : 0.0f;
-  const T* u = reinterpret_cast<const T*>(p.u) + d;
-  const T* dt = reinterpret_cast<const T*>(p.dt) + d;
-  const T* z = reinterpret_cast<const T*>(p.z) + d;
-  const T* B = reinterpret_cast<const T*>(p.B) + (long long)w.group * p.Ns;
-  const T* C = reinterpret_cast<const T*>(p.C) + (long long)w.group * p.Ns;
-  T* out = reinterpret_cast<T*>(p.out) + d;
-  const int n = tid % NP, brow = tid / NP;           // NP divides the helpers' number
-  constexpr int BROWS = SCAN_LANES / NP;
-  const bool has_z = p.z != nullptr, state_in = n < p.Ns;
+constexpr int RANKED = 128;                          // up to so many sequences the longest goes first
 
-  T ru[E], rdt[E], rz[E], rb[EB], rc[EB];
-  const T none = from_float<T>(0.0f);
-  auto load = [&](long long t0) {
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const long long t = t0 + row + e * ROWS;
-      const bool on = mine && t < w.end;
-      ru[e] = on ? u[t * p.ldu] : none;
-      rdt[e] = on ? dt[t * p.lddt] : none;
-      rz[e] = on && has_z ? z[t * p.ldz] : none;
-    }
-#pragma unroll
-    for (int e = 0; e < EB; e++) {
-      const long long t = t0 + brow + e * BROWS;
-      const bool on = state_in && t < w.end;
-      rb[e] = on ? B[t * p.ldb + n] : none;
-      rc[e] = on ? C[t * p.ldc + n] : none;
-    }
-  };
-  auto store = [&](long long t0, int stage) {
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int j = row + e * ROWS;
-      if (mine && t0 + j < w.end) out[(t0 + j) * p.ldo] = from_float<T>(sh.y[stage][j][c] * sh.gate[stage][j][c]);
-    }
-  };
+// Pieces that a sequence is cut into (empty sequences have one, for their state).
+__device__ __forceinline__ int pieces_of(const ScanParams& p, bool rejected, int seq) {
+  const long long n = rejected ? 0 : cu_at(p.seq, seq + 1) - cu_at(p.seq, seq);
+  return n > p.piece ? (int)((n + p.piece - 1) / p.piece) : 1;
+}
 
-  const long long tiles = (w.end - w.begin + TILE - 1) / TILE;
-  load(w.begin);
-  for (long long i = 0; i < tiles; i++) {
-    const int stage = (int)(i & 1);
-    const long long t0 = w.begin + i * TILE;
-    if (i >= 2) {
-      bar_sync(BAR_DONE + stage);
-      store(t0 - 2 * TILE, stage);
-    }
+// Which sequence holds piece `at` of the launch, and which of its pieces that is; false: none.  Each warp looks for itself: a lane
+// counts the pieces of N / 32 sequences.
+__device__ __forceinline__ bool find_piece(const ScanParams& p, bool rejected, int at, Work& w) {
+  const int lane = threadIdx.x % 32, each = (p.seq.N + 31) / 32;
+  const int first = min(p.seq.N, lane * each), last = min(p.seq.N, first + each);
+  int sum = 0;
+  for (int i = first; i < last; i++) sum += pieces_of(p, rejected, i);
+  int before = sum;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int j = row + e * ROWS;
-      const float uf = to_float(ru[e]);
-      float s = to_float(rdt[e]) + bias;
-      if (p.softplus) s = softplus(s);
-      if (t0 + j >= w.end) s = 0.0f;                 // leaves the state as it is
-      sh.step[stage][j][c] = make_float2(s, s * uf);
-      sh.y[stage][j][c] = skip * uf;
-      sh.gate[stage][j][c] = has_z ? silu<T>(to_float(rz[e])) : 1.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < EB; e++) {
-      sh.b[stage][brow + e * BROWS][n] = to_float(rb[e]);
-      sh.c[stage][brow + e * BROWS][n] = to_float(rc[e]);
-    }
-    bar_arrive(BAR_FULL + stage);
-    load(t0 + TILE);
+  for (int m = 1; m < 32; m *= 2) {
+    const int up = __shfl_up_sync(0xffffffffu, before, m);
+    if (lane >= m) before += up;
   }
-  for (long long i = tiles > 2 ? tiles - 2 : 0; i < tiles; i++) {
-    bar_sync(BAR_DONE + (int)(i & 1));
-    store(w.begin + i * TILE, (int)(i & 1));
+  before -= sum;
+  const unsigned has = __ballot_sync(0xffffffffu, at >= before && at < before + sum);
+  if (has == 0) return false;
+  int seq = first, n = 0;
+  if (at >= before && at < before + sum)
+    for (;; seq++) {
+      n = pieces_of(p, rejected, seq);
+      if (at < before + n) break;
+      before += n;
+    }
+  const int from = __ffs(has) - 1;
+  w.seq = __shfl_sync(0xffffffffu, seq, from);
+  w.pieces = __shfl_sync(0xffffffffu, n, from);
+  w.piece = at - __shfl_sync(0xffffffffu, before, from);
+  return true;
+}
+
+// The sequence of rank `r` by length, the longest first.
+__device__ __forceinline__ int by_length(const ScanParams& p, int r) {
+  const int lane = threadIdx.x % 32, N = p.seq.N;
+  int found = 0;
+  for (int i0 = 0; i0 < N; i0 += 32) {
+    const int i = i0 + lane;
+    const long long mine = i < N ? cu_at(p.seq, i + 1) - cu_at(p.seq, i) : -1;
+    int rank = 0;
+    for (int j0 = 0; j0 < N; j0 += 32) {
+      const long long other = j0 + lane < N ? cu_at(p.seq, j0 + lane + 1) - cu_at(p.seq, j0 + lane) : -1;
+      for (int j = 0; j < min(32, N - j0); j++) {
+        const int theirs = __shfl_sync(0xffffffffu, (int)other, j);
+        rank += theirs > (int)mine || (theirs == (int)mine && j0 + j < i);
+      }
+    }
+    const unsigned has = __ballot_sync(0xffffffffu, i < N && rank == r);
+    if (has != 0) found = i0 + __ffs(has) - 1;
+  }
+  return found;
+}
+
+// Helper `i` of a tile whose rows are `n` accesses wide: which access of the row and which quad of tokens.  Eight neighbours
+// write 16 bytes each, of four accesses' rows and two quads, to different banks (accesses of two values).
+__device__ __forceinline__ void place(int i, int n, int& access, int& quad) {
+  if (n >= 4) {
+    const int rest = i / 8;
+    access = i % 4 + rest % (n / 4) * 4;
+    quad = i / 4 % 2 + rest / (n / 4) * 2;
+  } else {
+    access = i % n;
+    quad = i / n;
   }
 }
 
-// The scan warps' half.
-template <int L, int S>
-__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[S], float (&h)[S]) {
-  const int lane = tid % L, c = tid / L;
-  const long long tiles = (w.end - w.begin + TILE - 1) / TILE;
-  for (long long i = 0; i < tiles; i++) {
-    const int stage = (int)(i & 1);
-    const int left = (int)min((long long)TILE, w.end - w.begin - i * TILE);
-    bar_sync(BAR_FULL + stage);
-    for (int j0 = 0; j0 < left; j0 += L) {
-      float part[L];
+__device__ __forceinline__ void copy16(void* to, const void* from, bool on) {       // not `on`: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+
+// A tile's rows of WIDTH values, `valid` of them there are, on their way into shared memory with zeros around: whole 16 bytes at
+// a time where the rows start on them, else value by value.
+template <typename T, int WIDTH, int STRIDE>
+struct Bring {
+  static constexpr int PER = 16 / sizeof(T), CHUNKS = (WIDTH + PER - 1) / PER, N = (CHUNKS * TILE + HELPERS - 1) / HELPERS;
+  const T* from;           // the first access of this thread, one tile after the other
+  long long ld;
+  int valid, t, c;
+  __device__ __forceinline__ Bring(const void* base, long long ld_, long long row, long long col, int valid_, bool async, int tid) : ld(ld_), valid(valid_) {
+    t = async ? tid / CHUNKS : tid / WIDTH;
+    c = async ? tid % CHUNKS * PER : tid % WIDTH;
+    from = reinterpret_cast<const T*>(base) + (row + t) * ld + col + c;
+  }
+  __device__ __forceinline__ void operator()(T (*to)[STRIDE], int left, bool async) {
+    if (async) {
+      const T* q = from;
 #pragma unroll
-      for (int j = 0; j < L; j++) {
-        const float2 st = sh.step[stage][j0 + j][c];
-        const Values<S> b = load_values<S>(&sh.b[stage][j0 + j][lane * S]), cc = load_values<S>(&sh.c[stage][j0 + j][lane * S]);
-        if constexpr (S > 1) {
-          F2 sum;
+      for (int i = 0; i < N; i++) {
+        constexpr int STEP = HELPERS / CHUNKS;
+        const int at = t + i * STEP;
+        const bool on = at < left && c < valid;
+        if (at < TILE && (HELPERS % CHUNKS == 0 || t < STEP)) copy16(&to[at][c], on ? q : from, on);
+        q += STEP * ld;
+      }
+    } else {
+      constexpr int M = (WIDTH * TILE + HELPERS - 1) / HELPERS, STEP = HELPERS / WIDTH > 0 ? HELPERS / WIDTH : 1;
+      T v[M];
+      const T* q = from;
 #pragma unroll
-          for (int k = 0; k < S; k += 2) {
-            float x0, x1;
-            split(mul2(f2(st.x, st.x), f2(a[k], a[k + 1])), x0, x1);
-            const F2 hn = fma2(f2(exp2_fast(x0), exp2_fast(x1)), f2(h[k], h[k + 1]), mul2(f2(st.y, st.y), f2(b.v[k], b.v[k + 1])));
-            split(hn, h[k], h[k + 1]);
-            sum = k == 0 ? mul2(f2(cc.v[0], cc.v[1]), hn) : fma2(f2(cc.v[k], cc.v[k + 1]), hn, sum);
+      for (int i = 0; i < M; i++) {
+        v[i] = from_float<T>(0.0f);
+        if (t + i * STEP < left && c < valid) v[i] = *q;
+        q += STEP * ld;
+      }
+#pragma unroll
+      for (int i = 0; i < M; i++)
+        if (t + i * STEP < TILE) to[t + i * STEP][c] = v[i];
+    }
+    from += TILE * ld;
+  }
+};
+
+// The helpers' half: tokens in, outputs out.  Copies run DEPTH - 1 tiles ahead.  A thread then has two channels of four
+// consecutive tokens at a time.
+template <typename T, int L, int S, bool LOCAL>
+__device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanShared<L, S>& sh, RawShared<T, L, S>& raw, int tid) {
+  using Sh = ScanShared<L, S>;
+  using Rw = RawShared<T, L, S>;
+  using P = Pack<T, 2>;
+  constexpr int DEPTH = Rw::DEPTH, R = Sh::R;
+  constexpr int CA = Sh::CB / 2;
+  static_assert(CA * QUADS <= HELPERS, "one block of two channels and four tokens a helper");
+  constexpr int NA = Sh::NP / 2, BBLOCKS = (LOCAL ? 1 : 2) * NA * QUADS, EB = (BBLOCKS + HELPERS - 1) / HELPERS;     // blocks of B, then of C
+  const bool has_z = !LOCAL && p.z != nullptr, async_x = p.async_x, async_bc = p.async_bc;
+  const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
+  const long long bn = (long long)w.group * p.Ns;
+  Bring<T, Sh::CB, Rw::XS> bu(p.u, p.ldu, w.begin, w.d0, w.channels, async_x, tid), bd(p.dt, p.lddt, w.begin, w.d0, w.channels, async_x, tid),
+      bz(p.z, p.ldz, w.begin, w.d0, w.channels, async_x, tid);
+  Bring<T, Sh::NP, Rw::NS> bb(p.B, p.ldb, w.begin, bn, p.Ns, async_bc, tid), bc(p.C, p.ldc, w.begin, bn, p.Ns, async_bc, tid);
+  auto bring_tile = [&](int i) {
+    if (i < tiles) {
+      const int left = w.tokens - i * TILE, at = i % DEPTH;
+      bu(raw.x[at][0], left, async_x);
+      bd(raw.x[at][1], left, async_x);
+      if (has_z) bz(raw.x[at][2], left, async_x);
+      bb(raw.bc[at][0], left, async_bc);
+      if constexpr (!LOCAL) bc(raw.bc[at][1], left, async_bc);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int c, quad;
+  place(tid, CA, c, quad);
+  c *= 2;
+  const int j = 4 * quad;                            // first token of this thread in a tile
+  const bool mine = quad < QUADS;
+  const int channels = mine ? w.channels - c : 0;    // of this thread, two at most
+  T* out = reinterpret_cast<T*>(p.out) + (w.begin + j) * p.ldo + w.d0 + c;
+  float skip[2], bias[2];
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    const int d = w.d0 + (v < channels ? c + v : 0);
+    skip[v] = p.D != nullptr ? p.D[d] : 0.0f;
+    bias[v] = p.dt_bias != nullptr ? p.dt_bias[d] : 0.0f;
+  }
+  float* const row = mine ? &sh.step[c][j] : &sh.step[0][0];               // step, input, y, skip, gate lie CB rows apart
+  constexpr int ARRAY = Sh::CB * R;
+  auto store = [&](int i) {
+    const int left = w.tokens - i * TILE - j;
+    if (channels > 0 && left > 0) {
+      const float* y0 = row + (i & 1) * TILE + 2 * ARRAY;
+      float y[4][2];
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        float4 f = *reinterpret_cast<const float4*>(y0 + v * R);
+        const float4 d = *reinterpret_cast<const float4*>(y0 + v * R + ARRAY);
+        f.x += d.x; f.y += d.y; f.z += d.z; f.w += d.w;
+        if (has_z) {
+          const float4 g = *reinterpret_cast<const float4*>(y0 + v * R + 2 * ARRAY);
+          f.x *= g.x; f.y *= g.y; f.z *= g.z; f.w *= g.w;
+        }
+        y[0][v] = f.x; y[1][v] = f.y; y[2][v] = f.z; y[3][v] = f.w;
+      }
+      T* to = out;
+      if (async_x && left >= 4) {
+#pragma unroll
+        for (int k = 0; k < 4; k++, to += p.ldo) *reinterpret_cast<P*>(to) = pack<T, 2>(y[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++, to += p.ldo)
+          if (k < left) {
+            to[0] = from_float<T>(y[k][0]);
+            if (channels > 1) to[1] = from_float<T>(y[k][1]);
           }
-          float s0, s1;
-          split(sum, s0, s1);
-          part[j] = s0 + s1;
+      }
+    }
+    out += TILE * p.ldo;
+  };
+  for (int i = 0; i < DEPTH - 1; i++) bring_tile(i);
+  for (int i = 0; i < tiles; i++) {
+    const int stage = i & 1, slot = i % DEPTH;
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"n"((int)BAR_HELPERS), "n"(HELPERS) : "memory");         // tile i is here, tile i - 1 has been read
+    bring_tile(i + DEPTH - 1);
+    if (i >= 2) {
+      bar_sync(BAR_DONE + stage);
+      if constexpr (!LOCAL) store(i - 2);
+    }
+    if (mine) {
+      const int left = w.tokens - i * TILE - j;
+      const T* x = &raw.x[slot][0][j][c];
+      constexpr int X = TILE * Rw::XS;
+      float uf[4][2], df[4][2], zf[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        unpack(*reinterpret_cast<const P*>(x + k * Rw::XS), uf[k]);
+        unpack(*reinterpret_cast<const P*>(x + k * Rw::XS + X), df[k]);
+        if (has_z) unpack(*reinterpret_cast<const P*>(x + k * Rw::XS + 2 * X), zf[k]);
+      }
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        float s[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[k] = df[k][v] + bias[v];
+        if (p.softplus) {
+          split(softplus2(s[0], s[1]), s[0], s[1]);
+          split(softplus2(s[2], s[3]), s[2], s[3]);
+        }
+        if (left < 4)
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (k >= left) s[k] = 0.0f;              // leaves the state as it is
+        float* to = row + stage * TILE + v * R;
+        *reinterpret_cast<float4*>(to) = make_float4(s[0], s[1], s[2], s[3]);
+        *reinterpret_cast<float4*>(to + ARRAY) = make_float4(s[0] * uf[0][v], s[1] * uf[1][v], s[2] * uf[2][v], s[3] * uf[3][v]);
+        if constexpr (!LOCAL) *reinterpret_cast<float4*>(to + 3 * ARRAY) = make_float4(skip[v] * uf[0][v], skip[v] * uf[1][v], skip[v] * uf[2][v], skip[v] * uf[3][v]);
+        if (has_z) *reinterpret_cast<float4*>(to + 4 * ARRAY) = make_float4(silu<T>(zf[0][v]), silu<T>(zf[1][v]), silu<T>(zf[2][v]), silu<T>(zf[3][v]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < EB; e++) {
+      int n, q;
+      const int id = tid + e * HELPERS, second = id >= NA * QUADS;
+      place(id % (NA * QUADS), NA, n, q);
+      if (id >= BBLOCKS) continue;
+      float f[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; k++) unpack(*reinterpret_cast<const P*>(&raw.bc[slot][second][4 * q + k][2 * n]), f[k]);
+      float* to = (second ? &sh.c[0][0] : &sh.b[0][0]) + 2 * n * R + stage * TILE + 4 * q;
+      *reinterpret_cast<float4*>(to) = make_float4(f[0][0], f[1][0], f[2][0], f[3][0]);
+      *reinterpret_cast<float4*>(to + R) = make_float4(f[0][1], f[1][1], f[2][1], f[3][1]);
+    }
+    bar_arrive(BAR_FULL + stage);
+  }
+  for (int i = tiles > 2 ? tiles - 2 : 0; i < tiles; i++) {
+    bar_sync(BAR_DONE + (i & 1));
+    if constexpr (!LOCAL) store(i);
+  }
+}
+
+// The scan warps' half: lane l of a channel holds the state values l + k L.  A tile is one run of instructions, four tokens after
+// four; tokens behind the last one leave the state as it is.
+// LOCAL: the state alone, and the sum of the steps.
+template <int L, int S, bool LOCAL>
+__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[S], float (&h)[S], float& sum) {
+  constexpr int R = ScanShared<L, S>::R;
+  const int lane = tid % L, c = tid / L;
+  const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
+  F2 aa[S];
+#pragma unroll
+  for (int k = 0; k < S; k++) aa[k] = f2(a[k], a[k]);
+  for (int i = 0; i < tiles; i++) {
+    const int stage = i & 1;
+    bar_sync(BAR_FULL + stage);
+    const float *step = &sh.step[c][stage * TILE], *input = &sh.input[c][stage * TILE];
+    const float *b = &sh.b[lane][stage * TILE], *cc = &sh.c[lane][stage * TILE];
+    float* out = &sh.y[c][stage * TILE + (L >= 4 ? lane / (L / 4) : 0)];
+#pragma unroll
+    for (int j = 0; j < TILE; j += 4) {
+      const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(step + j), in = *reinterpret_cast<const ulonglong2*>(input + j);
+      F2 y01, y23;
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        const ulonglong2 bk = *reinterpret_cast<const ulonglong2*>(b + k * L * R + j);
+        float x0, x1, x2, x3, i0, i1, i2, i3;
+        split(mul2(st.x, aa[k]), x0, x1);
+        split(mul2(st.y, aa[k]), x2, x3);
+        split(mul2(in.x, bk.x), i0, i1);
+        split(mul2(in.y, bk.y), i2, i3);
+        const float h0 = fmaf(exp2_fast(x0), h[k], i0), h1 = fmaf(exp2_fast(x1), h0, i1), h2 = fmaf(exp2_fast(x2), h1, i2);
+        h[k] = fmaf(exp2_fast(x3), h2, i3);
+        if constexpr (LOCAL) continue;
+        const ulonglong2 ck = *reinterpret_cast<const ulonglong2*>(cc + k * L * R + j);
+        y01 = k == 0 ? mul2(ck.x, f2(h0, h1)) : fma2(ck.x, f2(h0, h1), y01);
+        y23 = k == 0 ? mul2(ck.y, f2(h2, h[k])) : fma2(ck.y, f2(h2, h[k]), y23);
+      }
+      if constexpr (LOCAL) {
+        float s0, s1, s2, s3;
+        split(st.x, s0, s1);
+        split(st.y, s2, s3);
+        sum += (s0 + s1) + (s2 + s3);
+        continue;
+      }
+      float part[4];
+      split(y01, part[0], part[1]);
+      split(y23, part[2], part[3]);
+      // lane l ends with the sum of token l / (L / 4)
+#pragma unroll
+      for (int m = L / 2, n = 2; m >= 1; m /= 2, n /= 2) {
+        if (n >= 1) {
+#pragma unroll
+          for (int k = 0; k < n; k++) {
+            const bool up = lane & m;
+            const float give = up ? part[k] : part[n + k], keep = up ? part[n + k] : part[k];
+            part[k] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+          }
         } else {
-          h[0] = fmaf(exp2_fast(st.x * a[0]), h[0], st.y * b.v[0]);
-          part[j] = cc.v[0] * h[0];
+          part[0] += __shfl_xor_sync(0xffffffffu, part[0], m);
         }
       }
-      // lane l ends with the sum of token j0 + l
-#pragma unroll
-      for (int m = L / 2; m >= 1; m /= 2) {
-#pragma unroll
-        for (int k = 0; k < m; k++) {
-          const bool up = lane & m;
-          const float give = up ? part[k] : part[m + k], keep = up ? part[m + k] : part[k];
-          part[k] = keep + __shfl_xor_sync(0xffffffffu, give, m);
-        }
-      }
-      sh.y[stage][j0 + lane][c] += part[0];
+      out[j] = part[0];                              // L / 4 lanes write the same value
     }
     bar_arrive(BAR_DONE + stage);
   }
 }
 
-// One sequence and up to CB channels of one group a block.
-template <typename T, int L, int S>
-__global__ void __launch_bounds__(SCAN_THREADS) kda_selective_scan_kernel(const ScanParams p) {
+// A sequence, or a piece of one, and up to CB channels of one group a block.
+template <typename T, int L, int S, bool LOCAL>
+__global__ void __launch_bounds__(SCAN_THREADS, 2) kda_selective_scan_kernel(const ScanParams p) {
   using Sh = ScanShared<L, S>;
   constexpr int CB = Sh::CB;
   extern __shared__ __align__(16) unsigned char smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
-  const int per = p.Dm / p.groups, gblocks = (per + CB - 1) / CB;
-  const int seq = blockIdx.x / (gblocks * p.groups), block = blockIdx.x % (gblocks * p.groups);
-  const int tid = threadIdx.x % SCAN_LANES;
+  RawShared<T, L, S>& raw = *reinterpret_cast<RawShared<T, L, S>*>(smem + sizeof(Sh));
+  const int per = p.Dm / p.groups, gblocks = (per + CB - 1) / CB, block = blockIdx.x % (gblocks * p.groups);
+  const int tid = threadIdx.x % SCAN_LANES;          // scan threads first
   const bool helper = threadIdx.x >= SCAN_LANES;
   Work w;
   w.group = block / gblocks;
   w.d0 = w.group * per + block % gblocks * CB;
   w.channels = min(CB, (w.group + 1) * per - w.d0);
   const bool rejected = cu_rejected(p.seq);
-  const long long slot = claim_slot(p.seq, seq);
-  w.begin = rejected ? 0 : cu_at(p.seq, seq);
-  w.end = rejected ? 0 : cu_at(p.seq, seq + 1);
+  w.at = blockIdx.x / (gblocks * p.groups);
+  if (p.piece > 0) {
+    if (!find_piece(p, rejected, w.at, w) || (LOCAL && w.piece + 1 == w.pieces)) return;
+  } else {
+    w.seq = p.seq.N > 1 && p.seq.N <= RANKED && !rejected ? by_length(p, w.at) : w.at;
+    w.piece = 0;
+    w.pieces = 1;
+  }
+  const long long slot = claim_slot(p.seq, w.seq);
+  long long end = rejected ? 0 : cu_at(p.seq, w.seq + 1);
+  w.begin = (rejected ? 0 : cu_at(p.seq, w.seq)) + (long long)w.piece * p.piece;
+  if (w.piece + 1 < w.pieces) end = w.begin + p.piece;
+  w.tokens = __reduce_max_sync(0xffffffffu, (int)(end - w.begin));       // the same in all lanes, and known to be: no divergence in the loops
   if (helper) {
-    help<T, L, S>(p, w, sh, tid);
+    help<T, L, S, LOCAL>(p, w, sh, raw, tid);
     // rows behind the last sequence
-    if (seq == p.seq.N - 1 && (rejected || p.zero_pad) && tid % CB < w.channels)
-      for (long long t = w.end + tid / CB; t < p.seq.T; t += L) reinterpret_cast<T*>(p.out)[t * p.ldo + w.d0 + tid % CB] = from_float<T>(0.0f);
+    if (!LOCAL && w.seq == p.seq.N - 1 && w.piece + 1 == w.pieces && (rejected || p.zero_pad) && tid % CB < w.channels)
+      for (long long t = end + tid / CB; t < p.seq.T; t += HELPERS / CB) reinterpret_cast<T*>(p.out)[t * p.ldo + w.d0 + tid % CB] = from_float<T>(0.0f);
     return;
   }
   const int lane = tid % L, c = tid / L;
   const bool mine = c < w.channels;
-  const long long at = (long long)(w.d0 + (mine ? c : 0)) * p.Ns + lane * S;
-  float a[S], h[S];
+  const long long at = (long long)(w.d0 + (mine ? c : 0)) * p.Ns + lane, rows = (long long)p.Dm * p.Ns;
+  float* const own = p.ws_state + w.at * rows;       // a piece's state: first what it adds to the state, then the state it starts from
+  const float* from = w.pieces > 1 ? own : (p.src != nullptr && slot >= 0 ? p.src + slot * p.src_stride : nullptr);
+  float a[S], h[S], sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < S; k++) {
-    const bool on = mine && lane * S + k < p.Ns;
-    a[k] = on ? p.A[at + k] * LOG2E_F : 0.0f;
-    if (a[k] < -3.0e38f) a[k] = -3.0e38f;            // -inf times a step of zero (behind the last token) would be NaN
-    h[k] = on && p.src != nullptr && slot >= 0 ? p.src[slot * p.src_stride + at + k] : 0.0f;
+    const bool on = mine && lane + k * L < p.Ns;
+    a[k] = on ? decay_rate(p.A[at + k * L]) : 0.0f;
+    h[k] = !LOCAL && on && from != nullptr ? from[at + k * L] : 0.0f;
   }
-  scan<L, S>(w, sh, tid, a, h);
-  if (p.dst == nullptr || slot < 0 || !mine) return;
+  scan<L, S, LOCAL>(w, sh, tid, a, h, sum);
+  float* to = LOCAL ? own : (w.piece + 1 == w.pieces && p.dst != nullptr && slot >= 0 ? p.dst + slot * p.dst_stride : nullptr);
+  if (to == nullptr || !mine) return;
 #pragma unroll
   for (int k = 0; k < S; k++)
-    if (lane * S + k < p.Ns) p.dst[slot * p.dst_stride + at + k] = h[k];
+    if (lane + k * L < p.Ns) to[at + k * L] = h[k];
+  if (LOCAL && lane == 0) p.ws_sum[(long long)w.at * p.Dm + w.d0 + c] = sum;
+}
+
+// Between the passes over pieces: from what each piece adds to the state (and exp(A sum of its steps), what it leaves of the
+// state in front) to the state that each starts from.  A thread follows one state value through its sequence.
+constexpr int JOIN_THREADS = 256;
+__global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(const ScanParams p) {
+  const long long rows = (long long)p.Dm * p.Ns;
+  const int blocks = (int)((rows + JOIN_THREADS - 1) / JOIN_THREADS), seq = blockIdx.x / blocks;
+  const bool rejected = cu_rejected(p.seq);
+  const int n = pieces_of(p, rejected, seq);
+  if (n < 2) return;
+  const long long slot = claim_slot(p.seq, seq);
+  int first = 0;
+  for (int i = threadIdx.x % 32; i < seq; i += 32) first += pieces_of(p, rejected, i);
+  first = __reduce_add_sync(0xffffffffu, first);
+  const long long at = (long long)(blockIdx.x % blocks) * JOIN_THREADS + threadIdx.x;
+  if (at >= rows) return;
+  const long long d = at / p.Ns;
+  const float a = decay_rate(p.A[at]);
+  float h = p.src != nullptr && slot >= 0 ? p.src[slot * p.src_stride + at] : 0.0f;
+  float *state = p.ws_state + first * rows + at, *sums = p.ws_sum + (long long)first * p.Dm + d;
+  constexpr int AHEAD = 8;
+  for (int i0 = 0; i0 < n; i0 += AHEAD) {
+    float add[AHEAD], keep[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      const bool on = i0 + i + 1 < n;                // the last piece adds nothing here
+      add[i] = on ? state[(i0 + i) * rows] : 0.0f;
+      keep[i] = on ? exp2_fast(a * sums[(long long)(i0 + i) * p.Dm]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (i0 + i < n) {
+        state[(i0 + i) * rows] = h;
+        h = fmaf(keep[i], h, add[i]);
+      }
+  }
 }
 
 // One token a row: L lanes hold a channel's state, S values each.  Bound by memory: the state goes through once.
 template <typename T, int L, int S>
-__global__ void __launch_bounds__(SCAN_LANES) kda_selective_scan_step_kernel(const ScanParams p) {
-  constexpr int CB = SCAN_LANES / L;
+__global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(const ScanParams p) {
+  constexpr int CB = STEP_LANES / L;
   const int cblocks = (p.Dm + CB - 1) / CB;
   const long long row = blockIdx.x / cblocks;
   const int lane = threadIdx.x % L, d = (int)(blockIdx.x % cblocks) * CB + threadIdx.x / L;
@@ -319,45 +575,89 @@ __global__ void __launch_bounds__(SCAN_LANES) kda_selective_scan_step_kernel(con
   }
 }
 
+template <typename T, int L, int S, bool LOCAL>
+cudaError_t launch_pass(const ScanParams& p, long long pieces, cudaStream_t stream) {
+  constexpr int bytes = sizeof(ScanShared<L, S>) + sizeof(RawShared<T, L, S>), CB = ScanShared<L, S>::CB;
+  const long long blocks = (long long)((p.Dm / p.groups + CB - 1) / CB) * p.groups * pieces;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const cudaError_t e = cudaFuncSetAttribute(kda_selective_scan_kernel<T, L, S, LOCAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  kda_selective_scan_kernel<T, L, S, LOCAL><<<(unsigned)blocks, SCAN_THREADS, bytes, stream>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T, int L, int S>
-cudaError_t launch_lanes(const ScanParams& p, bool step, cudaStream_t stream) {
-  constexpr int CB = SCAN_LANES / L;
-  const int per = p.Dm / p.groups;
-  const long long blocks = step ? (long long)((p.Dm + CB - 1) / CB) * p.seq.N : (long long)((per + CB - 1) / CB) * p.groups * p.seq.N;
+cudaError_t launch_lanes(const ScanParams& p, cudaStream_t stream) {
+  if (p.piece == 0) return launch_pass<T, L, S, false>(p, p.seq.N, stream);
+  const long long pieces = p.seq.T / p.piece + p.seq.N;
+  cudaError_t e = launch_pass<T, L, S, true>(p, pieces, stream);
+  if (e != cudaSuccess) return e;
+  const long long rows = (long long)p.Dm * p.Ns, blocks = (rows + JOIN_THREADS - 1) / JOIN_THREADS * p.seq.N;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  kda_selective_scan_join_kernel<<<(unsigned)blocks, JOIN_THREADS, 0, stream>>>(p);
+  e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_pass<T, L, S, false>(p, pieces, stream);
+}
+
+// Whether the rows that `p` and `ld` name start on 16 bytes, and are whole 16 bytes wide.
+template <typename T>
+bool rows16(const void* p, long long ld, long long width) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * (long long)sizeof(T)) | (uintptr_t)(width * (long long)sizeof(T))) & 15) == 0;
+}
+
+template <typename T>
+cudaError_t launch_type(ScanParams p, cudaStream_t stream) {
+  const long long per = p.Dm / p.groups;
+  p.async_x = rows16<T>(p.u, p.ldu, per) && rows16<T>(p.dt, p.lddt, per) && rows16<T>(p.z, p.ldz, per) && rows16<T>(p.out, p.ldo, per);
+  p.async_bc = rows16<T>(p.B, p.ldb, p.Ns) && rows16<T>(p.C, p.ldc, p.Ns);
+  if (p.Ns <= 4) return launch_lanes<T, 4, 1>(p, stream);
+  if (p.Ns <= 8) return launch_lanes<T, 4, 2>(p, stream);
+  if (p.Ns <= 16) return launch_lanes<T, 4, 4>(p, stream);
+  if (p.Ns <= 32) return launch_lanes<T, 8, 4>(p, stream);
+  if (p.Ns <= 64) return launch_lanes<T, 16, 4>(p, stream);
+  return launch_lanes<T, 32, 4>(p, stream);
+}
+
+template <typename T, int L, int S>
+cudaError_t launch_step(const ScanParams& p, cudaStream_t stream) {
+  const long long blocks = (long long)((p.Dm + STEP_LANES / L - 1) / (STEP_LANES / L)) * p.seq.N;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (blocks == 0) return cudaSuccess;
-  if (step) {
-    kda_selective_scan_step_kernel<T, L, S><<<(unsigned)blocks, SCAN_LANES, 0, stream>>>(p);
-  } else {
-    constexpr int bytes = sizeof(ScanShared<L, S>);
-    if (bytes > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kda_selective_scan_kernel<T, L, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      if (e != cudaSuccess) return e;
-    }
-    kda_selective_scan_kernel<T, L, S><<<(unsigned)blocks, SCAN_THREADS, bytes, stream>>>(p);
-  }
+  kda_selective_scan_step_kernel<T, L, S><<<(unsigned)blocks, STEP_LANES, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_type(const ScanParams& p, bool step, cudaStream_t stream) {
-  if (p.Ns <= 4) return launch_lanes<T, 4, 1>(p, step, stream);
-  if (p.Ns <= 8) return launch_lanes<T, 4, 2>(p, step, stream);
-  if (p.Ns <= 16) return launch_lanes<T, 4, 4>(p, step, stream);
-  if (p.Ns <= 32) return launch_lanes<T, 8, 4>(p, step, stream);
-  if (p.Ns <= 64) return launch_lanes<T, 16, 4>(p, step, stream);
-  return launch_lanes<T, 32, 4>(p, step, stream);
-}
-
-cudaError_t launch_any(const ScanParams& p, int type, bool step, cudaStream_t stream) {
-  if (type == TYPE_BF16) return launch_type<__nv_bfloat16>(p, step, stream);
-  if (type == TYPE_FP16) return launch_type<__half>(p, step, stream);
-  return launch_type<float>(p, step, stream);
+cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
+  if (p.Ns <= 16) return launch_step<T, 4, 4>(p, stream);
+  if (p.Ns <= 32) return launch_step<T, 8, 4>(p, stream);
+  if (p.Ns <= 64) return launch_step<T, 16, 4>(p, stream);
+  return launch_step<T, 32, 4>(p, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_sscan(const ScanParams& p, int type, cudaStream_t stream) { return launch_any(p, type, false, stream); }
-cudaError_t launch_sscan_step(const ScanParams& p, int type, cudaStream_t stream) { return launch_any(p, type, true, stream); }
+// Where whole sequences would leave SMs without work, they are cut: a first pass over the pieces finds what each adds to the
+// state, the states are joined, a second pass computes the outputs.  That is about 1.6 times the work, for blocks that fill the
+// card (two an SM): 0 = no cut, else the tokens of a piece.
+long long sscan_piece(long long T, int N, int Dm, int Ns) {
+  const int lanes = Ns <= 16 ? 4 : (Ns <= 32 ? 8 : (Ns <= 64 ? 16 : 32));
+  const long long blocks = (Dm + SCAN_LANES / lanes - 1) / (SCAN_LANES / lanes), room = 2 * 148;
+  if (blocks * N >= room || N > room || T < 512) return 0;
+  const long long piece = (T * blocks / (4 * room) + TILE - 1) / TILE * TILE;
+  return piece < 128 ? 128 : piece;
+}
+
+cudaError_t launch_sscan(const ScanParams& p, int type, cudaStream_t stream) {
+  if (type == TYPE_BF16) return launch_type<__nv_bfloat16>(p, stream);
+  if (type == TYPE_FP16) return launch_type<__half>(p, stream);
+  return launch_type<float>(p, stream);
+}
+
+cudaError_t launch_sscan_step(const ScanParams& p, int type, cudaStream_t stream) {
+  if (type == TYPE_BF16) return launch_step_type<__nv_bfloat16>(p, stream);
+  if (type == TYPE_FP16) return launch_step_type<__half>(p, stream);
+  return launch_step_type<float>(p, stream);
+}
 
 }  // namespace kda
