@@ -94,8 +94,10 @@ struct RawShared {
 
   // rows of whole 16 bytes; 16-bit rows four apart fall into different halves of the banks
   static constexpr int XS = SCAN_LANES / L + 8, NS = L * S + 8;
-  T x[DEPTH][3][TILE][XS];                           // u, dt, z
-  T bc[DEPTH][2][TILE][NS];
+  struct Slot {
+    T x[3][TILE][XS];                                // u, dt, z
+    T bc[2][TILE][NS];
+  } slot[DEPTH];
 };
 
 template <int L, int S>
@@ -200,11 +202,13 @@ template <typename T, int WIDTH, int STRIDE>
 struct Bring {
   static constexpr int PER = 16 / sizeof(T), CHUNKS = (WIDTH + PER - 1) / PER, N = (CHUNKS * TILE + HELPERS - 1) / HELPERS;
   const T* from;           // the first access of this thread, one tile after the other
-  long long ld;
-  int valid, t, c;
-  __device__ __forceinline__ Bring(const void* base, long long ld_, long long row, long long col, int valid_, bool async, int tid) : ld(ld_), valid(valid_) {
+  long long ld, tile;
+  int t, c;
+  bool inside;
+  __device__ __forceinline__ Bring(const void* base, long long ld_, long long row, long long col, int valid_, bool async, int tid) : ld(ld_), tile(TILE * ld_) {
     t = async ? tid / CHUNKS : tid / WIDTH;
     c = async ? tid % CHUNKS * PER : tid % WIDTH;
+    inside = c < valid_;
     from = reinterpret_cast<const T*>(base) + (row + t) * ld + col + c;
   }
   __device__ __forceinline__ void operator()(T (*to)[STRIDE], int left, bool async) {
@@ -214,7 +218,7 @@ struct Bring {
       for (int i = 0; i < N; i++) {
         constexpr int STEP = HELPERS / CHUNKS;
         const int at = t + i * STEP;
-        const bool on = at < left && c < valid;
+        const bool on = inside && at < left;
         if (at < TILE && (HELPERS % CHUNKS == 0 || t < STEP)) copy16(&to[at][c], on ? q : from, on);
         q += STEP * ld;
       }
@@ -225,14 +229,14 @@ struct Bring {
 #pragma unroll
       for (int i = 0; i < M; i++) {
         v[i] = from_float<T>(0.0f);
-        if (t + i * STEP < left && c < valid) v[i] = *q;
+        if (inside && t + i * STEP < left) v[i] = *q;
         q += STEP * ld;
       }
 #pragma unroll
       for (int i = 0; i < M; i++)
         if (t + i * STEP < TILE) to[t + i * STEP][c] = v[i];
     }
-    from += TILE * ld;
+    from += tile;
   }
 };
 
@@ -255,12 +259,13 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
   Bring<T, Sh::NP, Rw::NS> bb(p.B, p.ldb, w.begin, bn, p.Ns, async_bc, tid), bc(p.C, p.ldc, w.begin, bn, p.Ns, async_bc, tid);
   auto bring_tile = [&](int i) {
     if (i < tiles) {
-      const int left = w.tokens - i * TILE, at = i % DEPTH;
-      bu(raw.x[at][0], left, async_x);
-      bd(raw.x[at][1], left, async_x);
-      if (has_z) bz(raw.x[at][2], left, async_x);
-      bb(raw.bc[at][0], left, async_bc);
-      if constexpr (!LOCAL) bc(raw.bc[at][1], left, async_bc);
+      const int left = w.tokens - i * TILE;
+      typename Rw::Slot& to = raw.slot[i % DEPTH];
+      bu(to.x[0], left, async_x);
+      bd(to.x[1], left, async_x);
+      if (has_z) bz(to.x[2], left, async_x);
+      bb(to.bc[0], left, async_bc);
+      if constexpr (!LOCAL) bc(to.bc[1], left, async_bc);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -268,7 +273,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
   place(tid, CA, c, quad);
   c *= 2;
   const int j = 4 * quad;                            // first token of this thread in a tile
-  const bool mine = quad < QUADS;
+  const bool mine = CA * QUADS == HELPERS || quad < QUADS;
   const int channels = mine ? w.channels - c : 0;    // of this thread, two at most
   T* out = reinterpret_cast<T*>(p.out) + (w.begin + j) * p.ldo + w.d0 + c;
   float skip[2], bias[2];
@@ -313,7 +318,8 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
   };
   for (int i = 0; i < DEPTH - 1; i++) bring_tile(i);
   for (int i = 0; i < tiles; i++) {
-    const int stage = i & 1, slot = i % DEPTH;
+    const int stage = i & 1;
+    const typename Rw::Slot& slot = raw.slot[i % DEPTH];
     asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
     asm volatile("bar.sync %0, %1;" ::"n"((int)BAR_HELPERS), "n"(HELPERS) : "memory");         // tile i is here, tile i - 1 has been read
     bring_tile(i + DEPTH - 1);
@@ -323,7 +329,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
     }
     if (mine) {
       const int left = w.tokens - i * TILE - j;
-      const T* x = &raw.x[slot][0][j][c];
+      const T* x = &slot.x[0][j][c];
       constexpr int X = TILE * Rw::XS;
       float uf[4][2], df[4][2], zf[4][2];
 #pragma unroll
@@ -360,7 +366,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
       if (id >= BBLOCKS) continue;
       float f[4][2];
 #pragma unroll
-      for (int k = 0; k < 4; k++) unpack(*reinterpret_cast<const P*>(&raw.bc[slot][second][4 * q + k][2 * n]), f[k]);
+      for (int k = 0; k < 4; k++) unpack(*reinterpret_cast<const P*>(&slot.bc[second][4 * q + k][2 * n]), f[k]);
       float* to = (second ? &sh.c[0][0] : &sh.b[0][0]) + 2 * n * R + stage * TILE + 4 * q;
       *reinterpret_cast<float4*>(to) = make_float4(f[0][0], f[1][0], f[2][0], f[3][0]);
       *reinterpret_cast<float4*>(to + R) = make_float4(f[0][1], f[1][1], f[2][1], f[3][1]);
@@ -379,6 +385,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 template <int L, int S, bool LOCAL>
 __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[S], float (&h)[S], float& sum) {
   constexpr int R = ScanShared<L, S>::R;
+  constexpr int SUMS = 8;                            // tokens that are summed over the lanes at a time: exchanges that do not wait for each other
   const int lane = tid % L, c = tid / L;
   const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
   F2 aa[S];
@@ -389,7 +396,7 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
     bar_sync(BAR_FULL + stage);
     const float *step = &sh.step[c][stage * TILE], *input = &sh.input[c][stage * TILE];
     const float *b = &sh.b[lane][stage * TILE], *cc = &sh.c[lane][stage * TILE];
-    float* out = &sh.y[c][stage * TILE + (L >= 4 ? lane / (L / 4) : 0)];
+    float part[SUMS];
 #pragma unroll
     for (int j = 0; j < TILE; j += 4) {
       const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(step + j), in = *reinterpret_cast<const ulonglong2*>(input + j);
@@ -416,12 +423,13 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
         sum += (s0 + s1) + (s2 + s3);
         continue;
       }
-      float part[4];
-      split(y01, part[0], part[1]);
-      split(y23, part[2], part[3]);
-      // lane l ends with the sum of token l / (L / 4)
+      split(y01, part[j % SUMS], part[j % SUMS + 1]);
+      split(y23, part[j % SUMS + 2], part[j % SUMS + 3]);
+      if ((j + 4) % SUMS != 0) continue;
+      // a step of the exchange leaves half of the tokens with each lane: lane l ends with the sums of tokens l SUMS / L and on
+      // (L > SUMS: neighbours with the same one)
 #pragma unroll
-      for (int m = L / 2, n = 2; m >= 1; m /= 2, n /= 2) {
+      for (int m = L / 2, n = SUMS / 2; m >= 1; m /= 2, n /= 2) {
         if (n >= 1) {
 #pragma unroll
           for (int k = 0; k < n; k++) {
@@ -433,7 +441,9 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
           part[0] += __shfl_xor_sync(0xffffffffu, part[0], m);
         }
       }
-      out[j] = part[0];                              // L / 4 lanes write the same value
+      float* out = &sh.y[c][stage * TILE + j + 4 - SUMS + lane * SUMS / L];
+      if constexpr (L == 4) *reinterpret_cast<float2*>(out) = make_float2(part[0], part[1]);
+      else *out = part[0];
     }
     bar_arrive(BAR_DONE + stage);
   }

@@ -175,3 +175,16 @@ def lib():
 def check(rc: int, what: str):
     if rc != 0:
         raise RuntimeError(f"{what} failed: {lib().kda_error_string(rc).decode()} (code {rc})")
+
+
+_raw = {}
+
+
+def raw(name):
+    """The entry point with an untyped argument block (words instead of the struct)."""
+    f = _raw.get(name)
+    if f is None:
+        f = lib()[name]
+        f.argtypes, f.restype = [C.c_void_p, C.c_void_p], C.c_int
+        _raw[name] = f
+    return f

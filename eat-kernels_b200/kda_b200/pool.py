@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _cabi, _err, _reject_aliasing
-from .serving import _enqueue, _pool_rows, _ptr
+from .serving import _call, _pool_rows, _ptr, _Ready
 
 
 def _index(t, name, dev=None):
@@ -30,8 +30,6 @@ def _index(t, name, dev=None):
 
 def _args(pools, used, status, dev, slots, written, read):
     """Argument block of a call: pools, `used` and status checked and filled in."""
-    if not isinstance(pools, (list, tuple)) or len(pools) > _cabi.MAX_POOLS:
-        raise _err(f"pools must be a list of at most {_cabi.MAX_POOLS} tensors")
     a = _cabi.KdaPoolArgs()
     for i, t in enumerate(pools):
         if not (torch.is_tensor(t) and t.is_cuda and t.dim() >= 1):
@@ -88,58 +86,72 @@ def _workspace(a, n, dev):
     return ws
 
 
-def pool_copy(pools, src, dst, *, status=None):
-    """Row dst[i] of every pool <- row src[i] (a negative source: zeros; a negative destination: padding).  Left out, with bit 2: an
-    entry out of range, a destination that an earlier entry names, and one that any entry reads (the result would depend on the
-    order)."""
+def _ready(name, dev, a, first, given, fresh, result, n_pools, written):
+    """The pools are the caller's tensors from `first` on."""
+    given.update({first + i: [f"base[{i}]"] for i in range(n_pools)})
+    return _Ready(name, dev, a, given, fresh, result, [*written, *range(first, first + n_pools)])
+
+
+def _pools(pools):
+    if not isinstance(pools, (list, tuple)) or len(pools) > _cabi.MAX_POOLS:
+        raise _err(f"pools must be a list of at most {_cabi.MAX_POOLS} tensors")
+    return tuple(pools)
+
+
+def _copy(src, dst, status, *pools):
     _index(src, "src")
     _index(dst, "dst", src.device)
     if src.numel() != dst.numel():
         raise _err(f"src and dst must have the same number of entries, got {src.numel()} and {dst.numel()}")
     a, dev = _args(pools, None, status, src.device, None, [], [("src", src), ("dst", dst)])
-    if src.numel() == 0:
-        return
     ws = _workspace(a, src.numel(), dev)
-    a.src, a.src_is64, a.dst, a.dst_is64 = src.data_ptr(), src.dtype == torch.int64, dst.data_ptr(), dst.dtype == torch.int64
-    _enqueue("kda_pool_copy_launch", a, dev)
-    del ws
+    a.src, a.src_is64, a.dst, a.dst_is64 = _ptr(src), src.dtype == torch.int64, _ptr(dst), dst.dtype == torch.int64
+    return _ready("kda_pool_copy_launch" if src.numel() else None, dev, a, 3, {0: ["src"], 1: ["dst"], 2: ["status"]}, [(ws, ["workspace"])], (),
+                  len(pools), [])
+
+
+def pool_copy(pools, src, dst, *, status=None):
+    """Row dst[i] of every pool <- row src[i] (a negative source: zeros; a negative destination: padding).  Left out, with bit 2: an
+    entry out of range, a destination that an earlier entry names, and one that any entry reads (the result would depend on the
+    order)."""
+    _call(_copy, (src, dst, status, *_pools(pools)))
+
+
+def _fork(used, parents, status, *pools):
+    dev, P = _used(used)
+    _index(parents, "parents", dev)
+    slots = torch.empty(parents.numel(), dtype=torch.int32, device=dev)
+    a, dev = _args(pools, used, status, dev, P, [], [("parents", parents)])
+    ws = _workspace(a, parents.numel(), dev)
+    a.src, a.src_is64, a.slots_out = _ptr(parents), parents.dtype == torch.int64, _ptr(slots)
+    return _ready("kda_pool_fork_launch" if parents.numel() else None, dev, a, 3, {0: ["used"], 1: ["src"], 2: ["status"]},
+                  [(slots, ["slots_out"]), (ws, ["workspace"])], (-1,), len(pools), [0])
 
 
 def pool_fork(pools, used, parents, *, status=None):
     """A slot for each entry of `parents`, in order the lowest free ones: marked used, and filled with the parent's row of every
     pool (a negative parent: a new sequence, zeros).  Returns the slots, int32; -1 where the parent is out of range or was not in
     use before the call (bit 2) and where no slot was left (bit 32)."""
+    return _call(_fork, (used, parents, status, *_pools(pools)))[0]
+
+
+def _free(used, slots, status):
     dev, P = _used(used)
-    _index(parents, "parents", dev)
-    slots = torch.empty(parents.numel(), dtype=torch.int32, device=dev)
-    a, dev = _args(pools, used, status, dev, P, [], [("parents", parents)])
-    if parents.numel() == 0:
-        return slots
-    ws = _workspace(a, parents.numel(), dev)
-    a.src, a.src_is64, a.slots_out = parents.data_ptr(), parents.dtype == torch.int64, slots.data_ptr()
-    _enqueue("kda_pool_fork_launch", a, dev)
-    del ws
-    return slots
+    _index(slots, "slots", dev)
+    a, dev = _args([], used, status, dev, P, [], [("slots", slots)])
+    a.n, a.src, a.src_is64 = slots.numel(), _ptr(slots), slots.dtype == torch.int64
+    return _ready("kda_pool_free_launch" if slots.numel() else None, dev, a, 3, {0: ["used"], 1: ["src"], 2: ["status"]}, [], (), 0, [0])
 
 
 def pool_free(used, slots, *, status=None):
     """Marks slots free (negative entries: padding).  Bit 2: one is out of range, free already or named twice."""
-    dev, P = _used(used)
-    _index(slots, "slots", dev)
-    a, dev = _args([], used, status, dev, P, [], [("slots", slots)])
-    if slots.numel() == 0:
-        return
-    a.n, a.src, a.src_is64 = slots.numel(), slots.data_ptr(), slots.dtype == torch.int64
-    _enqueue("kda_pool_free_launch", a, dev)
+    _call(_free, (used, slots, status))
 
 
-def pool_compact(pools, used, tables=(), *, status=None):
-    """With m slots in use, moves those behind the first m, in order, into the holes among them: `used` becomes m ones and then
-    zeros, and the entries of `tables` (slot tables, at most 8; negative entries: padding) follow.  An entry that names no slot in
-    use becomes -1 (bit 2).  Returns where each slot went, int32 [P], -1 for those that were free."""
+def _compact(*tensors):
+    used, status, *rest = tensors[:-1]
+    tables, pools = rest[:tensors[-1]], rest[tensors[-1]:]
     dev, P = _used(used)
-    if not isinstance(tables, (list, tuple)) or len(tables) > _cabi.MAX_TABLES:
-        raise _err(f"tables must be a list of at most {_cabi.MAX_TABLES} tensors")
     remap = torch.empty(P, dtype=torch.int32, device=dev)
     for i, t in enumerate(tables):
         _index(t, f"tables[{i}]", dev)
@@ -148,6 +160,15 @@ def pool_compact(pools, used, tables=(), *, status=None):
         a.tables[i], a.table_n[i], a.table_is64[i] = _ptr(t), t.numel(), t.dtype == torch.int64
     a.n_tables, a.remap = len(tables), remap.data_ptr()
     ws = _workspace(a, 0, dev)
-    _enqueue("kda_pool_compact_launch", a, dev)
-    del ws
-    return remap
+    given = {0: ["used"], 1: ["status"], **{2 + i: [f"tables[{i}]"] for i in range(len(tables))}}
+    return _ready("kda_pool_compact_launch", dev, a, 2 + len(tables), given, [(remap, ["remap"]), (ws, ["workspace"])], (-1,), len(pools),
+                  [0, *range(2, 2 + len(tables))])
+
+
+def pool_compact(pools, used, tables=(), *, status=None):
+    """With m slots in use, moves those behind the first m, in order, into the holes among them: `used` becomes m ones and then
+    zeros, and the entries of `tables` (slot tables, at most 8; negative entries: padding) follow.  An entry that names no slot in
+    use becomes -1 (bit 2).  Returns where each slot went, int32 [P], -1 for those that were free."""
+    if not isinstance(tables, (list, tuple)) or len(tables) > _cabi.MAX_TABLES:
+        raise _err(f"tables must be a list of at most {_cabi.MAX_TABLES} tensors")
+    return _call(_compact, (used, status, *tables, *_pools(pools)), len(tables))[0]

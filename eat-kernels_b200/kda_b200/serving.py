@@ -23,14 +23,88 @@ import ctypes as C
 
 import torch
 
-from . import D, LOWER_BOUND, _cabi, _err, _reject_aliasing, _table
+from . import D, LOWER_BOUND, _byte_interval, _cabi, _err, _reject_aliasing, _table
 
 TYPES = {torch.bfloat16: _cabi.TYPE_BF16, torch.float16: _cabi.TYPE_FP16, torch.float32: _cabi.TYPE_FP32}
 INT32_MAX = 0x7fffffff
 
 
-def _enqueue(name, args, dev):
-    entry = getattr(_cabi.lib(), name)
+class _Ready:
+    """A checked call: the argument block, where the pointers of the caller's tensors and of the ones made for this call go in it,
+    and what it returns."""
+
+    def __init__(self, name, dev, args, given, fresh, result, written=(), aligned=()):
+        self.name, self.dev, self.args = name, dev, args
+        self.given = given            # {index among the caller's tensors: names of pointer fields}
+        self.fresh = fresh            # [(tensor made for this call, names of pointer fields)]
+        self.result = result          # indices among the caller's tensors, or -1 - index in `fresh`
+        self.written = written        # caller's tensors that the call writes
+        self.aligned = aligned        # caller's tensors that must lie on 16 bytes
+
+
+def _offset(block, field):
+    """Byte offset of a field, "a.b" in a nested block and "a[i]" in an array."""
+    at = 0
+    for part in field.split("."):
+        part, _, i = part.partition("[")
+        f = getattr(block, part)
+        at += f.offset
+        kind = dict(block._fields_)[part]
+        if i:
+            at += int(i[:-1]) * C.sizeof(kind._type_)
+        block = kind
+    return at
+
+
+class _Plan:
+    """What the checks of a call found, for later calls whose tensors have the same types, shapes, strides and devices: the argument
+    block without its pointers.  Nothing of the tensors themselves is kept."""
+
+    def __init__(self, ready, tensors):
+        block = type(ready.args)
+        self.words = C.c_uint64 * (C.sizeof(block) // 8)
+        self.template = bytes(ready.args)
+        self.given = [(_offset(block, f) // 8, i) for i, fields in ready.given.items() if tensors[i] is not None for f in fields]
+        self.fresh = [([_offset(block, f) // 8 for f in fields], t.shape, t.dtype) for t, fields in ready.fresh]
+        self.result, self.written, self.aligned = ready.result, [i for i in ready.written if tensors[i] is not None], ready.aligned
+        self.present = [i for i, t in enumerate(tensors) if t is not None]
+        spans = [_byte_interval(t) for t in tensors]
+        self.reach = [0 if s is None else s[1] - s[0] for s in spans]
+        self.name, self.dev = ready.name, ready.dev
+        self.entry = _cabi.raw(ready.name)
+
+    def run(self, tensors):
+        """The call's results, or None where the tensors' addresses need another look."""
+        at = [0] * len(tensors)
+        for i in self.present:
+            at[i] = tensors[i].data_ptr()
+        for i in self.aligned:
+            if at[i] & 15:
+                return None
+        reach = self.reach
+        for w in self.written:
+            lo, hi = at[w], at[w] + reach[w]
+            for i in self.present:
+                if i != w and at[i] < hi and lo < at[i] + reach[i]:
+                    return None
+        args, dev = self.words.from_buffer_copy(self.template), self.dev
+        for word, i in self.given:
+            args[word] = at[i]
+        fresh = []
+        for words, shape, dtype in self.fresh:
+            t = torch.empty(shape, dtype=dtype, device=dev)
+            fresh.append(t)
+            for word in words:
+                args[word] = t.data_ptr()
+        _launch(self.entry, self.name, args, dev)
+        return tuple([tensors[i] if i >= 0 else fresh[-1 - i] for i in self.result])
+
+
+_plans = {}
+PLANS_MAX = 1024          # layouts remembered; a program that has more starts over
+
+
+def _launch(entry, name, args, dev):
     if torch.cuda.current_device() == dev.index:
         rc = entry(args, torch.cuda.current_stream(dev).cuda_stream)
     else:
@@ -38,6 +112,31 @@ def _enqueue(name, args, dev):
             rc = entry(args, torch.cuda.current_stream(dev).cuda_stream)
     if rc:
         _cabi.check(rc, name)
+
+
+def _call(check, tensors, *options):
+    """Runs `check`, which returns a _Ready, and what it found; a layout that has been checked before goes straight to the launch."""
+    try:
+        key = (check, options, *[t if t is None else (t.dtype, t.shape, t.stride(), t.device) for t in tensors])
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):                # not tensors: the checks say so
+        key = plan = None
+    if plan is not None:
+        result = plan.run(tensors)
+        if result is not None:
+            return result
+    ready = check(*tensors, *options)
+    if ready.name is not None:
+        _launch(_cabi.raw(ready.name), ready.name, C.byref(ready.args), ready.dev)
+        block = type(ready.args)
+        raw = bytes(ready.args)
+        same = all(int.from_bytes(raw[o:o + 8], "little") == tensors[i].data_ptr() for i, fields in ready.given.items()
+                   if tensors[i] is not None for o in (_offset(block, f) for f in fields))
+        if key is not None and same:                   # nothing was copied on the way
+            if len(_plans) >= PLANS_MAX:
+                _plans.clear()
+            _plans[key] = _Plan(ready, tensors)
+    return tuple([tensors[i] if i >= 0 else ready.fresh[-1 - i][0] for i in ready.result])
 
 
 def _cuda(dev, **tensors):
@@ -176,7 +275,7 @@ def _step_slots(dev, slots, N, pool):
 
 
 # ------------------------------------------------------------------------------------------------ short convolution
-def _conv(x, weight, bias, state, cu_seqlens, activation, slots, out, status, step):
+def _conv(x, weight, bias, state, cu_seqlens, slots, out, status, activation, step):
     T = _lead(x, "x", 1)
     dev, channels = x.device, x.shape[2]
     if x.dtype not in TYPES:
@@ -210,9 +309,12 @@ def _conv(x, weight, bias, state, cu_seqlens, activation, slots, out, status, st
     args = _cabi.KdaConvArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(src), _ptr(dst), ldx, _rows(y)[1], src_stride, dst_stride,
                              _sequences(dev, T, N, cu, slots, n_slots, status, int(out is None)), channels, W, TYPES[x.dtype],
                              TYPES[weight.dtype], int(activation is not None))
-    if not step or T:
-        _enqueue("kda_short_conv_step_launch" if step else "kda_short_conv_launch", args, dev)
-    return y, dst
+    given = {0: ["x"], 1: ["weight"], 2: ["bias"], 4: ["seq.cu_seqlens"], 5: ["seq.slots"], 6: ["out"], 7: ["seq.status"]}
+    given[3] = ["src", "dst"] if in_place else ["src"]
+    fresh = ([(y, ["out"])] if out is None else []) + ([] if in_place else [(dst, ["dst"])])
+    result = (6 if out is not None else -1, 3 if in_place else -len(fresh))
+    name = None if step and not T else "kda_short_conv_step_launch" if step else "kda_short_conv_launch"
+    return _Ready(name, dev, args, given, fresh, result, [6] + [3] * in_place)
 
 
 def short_conv(x, weight, bias=None, initial_state=None, cu_seqlens=None, *, activation="silu", ssm_state_indices=None, out=None,
@@ -222,16 +324,16 @@ def short_conv(x, weight, bias=None, initial_state=None, cu_seqlens=None, *, act
     x [1, T, C] bf16, fp16 or fp32 (any token stride); weight [C, W] or [C, 1, W], W of 2 to 4, in any of these types, bias [C] in
     weight's type; activation "silu" or None.  State: the last W - 1 rows of a sequence, oldest first, in x's type: a pool
     [P, W - 1, C] with `ssm_state_indices`, else [N, W - 1, C].  Returns (y, pool or final state)."""
-    return _conv(x, weight, bias, initial_state, cu_seqlens, activation, ssm_state_indices, out, status, False)
+    return _call(_conv, (x, weight, bias, initial_state, cu_seqlens, ssm_state_indices, out, status), activation, False)
 
 
 def short_conv_step(x, weight, bias, pool, ssm_state_indices=None, *, activation="silu", out=None, status=None):
     """The convolution of the next token of each row, x [1, N, C]; the pool's slots move on by a row.  Returns (y, pool)."""
-    return _conv(x, weight, bias, pool, None, activation, ssm_state_indices, out, status, True)
+    return _call(_conv, (x, weight, bias, pool, None, ssm_state_indices, out, status), activation, True)
 
 
 # ------------------------------------------------------------------------------------------------ selective scan
-def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, softplus, slots, out, status, step):
+def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, slots, out, status, softplus, step):
     T = _lead(u, "u", 1)
     dev, channels = u.device, u.shape[2]
     if u.dtype not in TYPES:
@@ -279,9 +381,15 @@ def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, softplus, slots,
                              ldu, lddt, ldb, ldc, ldz, _rows(y)[1], src_stride, dst_stride,
                              _sequences(dev, T, N, cu, slots, n_slots, status, int(out is None)), channels, size, groups, TYPES[u.dtype],
                              int(bool(softplus)), _ptr(ws), ws_bytes)
-    if not step or T:
-        _enqueue("kda_selective_scan_step_launch" if step else "kda_selective_scan_launch", args, dev)
-    return y, dst
+    given = {i: [f] for i, f in enumerate(("u", "dt", "A", "B", "C", "D", "z", "dt_bias"))}
+    given.update({9: ["seq.cu_seqlens"], 10: ["seq.slots"], 11: ["out"], 12: ["seq.status"]})
+    given[8] = ["src", "dst"] if in_place else ["src"]
+    fresh = ([(y, ["out"])] if out is None else []) + ([] if in_place else [(dst, ["dst"])])
+    result = (11 if out is not None else -1, 8 if in_place else -len(fresh))
+    if ws is not None:
+        fresh.append((ws, ["workspace"]))
+    name = None if step and not T else "kda_selective_scan_step_launch" if step else "kda_selective_scan_launch"
+    return _Ready(name, dev, args, given, fresh, result, [11] + [8] * in_place)
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=None, cu_seqlens=None, *, dt_softplus=True,
@@ -293,16 +401,16 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     d // (channels / groups); A [channels, Ns] (Ns up to 128), D and dt_bias [channels] fp32; D, z and dt_bias may be None, and
     dt_softplus=False takes s = dt + dt_bias.  State fp32: a pool [P, channels, Ns] with `ssm_state_indices`, else
     [N, channels, Ns].  Returns (y, pool or final state)."""
-    return _scan(u, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, dt_softplus, ssm_state_indices, out, status, False)
+    return _call(_scan, (u, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, ssm_state_indices, out, status), bool(dt_softplus), False)
 
 
 def selective_scan_step(u, dt, A, B, C, D, z, dt_bias, pool, ssm_state_indices=None, *, dt_softplus=True, out=None, status=None):
     """The scan of the next token of each row: u, dt, z [1, N, channels], B, C [1, N, groups, Ns].  Returns (y, pool)."""
-    return _scan(u, dt, A, B, C, D, z, dt_bias, pool, None, dt_softplus, ssm_state_indices, out, status, True)
+    return _call(_scan, (u, dt, A, B, C, D, z, dt_bias, pool, None, ssm_state_indices, out, status), bool(dt_softplus), True)
 
 
 # ------------------------------------------------------------------------------------------------ KDA, one token
-def _kda(q, k, v, g, beta, A_log, dt_bias, scale, pool, slots, out, status, raw):
+def _kda(q, k, v, g, beta, A_log, dt_bias, pool, slots, out, status, scale, raw):
     N = _lead(q, "q", 2)
     dev, H = q.device, q.shape[2]
     if q.shape[3] != D:
@@ -331,19 +439,19 @@ def _kda(q, k, v, g, beta, A_log, dt_bias, scale, pool, slots, out, status, raw)
     args = _cabi.KdaStepArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(y), _ptr(A_log), _ptr(dt_bias), _ptr(pool), ldq, ldk, ldv,
                              ldg, ldbeta, _rows(y)[1], stride, _sequences(dev, N, N, None, slots, pool.shape[0], status, int(out is None)),
                              float(scale), LOWER_BOUND, _cabi.FRONTEND_RAW if raw else _cabi.FRONTEND_PLAIN, H)
-    if N:
-        _enqueue("kda_step_launch", args, dev)
-    return y, pool
+    given = {i: [f] for i, f in enumerate(("q", "k", "v", "g", "beta", "A_log", "dt_bias", "pool", "seq.slots", "out", "seq.status"))}
+    fresh = [(y, ["out"])] if out is None else []
+    return _Ready("kda_step_launch" if N else None, dev, args, given, fresh, (9 if out is not None else -1, 7), [9, 7], [7])
 
 
 def kda_step(q, k, v, g, beta, A_log, dt_bias, scale, pool, ssm_state_indices=None, *, out=None, status=None):
     """The next token of each row after `kda_prefill`, on the same pool (fp32 [P, H, 128 (V), 128 (K)]): q, k, v, g [1, N, H, 128]
     and beta [1, N, H] bf16 with the gate, beta's sigmoid and the L2 norm of q, k computed in the kernel (other types are cast, as
     there).  Returns (o [1, N, H, 128] bf16, pool)."""
-    return _kda(q, k, v, g, beta, A_log, dt_bias, scale, pool, ssm_state_indices, out, status, True)
+    return _call(_kda, (q, k, v, g, beta, A_log, dt_bias, pool, ssm_state_indices, out, status), scale, True)
 
 
 def kda_step_plain(q, k, v, g, beta, scale, pool, ssm_state_indices=None, *, out=None, status=None):
     """The next token of each row after `chunk_kda`: g the fp32 log-decay, beta fp32 in (0, 1), q, k normalised, the pool key-first
     [P, H, 128 (K), 128 (V)].  Returns (o [1, N, H, 128] bf16, pool)."""
-    return _kda(q, k, v, g, beta, None, None, q.shape[-1] ** -0.5 if scale is None else scale, pool, ssm_state_indices, out, status, False)
+    return _call(_kda, (q, k, v, g, beta, None, None, pool, ssm_state_indices, out, status), D ** -0.5 if scale is None else scale, False)
