@@ -8,21 +8,43 @@ namespace kda {
 namespace {
 
 constexpr int CONV_THREADS = 128;
+constexpr int GROUP = 8;                 // rows in flight
 
-__device__ __forceinline__ float weight_at(const void* p, int type, long long i) {
-  if (type == TYPE_BF16) return to_float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  if (type == TYPE_FP16) return to_float(reinterpret_cast<const __half*>(p)[i]);
-  return reinterpret_cast<const float*>(p)[i];
+// N consecutive values, in 8-byte accesses where they start on 8 bytes
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, float (&f)[N]) {
+  constexpr int PER = 8 / sizeof(T);
+  if (N % PER == 0 && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+#pragma unroll
+    for (int i = 0; i < N / PER; i++) {
+      const Pack<T, PER> v = reinterpret_cast<const Pack<T, PER>*>(p)[i];
+#pragma unroll
+      for (int j = 0; j < PER; j++) f[i * PER + j] = to_float(v.v[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = to_float(p[i]);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void load_run(const void* p, int type, long long at, float (&f)[N]) {
+  if (type == TYPE_BF16) load_run(reinterpret_cast<const __nv_bfloat16*>(p) + at, f);
+  else if (type == TYPE_FP16) load_run(reinterpret_cast<const __half*>(p) + at, f);
+  else load_run(reinterpret_cast<const float*>(p) + at, f);
 }
 
 template <int VEC, int W>
 __device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (&w)[W][VEC], float (&b)[VEC]) {
+  float run[VEC * W];
+  load_run(p.weight, p.weight_type, (long long)c * W, run);
 #pragma unroll
   for (int i = 0; i < VEC; i++) {
 #pragma unroll
-    for (int j = 0; j < W; j++) w[j][i] = weight_at(p.weight, p.weight_type, (long long)(c + i) * W + j);
-    b[i] = p.bias != nullptr ? weight_at(p.bias, p.weight_type, c + i) : 0.0f;
+    for (int j = 0; j < W; j++) w[j][i] = run[i * W + j];
+    b[i] = 0.0f;
   }
+  if (p.bias != nullptr) load_run(p.bias, p.weight_type, c, b);
 }
 
 // VEC channels a thread, a tile of tokens a block.  A sequence's first W - 1 tokens belong to the tile that holds its start,
@@ -48,38 +70,40 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const Conv
 #pragma unroll
   for (int i = 0; i < VEC; i++) zero.v[i] = from_float<T>(0.0f);
 
-  const bool rejected = cu_rejected(p.seq);
+  int lo;                                            // the first sequence that starts in this tile
+  const bool rejected = cu_rejected(p.seq, t0, lo);
   float w[W][VEC], b[VEC];
   if (mine) load_weights<VEC, W>(p, c, w, b);
 
-  auto run = [&](long long from, long long to, float (&win)[HW][VEC]) {
-#pragma unroll 4
-    for (long long t = from; t < to; t++) {
-      float cur[VEC], y[VEC];
-      unpack(*reinterpret_cast<const P*>(x + t * p.ldx), cur);
+  auto token = [&](long long t, const P& row, float (&win)[HW][VEC]) {
+    float cur[VEC], y[VEC];
+    unpack(row, cur);
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        float acc = b[i];
+    for (int i = 0; i < VEC; i++) {
+      float acc = b[i];
 #pragma unroll
-        for (int j = 0; j < HW; j++) acc = fmaf(w[j][i], win[j][i], acc);
-        acc = fmaf(w[HW][i], cur[i], acc);
-        y[i] = p.silu ? silu<T>(acc) : acc;
+      for (int j = 0; j < HW; j++) acc = fmaf(w[j][i], win[j][i], acc);
+      acc = fmaf(w[HW][i], cur[i], acc);
+      y[i] = p.silu ? silu<T>(acc) : acc;
 #pragma unroll
-        for (int j = 0; j + 1 < HW; j++) win[j][i] = win[j + 1][i];
-        win[HW - 1][i] = cur[i];
-      }
-      *reinterpret_cast<P*>(out + t * p.ldo) = pack<T, VEC>(y);
+      for (int j = 0; j + 1 < HW; j++) win[j][i] = win[j + 1][i];
+      win[HW - 1][i] = cur[i];
     }
+    *reinterpret_cast<P*>(out + t * p.ldo) = pack<T, VEC>(y);
+  };
+  // tokens in groups: a group's rows are all on their way before the first is used
+  auto run = [&](long long from, long long to, float (&win)[HW][VEC]) {
+    for (; from + GROUP <= to; from += GROUP) {
+      P rows[GROUP];
+#pragma unroll
+      for (int g = 0; g < GROUP; g++) rows[g] = *reinterpret_cast<const P*>(x + (from + g) * p.ldx);
+#pragma unroll
+      for (int g = 0; g < GROUP; g++) token(from + g, rows[g], win);
+    }
+    for (; from < to; from++) token(from, *reinterpret_cast<const P*>(x + from * p.ldx), win);
   };
 
-  // the first sequence that starts in this tile, and the one that reaches into it
-  int lo = 0, hi = N + 1;
-  if (!rejected) {
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (cu_at(p.seq, mid) >= t0) hi = mid; else lo = mid + 1;
-    }
-  }
+  // the sequence that reaches into this tile
   if (!rejected && mine && lo > 0 && lo <= N) {
     const long long begin = cu_at(p.seq, lo - 1), end = cu_at(p.seq, lo);
     const long long from = max(t0, begin + HW), to = min(end, t1);
@@ -121,66 +145,81 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const Conv
     for (long long t = rejected ? t0 : max(t0, cu_at(p.seq, N)); t < t1; t++) *reinterpret_cast<P*>(out + t * p.ldo) = zero;
 }
 
-// One token a row, VEC channels a thread: the window is the slot's history and the token.
+// One token a row, VEC channels a thread: the window is the slot's history and the token.  A block takes ROWS rows for one load of
+// the weights, all their histories in flight at once.
+constexpr int STEP_ROWS = 4;
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const ConvParams p) {
   constexpr int HW = W - 1;
   using P = Pack<T, VEC>;
   const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
-  const int row = blockIdx.x / cblocks;
+  const long long row0 = (long long)(blockIdx.x / cblocks) * p.tile;
+  const int rows = (int)min((long long)p.tile, p.seq.T - row0);
   const int c = ((int)(blockIdx.x % cblocks) * CONV_THREADS + (int)threadIdx.x) * VEC;
-  const long long slot = claim_row(p.seq, row);
+  long long slot[STEP_ROWS];
+#pragma unroll
+  for (int r = 0; r < STEP_ROWS; r++) slot[r] = r < rows ? claim_row(p.seq, (int)(row0 + r)) : -2;
   if (c >= p.C) return;
-  P* out = reinterpret_cast<P*>(reinterpret_cast<T*>(p.out) + row * p.ldo + c);
-  float y[VEC];
-  if (slot == -2) {
+  T* pool = reinterpret_cast<T*>(p.dst) + c;
+  P hist[STEP_ROWS][HW], cur[STEP_ROWS];
 #pragma unroll
-    for (int i = 0; i < VEC; i++) y[i] = 0.0f;
-    if (p.zero_pad) *out = pack<T, VEC>(y);
-    return;
+  for (int r = 0; r < STEP_ROWS; r++) {
+    if (slot[r] != -2) cur[r] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + (row0 + r) * p.ldx + c);
+#pragma unroll
+    for (int j = 0; j < HW; j++)
+      if (slot[r] >= 0) hist[r][j] = *reinterpret_cast<const P*>(pool + slot[r] * p.dst_stride + (long long)j * p.C);
   }
-  float w[W][VEC];
-  load_weights<VEC, W>(p, c, w, y);
-  T* pool = reinterpret_cast<T*>(p.dst) + slot * p.dst_stride + c;
-  const P cur = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + row * p.ldx + c);
-  P hist[HW];
-  if (slot >= 0) {
+  float w[W][VEC], b[VEC];
+  load_weights<VEC, W>(p, c, w, b);
 #pragma unroll
-    for (int j = 0; j < HW; j++) hist[j] = *reinterpret_cast<const P*>(pool + (long long)j * p.C);
+  for (int r = 0; r < STEP_ROWS; r++) {
+    if (r >= rows) break;
+    P* out = reinterpret_cast<P*>(reinterpret_cast<T*>(p.out) + (row0 + r) * p.ldo + c);
+    float y[VEC], f[VEC];
+    if (slot[r] == -2) {
 #pragma unroll
-    for (int j = 0; j + 1 < HW; j++) *reinterpret_cast<P*>(pool + (long long)j * p.C) = hist[j + 1];
-    *reinterpret_cast<P*>(pool + (long long)(HW - 1) * p.C) = cur;
-#pragma unroll
-    for (int j = 0; j < HW; j++) {
-      float f[VEC];
-      unpack(hist[j], f);
-#pragma unroll
-      for (int i = 0; i < VEC; i++) y[i] = fmaf(w[j][i], f[i], y[i]);
+      for (int i = 0; i < VEC; i++) y[i] = 0.0f;
+      if (p.zero_pad) *out = pack<T, VEC>(y);
+      continue;
     }
-  }
-  float f[VEC];
-  unpack(cur, f);
 #pragma unroll
-  for (int i = 0; i < VEC; i++) {
-    y[i] = fmaf(w[HW][i], f[i], y[i]);
-    if (p.silu) y[i] = silu<T>(y[i]);
+    for (int i = 0; i < VEC; i++) y[i] = b[i];
+    if (slot[r] >= 0) {
+      T* to = pool + slot[r] * p.dst_stride;
+#pragma unroll
+      for (int j = 0; j + 1 < HW; j++) *reinterpret_cast<P*>(to + (long long)j * p.C) = hist[r][j + 1];
+      *reinterpret_cast<P*>(to + (long long)(HW - 1) * p.C) = cur[r];
+#pragma unroll
+      for (int j = 0; j < HW; j++) {
+        unpack(hist[r][j], f);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) y[i] = fmaf(w[j][i], f[i], y[i]);
+      }
+    }
+    unpack(cur[r], f);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) {
+      y[i] = fmaf(w[HW][i], f[i], y[i]);
+      if (p.silu) y[i] = silu<T>(y[i]);
+    }
+    *out = pack<T, VEC>(y);
   }
-  *out = pack<T, VEC>(y);
 }
 
-// 16-byte accesses where every row starts on 16 bytes, single values elsewhere.
+// Four channels an access where every row starts on as many, single values elsewhere.  Eight 16-bit channels take 187 registers, which
+// leaves two blocks an SM: 471 us for 56 k tokens of 6144 channels against 273 us with four.
+constexpr int WIDE = 4;
 template <typename T>
 bool wide(const ConvParams& p) {
-  constexpr int VEC = 16 / sizeof(T);
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.src) |
                        reinterpret_cast<uintptr_t>(p.dst);
-  return (at & 15) == 0 && ((p.C | p.ldx | p.ldo | p.src_stride | p.dst_stride) & (VEC - 1)) == 0;
+  return (at & (WIDE * sizeof(T) - 1)) == 0 && ((p.C | p.ldx | p.ldo | p.src_stride | p.dst_stride) & (WIDE - 1)) == 0;
 }
 
 template <typename T, int VEC>
 cudaError_t launch_width(const ConvParams& p, bool step, cudaStream_t stream) {
   const long long cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
-  const long long rows = step ? p.seq.T : (p.seq.T > 0 ? (p.seq.T + p.tile - 1) / p.tile : 1);
+  const long long rows = step || p.seq.T > 0 ? (p.seq.T + p.tile - 1) / p.tile : 1;
   const long long blocks = cblocks * rows;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (blocks == 0) return cudaSuccess;
@@ -191,11 +230,20 @@ cudaError_t launch_width(const ConvParams& p, bool step, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+// Rows of a block: as many as leave two blocks an SM, so that small calls spread over the card and large ones share weights and
+// the rows in front of a tile.
+int tile_of(long long rows, long long cblocks, int least, int most) {
+  int tile = most;
+  while (tile > least && (rows + tile - 1) / tile * cblocks < 2 * 148) tile /= 2;
+  return tile;
+}
+
 template <typename T>
 cudaError_t launch_type(ConvParams p, bool step, cudaStream_t stream) {
-  p.tile = 32;
-  if (wide<T>(p)) return launch_width<T, 16 / sizeof(T)>(p, step, stream);
-  return launch_width<T, 1>(p, step, stream);
+  const bool w = wide<T>(p);
+  const long long cblocks = (p.C / (w ? WIDE : 1) + CONV_THREADS - 1) / CONV_THREADS;
+  p.tile = step ? tile_of(p.seq.T, cblocks, 1, STEP_ROWS) : tile_of(p.seq.T, cblocks, 8, 128);
+  return w ? launch_width<T, WIDE>(p, step, stream) : launch_width<T, 1>(p, step, stream);
 }
 
 cudaError_t launch_any(const ConvParams& p, int type, bool step, cudaStream_t stream) {

@@ -46,6 +46,25 @@ __device__ __forceinline__ bool cu_rejected(const SeqTable& s) {
   return rejected;
 }
 
+// The same, and how many entries lie below t (of a layout that is not rejected: the first sequence that starts at t or behind).
+__device__ __forceinline__ bool cu_rejected(const SeqTable& s, long long t, int& below) {
+  int bad = 0;
+  below = 0;
+  for (int i0 = 0; i0 <= s.N; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x;
+    long long c0 = t;
+    if (i <= s.N) {
+      c0 = cu_at(s, i);
+      const long long c1 = i < s.N ? cu_at(s, i + 1) : c0;
+      if (c0 < 0 || c0 > s.T || c1 < c0 || (i == 0 && c0 != 0)) bad = 1;
+    }
+    below += __syncthreads_count(c0 < t);
+  }
+  const bool rejected = __syncthreads_or(bad) != 0;
+  if (rejected && threadIdx.x == 0) report(s.status, SEQ_BAD_CU);
+  return rejected;
+}
+
 // Called by the whole block: the slot of sequence i, or -1 where its entry is out of range or repeats an earlier one (the
 // first claim keeps the slot, as in the prefill's planner).
 __device__ __forceinline__ long long claim_slot(const SeqTable& s, int i) {

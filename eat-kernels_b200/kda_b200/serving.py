@@ -448,10 +448,10 @@ def kda_step(q, k, v, g, beta, A_log, dt_bias, scale, pool, ssm_state_indices=No
     """The next token of each row after `kda_prefill`, on the same pool (fp32 [P, H, 128 (V), 128 (K)]): q, k, v, g [1, N, H, 128]
     and beta [1, N, H] bf16 with the gate, beta's sigmoid and the L2 norm of q, k computed in the kernel (other types are cast, as
     there).  Returns (o [1, N, H, 128] bf16, pool)."""
-    return _call(_kda, (q, k, v, g, beta, A_log, dt_bias, pool, ssm_state_indices, out, status), scale, True)
+    return _call(_kda, (q, k, v, g, beta, A_log, dt_bias, pool, ssm_state_indices, out, status), float(scale), True)
 
 
 def kda_step_plain(q, k, v, g, beta, scale, pool, ssm_state_indices=None, *, out=None, status=None):
     """The next token of each row after `chunk_kda`: g the fp32 log-decay, beta fp32 in (0, 1), q, k normalised, the pool key-first
     [P, H, 128 (K), 128 (V)].  Returns (o [1, N, H, 128] bf16, pool)."""
-    return _call(_kda, (q, k, v, g, beta, None, None, pool, ssm_state_indices, out, status), D ** -0.5 if scale is None else scale, False)
+    return _call(_kda, (q, k, v, g, beta, None, None, pool, ssm_state_indices, out, status), D ** -0.5 if scale is None else float(scale), False)
