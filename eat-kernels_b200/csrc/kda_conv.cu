@@ -157,18 +157,19 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const
   const int rows = (int)min((long long)p.tile, p.seq.T - row0);
   const int c = ((int)(blockIdx.x % cblocks) * CONV_THREADS + (int)threadIdx.x) * VEC;
   long long slot[STEP_ROWS];
-#pragma unroll
-  for (int r = 0; r < STEP_ROWS; r++) slot[r] = r < rows ? claim_row(p.seq, (int)(row0 + r)) : -2;
-  if (c >= p.C) return;
+  row_slots(p.seq, row0, rows, slot);
+  const bool mine = c < p.C;
   T* pool = reinterpret_cast<T*>(p.dst) + c;
   P hist[STEP_ROWS][HW], cur[STEP_ROWS];
 #pragma unroll
   for (int r = 0; r < STEP_ROWS; r++) {
-    if (slot[r] != -2) cur[r] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + (row0 + r) * p.ldx + c);
+    if (mine && slot[r] != -2) cur[r] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + (row0 + r) * p.ldx + c);
 #pragma unroll
     for (int j = 0; j < HW; j++)
-      if (slot[r] >= 0) hist[r][j] = *reinterpret_cast<const P*>(pool + slot[r] * p.dst_stride + (long long)j * p.C);
+      if (mine && slot[r] >= 0) hist[r][j] = *reinterpret_cast<const P*>(pool + slot[r] * p.dst_stride + (long long)j * p.C);
   }
+  drop_repeats(p.seq, row0, slot);
+  if (!mine) return;
   float w[W][VEC], b[VEC];
   load_weights<VEC, W>(p, c, w, b);
 #pragma unroll

@@ -78,10 +78,40 @@ __device__ __forceinline__ long long claim_slot(const SeqTable& s, int i) {
   return -1;
 }
 
-// The same for a row of a step, where a negative entry stands for a row of padding: -2.
-__device__ __forceinline__ long long claim_row(const SeqTable& s, int i) {
-  if (s.slots != nullptr && table_at(s.slots, s.slots_is64, i) < 0) return -2;
-  return claim_slot(s, i);
+// The slots of R rows of a step from row0 on, `rows` of them there are, in two parts, so that a block can ask for the states before
+// it has looked for repeats.  First: a slot, -1 for an entry out of range, -2 for a row of padding (a negative entry) or none.
+template <int R>
+__device__ __forceinline__ void row_slots(const SeqTable& s, long long row0, int rows, long long (&slot)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    slot[r] = -2;
+    if (r < rows) {
+      slot[r] = s.slots != nullptr ? table_at(s.slots, s.slots_is64, row0 + r) : row0 + r;
+      if (slot[r] < 0) slot[r] = -2;
+      else if (slot[r] >= s.n_slots) slot[r] = -1;
+    }
+  }
+}
+
+// Then, called by the whole block: -1 for a slot that an earlier row has claimed too.
+template <int R>
+__device__ __forceinline__ void drop_repeats(const SeqTable& s, long long row0, long long (&slot)[R]) {
+  if (s.slots == nullptr) return;
+  int bad = 0;
+  for (int j = threadIdx.x; j < (int)row0 + R - 1; j += blockDim.x) {
+    const long long d = j < s.N ? table_at(s.slots, s.slots_is64, j) : -1;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      if (d >= 0 && d == slot[r] && j < row0 + r) bad |= 1 << r;
+  }
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if (slot[r] == -1) bad |= 1 << r;
+  if (__syncthreads_or(bad) == 0) return;
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if (__syncthreads_or(bad >> r & 1)) slot[r] = -1;
+  if (threadIdx.x == 0) report(s.status, SEQ_BAD_SLOT);
 }
 
 // ---- token types

@@ -100,6 +100,27 @@ struct RawShared {
   } slot[DEPTH];
 };
 
+template <int S>
+struct Values {
+  float v[S] = {};
+};
+// S consecutive values in one access
+template <int S>
+__device__ __forceinline__ Values<S> load_values(const float* p) {
+  Values<S> r;
+  const Pack<float, S> v = *reinterpret_cast<const Pack<float, S>*>(p);
+#pragma unroll
+  for (int k = 0; k < S; k++) r.v[k] = v.v[k];
+  return r;
+}
+template <int S>
+__device__ __forceinline__ void store_values(float* p, const Values<S>& v) {
+  Pack<float, S> f;
+#pragma unroll
+  for (int k = 0; k < S; k++) f.v[k] = v.v[k];
+  *reinterpret_cast<Pack<float, S>*>(p) = f;
+}
+
 template <int L, int S>
 struct ScanShared {
   static constexpr int CB = SCAN_LANES / L;          // channels of a block
@@ -543,46 +564,118 @@ __global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(c
   }
 }
 
-// One token a row: L lanes hold a channel's state, S values each.  Bound by memory: the state goes through once.
-template <typename T, int L, int S>
+// One token a row, ROWS rows a block for one load of A.  L lanes hold a channel's state, S consecutive values each; lane r works out
+// the step, the gate and the output of row r and hands the step round.  Bound by memory: the states of all rows are asked for before
+// anything else, and go through once.
+constexpr int ROWS = 4;
+template <typename T, int L, int S, bool WIDE>
 __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(const ScanParams p) {
+  static_assert(L >= ROWS, "a lane for each row");
   constexpr int CB = STEP_LANES / L;
-  const int cblocks = (p.Dm + CB - 1) / CB;
-  const long long row = blockIdx.x / cblocks;
-  const int lane = threadIdx.x % L, d = (int)(blockIdx.x % cblocks) * CB + threadIdx.x / L;
+  const int lane = threadIdx.x % L;
+  const long long row0 = (long long)blockIdx.y * ROWS;
+  const int rows = (int)min((long long)ROWS, p.seq.T - row0);
+  const int d = (int)blockIdx.x * CB + threadIdx.x / L;
   const bool mine = d < p.Dm;
-  const int dc = mine ? d : p.Dm - 1;
-  const int group = dc / (p.Dm / p.groups);
-  const long long slot = claim_row(p.seq, (int)row);
-  T* out = reinterpret_cast<T*>(p.out) + row * p.ldo + dc;
-  if (slot == -2) {
-    if (p.zero_pad && lane == 0 && mine) *out = from_float<T>(0.0f);
-    return;
-  }
-  const long long at = (long long)dc * p.Ns + lane * S;
-  float h[S];
+  const int dc = mine ? d : p.Dm - 1, group = p.groups > 1 ? dc / (p.Dm / p.groups) : 0, n = lane * S;
+  long long slot[ROWS];
+  row_slots(p.seq, row0, rows, slot);
+  const long long at = (long long)dc * p.Ns + n;
+  // S consecutive values of which `left` there are: one access where WIDE
+  auto values = [&](const float* q) {
+    Values<S> v;
+    if constexpr (WIDE) {
+      v = n < p.Ns ? load_values<S>(q) : Values<S>();
+    } else {
 #pragma unroll
-  for (int k = 0; k < S; k++) h[k] = lane * S + k < p.Ns && slot >= 0 ? p.src[slot * p.src_stride + at + k] : 0.0f;
-  const T* B = reinterpret_cast<const T*>(p.B) + row * p.ldb + (long long)group * p.Ns + lane * S;
-  const T* C = reinterpret_cast<const T*>(p.C) + row * p.ldc + (long long)group * p.Ns + lane * S;
-  const float u = to_float(reinterpret_cast<const T*>(p.u)[row * p.ldu + dc]);
-  float s = to_float(reinterpret_cast<const T*>(p.dt)[row * p.lddt + dc]) + (p.dt_bias != nullptr ? p.dt_bias[dc] : 0.0f);
+      for (int k = 0; k < S; k++) v.v[k] = n + k < p.Ns ? q[k] : 0.0f;
+    }
+    return v;
+  };
+  Values<S> h[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; r++)
+    if (slot[r] >= 0) h[r] = values(p.src + slot[r] * p.src_stride + at);
+  // lane r: row r
+  const long long mine_row = row0 + min(lane, rows - 1);
+  const float u = to_float(reinterpret_cast<const T*>(p.u)[mine_row * p.ldu + dc]);
+  float s = to_float(reinterpret_cast<const T*>(p.dt)[mine_row * p.lddt + dc]) + (p.dt_bias != nullptr ? p.dt_bias[dc] : 0.0f);
+  const float z = p.z != nullptr ? to_float(reinterpret_cast<const T*>(p.z)[mine_row * p.ldz + dc]) : 0.0f;
+  const float skip = p.D != nullptr ? p.D[dc] : 0.0f;
+  const Values<S> a = values(p.A + at);
   if (p.softplus) s = softplus(s);
-  float y = 0.0f;
+  const float su = s * u;
+  drop_repeats(p.seq, row0, slot);
+  float part[ROWS];
 #pragma unroll
-  for (int k = 0; k < S; k++)
-    if (lane * S + k < p.Ns) {
-      h[k] = fmaf(exp2_fast(s * p.A[at + k] * LOG2E_F), h[k], s * u * to_float(B[k]));
-      y = fmaf(to_float(C[k]), h[k], y);
-      if (slot >= 0 && mine) p.dst[slot * p.dst_stride + at + k] = h[k];
+  for (int r = 0; r < ROWS; r++) {
+    const float sr = __shfl_sync(0xffffffffu, s, r, L), sur = __shfl_sync(0xffffffffu, su, r, L);
+    part[r] = 0.0f;
+    if (slot[r] == -2) continue;
+    if (slot[r] == -1) h[r] = Values<S>();
+    const T* B = reinterpret_cast<const T*>(p.B) + (row0 + r) * p.ldb + (long long)group * p.Ns + n;
+    const T* C = reinterpret_cast<const T*>(p.C) + (row0 + r) * p.ldc + (long long)group * p.Ns + n;
+    float b[S], c[S];
+    if constexpr (WIDE) {
+      if (n < p.Ns) {
+        unpack(*reinterpret_cast<const Pack<T, S>*>(B), b);
+        unpack(*reinterpret_cast<const Pack<T, S>*>(C), c);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S; k++) b[k] = c[k] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < S; k++) {
+        b[k] = n + k < p.Ns ? to_float(B[k]) : 0.0f;
+        c[k] = n + k < p.Ns ? to_float(C[k]) : 0.0f;
+      }
     }
 #pragma unroll
-  for (int m = 1; m < L; m *= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
-  if (lane == 0 && mine) {
-    if (p.D != nullptr) y = fmaf(p.D[dc], u, y);
-    if (p.z != nullptr) y *= silu<T>(to_float(reinterpret_cast<const T*>(p.z)[row * p.ldz + dc]));
-    *out = from_float<T>(y);
+    for (int k = 0; k < S; k++) {
+      if (!WIDE && n + k >= p.Ns) continue;
+      h[r].v[k] = fmaf(exp2_fast(sr * a.v[k] * LOG2E_F), h[r].v[k], sur * b[k]);
+      part[r] = fmaf(c[k], h[r].v[k], part[r]);
+    }
+    if (slot[r] >= 0 && mine) {
+      float* to = p.dst + slot[r] * p.dst_stride + at;
+      if constexpr (WIDE) {
+        if (n < p.Ns) store_values<S>(to, h[r]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S; k++)
+          if (n + k < p.Ns) to[k] = h[r].v[k];
+      }
+    }
   }
+  // sums over the lanes: lane r ends with row r (L > ROWS: the first of L / ROWS lanes, which hands it on)
+#pragma unroll
+  for (int m = L / 2, k = ROWS / 2; m >= 1; m /= 2, k /= 2) {
+    if (k >= 1) {
+#pragma unroll
+      for (int r = 0; r < k; r++) {
+        const bool up = lane & m;
+        const float give = up ? part[r] : part[k + r], keep = up ? part[k + r] : part[r];
+        part[r] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+      }
+    } else {
+      part[0] += __shfl_xor_sync(0xffffffffu, part[0], m);
+    }
+  }
+  float y = __shfl_sync(0xffffffffu, part[0], min(lane, ROWS - 1) * (L / ROWS), L);
+  long long own = -2;
+#pragma unroll
+  for (int r = 0; r < ROWS; r++)
+    if (lane == r) own = slot[r];
+  if (lane >= rows || !mine) return;
+  T* out = reinterpret_cast<T*>(p.out) + mine_row * p.ldo + dc;
+  if (own == -2) {
+    if (p.zero_pad) *out = from_float<T>(0.0f);
+    return;
+  }
+  y = fmaf(skip, u, y);
+  if (p.z != nullptr) y *= silu<T>(z);
+  *out = from_float<T>(y);
 }
 
 template <typename T, int L, int S, bool LOCAL>
@@ -630,15 +723,22 @@ cudaError_t launch_type(ScanParams p, cudaStream_t stream) {
 
 template <typename T, int L, int S>
 cudaError_t launch_step(const ScanParams& p, cudaStream_t stream) {
-  const long long blocks = (long long)((p.Dm + STEP_LANES / L - 1) / (STEP_LANES / L)) * p.seq.N;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (blocks == 0) return cudaSuccess;
-  kda_selective_scan_step_kernel<T, L, S><<<(unsigned)blocks, STEP_LANES, 0, stream>>>(p);
+  const long long rows = (p.seq.T + ROWS - 1) / ROWS;
+  if (rows == 0) return cudaSuccess;
+  if (rows > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)((p.Dm + STEP_LANES / L - 1) / (STEP_LANES / L)), (unsigned)rows);
+  // one access for S values where all start on as many
+  const uintptr_t f = reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.A) | (uintptr_t)(p.src_stride * 4);
+  const uintptr_t t = reinterpret_cast<uintptr_t>(p.B) | reinterpret_cast<uintptr_t>(p.C) | (uintptr_t)((p.ldb | p.ldc) * (long long)sizeof(T));
+  if ((f & (S * 4 - 1)) == 0 && (t & (S * sizeof(T) - 1)) == 0 && p.Ns % S == 0) kda_selective_scan_step_kernel<T, L, S, true><<<grid, STEP_LANES, 0, stream>>>(p);
+  else kda_selective_scan_step_kernel<T, L, S, false><<<grid, STEP_LANES, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
+  if (p.Ns <= 4) return launch_step<T, 4, 1>(p, stream);
+  if (p.Ns <= 8) return launch_step<T, 4, 2>(p, stream);
   if (p.Ns <= 16) return launch_step<T, 4, 4>(p, stream);
   if (p.Ns <= 32) return launch_step<T, 8, 4>(p, stream);
   if (p.Ns <= 64) return launch_step<T, 16, 4>(p, stream);

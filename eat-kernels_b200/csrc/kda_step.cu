@@ -23,22 +23,25 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams
   constexpr bool KEY_FIRST = !RAW;
   __shared__ __align__(16) float s_k[D], s_q[D], s_a[D];
   __shared__ float s_v[STEP_ROWS], s_part[3][STEP_THREADS / 32], s_sum[2][STEP_THREADS / 32][STEP_ROWS];
-  const int part = blockIdx.x % (D / STEP_ROWS), head = (blockIdx.x / (D / STEP_ROWS)) % p.H;
-  const int row = blockIdx.x / (D / STEP_ROWS) / p.H;
+  const int part = blockIdx.x % (D / STEP_ROWS), head = blockIdx.y;
+  const long long row = blockIdx.x / (D / STEP_ROWS);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const long long slot = claim_row(p.seq, row);
+  long long slot[1];
+  row_slots(p.seq, row, 1, slot);
   __nv_bfloat16* out = p.out + row * p.ldo + head * D + part * STEP_ROWS;
-  if (slot == -2) {
+  if (slot[0] == -2) {
     if (p.zero_pad && tid < STEP_ROWS) out[tid] = __float2bfloat16_rn(0.0f);
     return;
   }
   // the state's 16 KB: element i of a thread
-  float* state = p.pool + (slot < 0 ? 0 : slot) * p.slot_stride + (long long)head * STATE_ELEMS;
+  float* state = p.pool + (slot[0] < 0 ? 0 : slot[0]) * p.slot_stride + (long long)head * STATE_ELEMS;
   state += KEY_FIRST ? (warp * 4 + lane / 8) * D + part * STEP_ROWS + (lane % 8) * 4 : (part * STEP_ROWS + warp * 8) * D + lane * 4;
   constexpr int NEXT = KEY_FIRST ? 16 * D : D;
   float4 s[8];
+  if (slot[0] >= 0) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) s[i] = slot < 0 ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(state + i * NEXT);
+    for (int i = 0; i < 8; i++) s[i] = *reinterpret_cast<const float4*>(state + i * NEXT);
+  }
 
   // the token's operands, one key channel a thread
   const long long hd = (long long)head * D + tid;
@@ -60,6 +63,11 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams
     qk += __shfl_xor_sync(0xffffffffu, qk, m);
   }
   if (lane == 0) { s_part[0][warp] = kk; s_part[1][warp] = qq; s_part[2][warp] = qk; }
+  drop_repeats(p.seq, row, slot);
+  if (slot[0] < 0) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   __syncthreads();
   qk = s_part[2][0] + s_part[2][1] + s_part[2][2] + s_part[2][3];
   if (RAW) {
@@ -136,7 +144,7 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams
       s[i].x = fmaf(fk, r[0], s[i].x); s[i].y = fmaf(fk, r[1], s[i].y); s[i].z = fmaf(fk, r[2], s[i].z); s[i].w = fmaf(fk, r[3], s[i].w);
     }
   }
-  if (slot < 0) return;
+  if (slot[0] < 0) return;
 #pragma unroll
   for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(state + i * NEXT) = s[i];
 }
@@ -144,10 +152,10 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams
 }  // namespace
 
 cudaError_t launch_kda_step(const StepParams& p, cudaStream_t stream) {
-  const long long blocks = p.seq.T * p.H * (D / STEP_ROWS);
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const long long blocks = p.seq.T * (D / STEP_ROWS);
+  if (blocks > 0x7fffffffLL || p.H > 65535) return cudaErrorInvalidValue;
   if (blocks == 0) return cudaSuccess;
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid((unsigned)blocks, (unsigned)p.H);
   if (p.raw) kda_step_kernel<true><<<grid, STEP_THREADS, 0, stream>>>(p);
   else kda_step_kernel<false><<<grid, STEP_THREADS, 0, stream>>>(p);
   return cudaGetLastError();
