@@ -462,7 +462,7 @@ bool whole_table(const void* p, int is64) { return (reinterpret_cast<uintptr_t>(
 
 int check_sequences(const KdaSequences& s, bool step) {
   if (s.N < 0 || s.T < 0 || s.n_slots < 0) return KDA_ERR_ARG;
-  if (s.T > 0x7fffffffLL) return KDA_ERR_LIMIT;
+  if (s.T > 0x7fffffffLL || s.n_slots > 0x7fffffffLL) return KDA_ERR_LIMIT;
   if (!whole_table(s.cu_seqlens, s.cu_is64) || !whole_table(s.slots, s.slots_is64) || !whole_table(s.status, 0)) return KDA_ERR_ARG;
   if (step) return s.N == s.T && (s.slots != nullptr || s.n_slots >= s.N) ? KDA_OK : KDA_ERR_ARG;
   if (s.N < 1 || (s.cu_seqlens == nullptr && s.N != 1)) return KDA_ERR_ARG;

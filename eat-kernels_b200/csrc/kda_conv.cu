@@ -153,17 +153,16 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const
   constexpr int HW = W - 1;
   using P = Pack<T, VEC>;
   const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
-  const long long row0 = (long long)(blockIdx.x / cblocks) * p.tile;
-  const int rows = (int)min((long long)p.tile, p.seq.T - row0);
+  const int row0 = blockIdx.x / cblocks * p.tile, rows = min(p.tile, (int)p.seq.T - row0);
   const int c = ((int)(blockIdx.x % cblocks) * CONV_THREADS + (int)threadIdx.x) * VEC;
-  long long slot[STEP_ROWS];
+  int slot[STEP_ROWS];
   row_slots(p.seq, row0, rows, slot);
   const bool mine = c < p.C;
   T* pool = reinterpret_cast<T*>(p.dst) + c;
   P hist[STEP_ROWS][HW], cur[STEP_ROWS];
 #pragma unroll
   for (int r = 0; r < STEP_ROWS; r++) {
-    if (mine && slot[r] != -2) cur[r] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + (row0 + r) * p.ldx + c);
+    if (mine && slot[r] != -2) cur[r] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + (long long)(row0 + r) * p.ldx + c);
 #pragma unroll
     for (int j = 0; j < HW; j++)
       if (mine && slot[r] >= 0) hist[r][j] = *reinterpret_cast<const P*>(pool + slot[r] * p.dst_stride + (long long)j * p.C);
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const
 #pragma unroll
   for (int r = 0; r < STEP_ROWS; r++) {
     if (r >= rows) break;
-    P* out = reinterpret_cast<P*>(reinterpret_cast<T*>(p.out) + (row0 + r) * p.ldo + c);
+    P* out = reinterpret_cast<P*>(reinterpret_cast<T*>(p.out) + (long long)(row0 + r) * p.ldo + c);
     float y[VEC], f[VEC];
     if (slot[r] == -2) {
 #pragma unroll

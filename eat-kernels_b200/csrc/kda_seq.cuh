@@ -78,35 +78,45 @@ __device__ __forceinline__ long long claim_slot(const SeqTable& s, int i) {
   return -1;
 }
 
-// The slots of R rows of a step from row0 on, `rows` of them there are, in two parts, so that a block can ask for the states before
-// it has looked for repeats.  First: a slot, -1 for an entry out of range, -2 for a row of padding (a negative entry) or none.
+// An entry of a slot table of a step: itself, -1 out of range, -2 padding.  Slots fit 31 bits.
+__device__ __forceinline__ int slot_entry(const SeqTable& s, int i) {
+  if (s.slots_is64) {
+    const long long d = reinterpret_cast<const long long*>(s.slots)[i];
+    return d < 0 ? -2 : (d < s.n_slots ? (int)d : -1);
+  }
+  const int d = reinterpret_cast<const int*>(s.slots)[i];
+  return d < 0 ? -2 : (d < (int)s.n_slots ? d : -1);
+}
+
+// The slots of R rows of a step from row0 on, `rows` of them there are (others: -2), in two parts, so that a block can ask for the
+// states before it has looked for repeats.  First the entries.
 template <int R>
-__device__ __forceinline__ void row_slots(const SeqTable& s, long long row0, int rows, long long (&slot)[R]) {
+__device__ __forceinline__ void row_slots(const SeqTable& s, int row0, int rows, int (&slot)[R]) {
 #pragma unroll
   for (int r = 0; r < R; r++) {
     slot[r] = -2;
-    if (r < rows) {
-      slot[r] = s.slots != nullptr ? table_at(s.slots, s.slots_is64, row0 + r) : row0 + r;
-      if (slot[r] < 0) slot[r] = -2;
-      else if (slot[r] >= s.n_slots) slot[r] = -1;
-    }
+    if (r < rows) slot[r] = s.slots != nullptr ? slot_entry(s, row0 + r) : row0 + r;
   }
 }
 
 // Then, called by the whole block: -1 for a slot that an earlier row has claimed too.
 template <int R>
-__device__ __forceinline__ void drop_repeats(const SeqTable& s, long long row0, long long (&slot)[R]) {
+__device__ __forceinline__ void drop_repeats(const SeqTable& s, int row0, int (&slot)[R]) {
   if (s.slots == nullptr) return;
   int bad = 0;
-  for (int j = threadIdx.x; j < (int)row0 + R - 1; j += blockDim.x) {
-    const long long d = j < s.N ? table_at(s.slots, s.slots_is64, j) : -1;
+  for (int j = threadIdx.x; j < row0; j += blockDim.x) {
+    const int d = slot_entry(s, j);
 #pragma unroll
     for (int r = 0; r < R; r++)
-      if (d >= 0 && d == slot[r] && j < row0 + r) bad |= 1 << r;
+      if (d >= 0 && d == slot[r]) bad |= 1 << r;
   }
 #pragma unroll
-  for (int r = 0; r < R; r++)
+  for (int r = 0; r < R; r++) {
     if (slot[r] == -1) bad |= 1 << r;
+#pragma unroll
+    for (int q = 0; q < r; q++)
+      if (slot[r] >= 0 && slot[r] == slot[q]) bad |= 1 << r;
+  }
   if (__syncthreads_or(bad) == 0) return;
 #pragma unroll
   for (int r = 0; r < R; r++)

@@ -573,12 +573,11 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
   static_assert(L >= ROWS, "a lane for each row");
   constexpr int CB = STEP_LANES / L;
   const int lane = threadIdx.x % L;
-  const long long row0 = (long long)blockIdx.y * ROWS;
-  const int rows = (int)min((long long)ROWS, p.seq.T - row0);
+  const int row0 = blockIdx.y * ROWS, rows = min(ROWS, (int)p.seq.T - row0);
   const int d = (int)blockIdx.x * CB + threadIdx.x / L;
   const bool mine = d < p.Dm;
   const int dc = mine ? d : p.Dm - 1, group = p.groups > 1 ? dc / (p.Dm / p.groups) : 0, n = lane * S;
-  long long slot[ROWS];
+  int slot[ROWS];
   row_slots(p.seq, row0, rows, slot);
   const long long at = (long long)dc * p.Ns + n;
   // S consecutive values of which `left` there are: one access where WIDE
@@ -596,13 +595,37 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
 #pragma unroll
   for (int r = 0; r < ROWS; r++)
     if (slot[r] >= 0) h[r] = values(p.src + slot[r] * p.src_stride + at);
+  Pack<T, S> rb[ROWS], rc[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; r++) {
+    const T* B = reinterpret_cast<const T*>(p.B) + (long long)(row0 + r) * p.ldb + (long long)group * p.Ns + n;
+    const T* C = reinterpret_cast<const T*>(p.C) + (long long)(row0 + r) * p.ldc + (long long)group * p.Ns + n;
+#pragma unroll
+    for (int k = 0; k < S; k++) rb[r].v[k] = rc[r].v[k] = from_float<T>(0.0f);
+    if (slot[r] == -2) continue;
+    if constexpr (WIDE) {
+      if (n < p.Ns) {
+        rb[r] = *reinterpret_cast<const Pack<T, S>*>(B);
+        rc[r] = *reinterpret_cast<const Pack<T, S>*>(C);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < S; k++)
+        if (n + k < p.Ns) {
+          rb[r].v[k] = B[k];
+          rc[r].v[k] = C[k];
+        }
+    }
+  }
   // lane r: row r
   const long long mine_row = row0 + min(lane, rows - 1);
   const float u = to_float(reinterpret_cast<const T*>(p.u)[mine_row * p.ldu + dc]);
   float s = to_float(reinterpret_cast<const T*>(p.dt)[mine_row * p.lddt + dc]) + (p.dt_bias != nullptr ? p.dt_bias[dc] : 0.0f);
   const float z = p.z != nullptr ? to_float(reinterpret_cast<const T*>(p.z)[mine_row * p.ldz + dc]) : 0.0f;
   const float skip = p.D != nullptr ? p.D[dc] : 0.0f;
-  const Values<S> a = values(p.A + at);
+  Values<S> a = values(p.A + at);
+#pragma unroll
+  for (int k = 0; k < S; k++) a.v[k] *= LOG2E_F;
   if (p.softplus) s = softplus(s);
   const float su = s * u;
   drop_repeats(p.seq, row0, slot);
@@ -613,28 +636,13 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
     part[r] = 0.0f;
     if (slot[r] == -2) continue;
     if (slot[r] == -1) h[r] = Values<S>();
-    const T* B = reinterpret_cast<const T*>(p.B) + (row0 + r) * p.ldb + (long long)group * p.Ns + n;
-    const T* C = reinterpret_cast<const T*>(p.C) + (row0 + r) * p.ldc + (long long)group * p.Ns + n;
     float b[S], c[S];
-    if constexpr (WIDE) {
-      if (n < p.Ns) {
-        unpack(*reinterpret_cast<const Pack<T, S>*>(B), b);
-        unpack(*reinterpret_cast<const Pack<T, S>*>(C), c);
-      } else {
-#pragma unroll
-        for (int k = 0; k < S; k++) b[k] = c[k] = 0.0f;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < S; k++) {
-        b[k] = n + k < p.Ns ? to_float(B[k]) : 0.0f;
-        c[k] = n + k < p.Ns ? to_float(C[k]) : 0.0f;
-      }
-    }
+    unpack(rb[r], b);
+    unpack(rc[r], c);
 #pragma unroll
     for (int k = 0; k < S; k++) {
       if (!WIDE && n + k >= p.Ns) continue;
-      h[r].v[k] = fmaf(exp2_fast(sr * a.v[k] * LOG2E_F), h[r].v[k], sur * b[k]);
+      h[r].v[k] = fmaf(exp2_fast(sr * a.v[k]), h[r].v[k], sur * b[k]);
       part[r] = fmaf(c[k], h[r].v[k], part[r]);
     }
     if (slot[r] >= 0 && mine) {
@@ -663,7 +671,7 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
     }
   }
   float y = __shfl_sync(0xffffffffu, part[0], min(lane, ROWS - 1) * (L / ROWS), L);
-  long long own = -2;
+  int own = -2;
 #pragma unroll
   for (int r = 0; r < ROWS; r++)
     if (lane == r) own = slot[r];

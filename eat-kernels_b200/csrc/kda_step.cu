@@ -24,9 +24,9 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams
   __shared__ __align__(16) float s_k[D], s_q[D], s_a[D];
   __shared__ float s_v[STEP_ROWS], s_part[3][STEP_THREADS / 32], s_sum[2][STEP_THREADS / 32][STEP_ROWS];
   const int part = blockIdx.x % (D / STEP_ROWS), head = blockIdx.y;
-  const long long row = blockIdx.x / (D / STEP_ROWS);
+  const int row = blockIdx.x / (D / STEP_ROWS);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  long long slot[1];
+  int slot[1];
   row_slots(p.seq, row, 1, slot);
   __nv_bfloat16* out = p.out + row * p.ldo + head * D + part * STEP_ROWS;
   if (slot[0] == -2) {
