@@ -65,7 +65,12 @@ class _Plan:
         self.words = C.c_uint64 * (C.sizeof(block) // 8)
         self.template = bytes(ready.args)
         self.given = [(_offset(block, f) // 8, i) for i, fields in ready.given.items() if tensors[i] is not None for f in fields]
-        self.fresh = [([_offset(block, f) // 8 for f in fields], t.shape, t.dtype) for t, fields in ready.fresh]
+        # a tensor made for each call: like one of the caller's where that is a dense one (the cheaper way to ask for it)
+        self.fresh = []
+        for t, fields in ready.fresh:
+            like = [i for i, g in enumerate(tensors) if g is not None and g.shape == t.shape and g.dtype == t.dtype and g.is_contiguous()
+                    and type(g) is torch.Tensor]
+            self.fresh.append(([_offset(block, f) // 8 for f in fields], t.shape, t.dtype, like[0] if like else -1))
         self.result, self.written, self.aligned = ready.result, [i for i in ready.written if tensors[i] is not None], ready.aligned
         self.present = [i for i, t in enumerate(tensors) if t is not None]
         spans = [_byte_interval(t) for t in tensors]
@@ -91,8 +96,8 @@ class _Plan:
         for word, i in self.given:
             args[word] = at[i]
         fresh = []
-        for words, shape, dtype in self.fresh:
-            t = torch.empty(shape, dtype=dtype, device=dev)
+        for words, shape, dtype, like in self.fresh:
+            t = torch.empty_like(tensors[like]) if like >= 0 else torch.empty(shape, dtype=dtype, device=dev)
             fresh.append(t)
             for word in words:
                 args[word] = t.data_ptr()
@@ -104,12 +109,20 @@ _plans = {}
 PLANS_MAX = 1024          # layouts remembered; a program that has more starts over
 
 
+def _stream(index):
+    """Handle of the device's current stream."""
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)       # the same without a Stream object (2 us a call)
+
+
 def _launch(entry, name, args, dev):
     if torch.cuda.current_device() == dev.index:
-        rc = entry(args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = entry(args, _stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = entry(args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = entry(args, _stream(dev.index))
     if rc:
         _cabi.check(rc, name)
 
