@@ -32,7 +32,7 @@ struct ScanParams {
   int Dm, Ns, groups, softplus, zero_pad;
   int piece;               // tokens of a piece, 0: sequences are not cut
   float *ws_state, *ws_sum;    // [pieces][Dm][Ns], [pieces][Dm]
-  int async_x, async_bc;   // set by the launcher: rows on 16 bytes
+  int async;               // set by the launcher: rows on 16 bytes
 };
 long long sscan_piece(long long T, int N, int Dm, int Ns);
 cudaError_t launch_sscan(const ScanParams& p, int type, cudaStream_t stream);

@@ -130,7 +130,6 @@ struct ScanShared {
   static constexpr int R = 2 * TILE + 4;
   float step[CB][R], input[CB][R];                   // s, s u
   float y[CB][R];                                    // sums of C h
-  float skip[CB][R], gate[CB][R];                    // D u, silu(z)
   float b[NP][R], c[NP][R];
 };
 
@@ -213,57 +212,67 @@ __device__ __forceinline__ void place(int i, int n, int& access, int& quad) {
   }
 }
 
-__device__ __forceinline__ void copy16(void* to, const void* from, bool on) {       // not `on`: zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(unsigned to, const void* from, int bytes) {     // 16 bytes, or (0) zeros and nothing read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
-// A tile's rows of WIDTH values, `valid` of them there are, on their way into shared memory with zeros around: whole 16 bytes at
-// a time where the rows start on them, else value by value.
-template <typename T, int WIDTH, int STRIDE>
+// A tile's rows of WIDTH values, on their way into shared memory with zeros around them, for K tensors of one shape.  ASYNC: whole
+// 16 bytes at a time, which needs rows that start on them; else value by value.
+template <typename T, int WIDTH, int STRIDE, int K, bool ASYNC>
 struct Bring {
-  static constexpr int PER = 16 / sizeof(T), CHUNKS = (WIDTH + PER - 1) / PER, N = (CHUNKS * TILE + HELPERS - 1) / HELPERS;
-  const T* from;           // the first access of this thread, one tile after the other
-  long long ld, tile;
-  int t, c;
-  bool inside;
-  __device__ __forceinline__ Bring(const void* base, long long ld_, long long row, long long col, int valid_, bool async, int tid) : ld(ld_), tile(TILE * ld_) {
-    t = async ? tid / CHUNKS : tid / WIDTH;
-    c = async ? tid % CHUNKS * PER : tid % WIDTH;
-    inside = c < valid_;
-    from = reinterpret_cast<const T*>(base) + (row + t) * ld + col + c;
+  static constexpr int PER = ASYNC ? 16 / sizeof(T) : 1, CHUNKS = (WIDTH + PER - 1) / PER, STEP = HELPERS / CHUNKS > 0 ? HELPERS / CHUNKS : 1;
+  static constexpr int N = (TILE + STEP - 1) / STEP;                     // accesses of a thread: rows t, t + STEP, ...
+  static_assert(HELPERS % CHUNKS == 0, "every thread in one column");
+  const T* from[K];        // the first access of this thread, one tile after the other
+  long long ld[K];
+  int t, c, left;          // row, column, rows from t on that there are
+  __device__ __forceinline__ Bring(const void* const (&base)[K], const long long (&ld_)[K], long long row, long long col, int valid, int tokens, int tid) {
+    t = tid / CHUNKS;
+    c = tid % CHUNKS * PER;
+    left = c < valid ? tokens - t : 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      ld[k] = ld_[k];
+      from[k] = reinterpret_cast<const T*>(base[k]) + (row + t) * ld[k] + col + c;
+    }
   }
-  __device__ __forceinline__ void operator()(T (*to)[STRIDE], int left, bool async) {
-    if (async) {
-      const T* q = from;
+  __device__ __forceinline__ void operator()(T (*to)[TILE][STRIDE], int used) {       // the first `used` of the tensors
+    const unsigned at = (unsigned)__cvta_generic_to_shared(&to[0][t][c]);
+    T v[K][N];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      if (k >= used) break;
+      const T* q = from[k];
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        constexpr int STEP = HELPERS / CHUNKS;
-        const int at = t + i * STEP;
-        const bool on = inside && at < left;
-        if (at < TILE && (HELPERS % CHUNKS == 0 || t < STEP)) copy16(&to[at][c], on ? q : from, on);
-        q += STEP * ld;
+        if (TILE % STEP != 0 && t + i * STEP >= TILE) break;             // more threads than rows
+        const bool on = i * STEP < left;
+        if constexpr (ASYNC) {
+          copy16(at + (unsigned)sizeof(T) * (k * TILE * STRIDE + i * STEP * STRIDE), q, on ? 16 : 0);
+        } else {
+          v[k][i] = from_float<T>(0.0f);
+          if (on) v[k][i] = *q;
+        }
+        q += STEP * ld[k];
       }
-    } else {
-      constexpr int M = (WIDTH * TILE + HELPERS - 1) / HELPERS, STEP = HELPERS / WIDTH > 0 ? HELPERS / WIDTH : 1;
-      T v[M];
-      const T* q = from;
-#pragma unroll
-      for (int i = 0; i < M; i++) {
-        v[i] = from_float<T>(0.0f);
-        if (inside && t + i * STEP < left) v[i] = *q;
-        q += STEP * ld;
-      }
-#pragma unroll
-      for (int i = 0; i < M; i++)
-        if (t + i * STEP < TILE) to[t + i * STEP][c] = v[i];
+      from[k] += TILE * ld[k];
     }
-    from += tile;
+    if constexpr (!ASYNC) {
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        if (k >= used) break;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+          if (t + i * STEP < TILE) to[k][t + i * STEP][c] = v[k][i];
+      }
+    }
+    left -= TILE;
   }
 };
 
 // The helpers' half: tokens in, outputs out.  Copies run DEPTH - 1 tiles ahead.  A thread then has two channels of four
 // consecutive tokens at a time.
-template <typename T, int L, int S, bool LOCAL>
+template <typename T, int L, int S, bool LOCAL, bool ASYNC>
 __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanShared<L, S>& sh, RawShared<T, L, S>& raw, int tid) {
   using Sh = ScanShared<L, S>;
   using Rw = RawShared<T, L, S>;
@@ -272,21 +281,15 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
   constexpr int CA = Sh::CB / 2;
   static_assert(CA * QUADS <= HELPERS, "one block of two channels and four tokens a helper");
   constexpr int NA = Sh::NP / 2, BBLOCKS = (LOCAL ? 1 : 2) * NA * QUADS, EB = (BBLOCKS + HELPERS - 1) / HELPERS;     // blocks of B, then of C
-  const bool has_z = !LOCAL && p.z != nullptr, async_x = p.async_x, async_bc = p.async_bc;
+  const bool has_z = !LOCAL && p.z != nullptr;
   const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
-  const long long bn = (long long)w.group * p.Ns;
-  Bring<T, Sh::CB, Rw::XS> bu(p.u, p.ldu, w.begin, w.d0, w.channels, async_x, tid), bd(p.dt, p.lddt, w.begin, w.d0, w.channels, async_x, tid),
-      bz(p.z, p.ldz, w.begin, w.d0, w.channels, async_x, tid);
-  Bring<T, Sh::NP, Rw::NS> bb(p.B, p.ldb, w.begin, bn, p.Ns, async_bc, tid), bc(p.C, p.ldc, w.begin, bn, p.Ns, async_bc, tid);
+  Bring<T, Sh::CB, Rw::XS, 3, ASYNC> bx({p.u, p.dt, p.z}, {p.ldu, p.lddt, p.ldz}, w.begin, w.d0, w.channels, w.tokens, tid);
+  Bring<T, Sh::NP, Rw::NS, 2, ASYNC> bbc({p.B, p.C}, {p.ldb, p.ldc}, w.begin, (long long)w.group * p.Ns, p.Ns, w.tokens, tid);
   auto bring_tile = [&](int i) {
     if (i < tiles) {
-      const int left = w.tokens - i * TILE;
       typename Rw::Slot& to = raw.slot[i % DEPTH];
-      bu(to.x[0], left, async_x);
-      bd(to.x[1], left, async_x);
-      if (has_z) bz(to.x[2], left, async_x);
-      bb(to.bc[0], left, async_bc);
-      if constexpr (!LOCAL) bc(to.bc[1], left, async_bc);
+      bx(to.x, has_z ? 3 : 2);
+      bbc(to.bc, LOCAL ? 1 : 2);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -304,32 +307,37 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
     skip[v] = p.D != nullptr ? p.D[d] : 0.0f;
     bias[v] = p.dt_bias != nullptr ? p.dt_bias[d] : 0.0f;
   }
-  float* const row = mine ? &sh.step[c][j] : &sh.step[0][0];               // step, input, y, skip, gate lie CB rows apart
+  float* const row = mine ? &sh.step[c][j] : &sh.step[0][0];               // step, input, y lie CB rows apart
   constexpr int ARRAY = Sh::CB * R;
-  auto store = [&](int i) {
-    const int left = w.tokens - i * TILE - j;
-    if (channels > 0 && left > 0) {
-      const float* y0 = row + (i & 1) * TILE + 2 * ARRAY;
-      float y[4][2];
+  P u[2][4], z[2][4];                                // kept for the outputs, two tiles later
+  int left = w.tokens - j;                           // tokens from this thread's on, of the tile that is filled
+  // outputs of the tile two in front
+  auto store = [&](const P (&uo)[4], const P (&zo)[4], int stage) {
+    const int have = left + 2 * TILE;
+    if (channels > 0 && have > 0) {
+      const float4 f0 = *reinterpret_cast<const float4*>(row + stage * TILE + 2 * ARRAY);
+      const float4 f1 = *reinterpret_cast<const float4*>(row + stage * TILE + 2 * ARRAY + R);
+      float y[4][2] = {{f0.x, f1.x}, {f0.y, f1.y}, {f0.z, f1.z}, {f0.w, f1.w}};
 #pragma unroll
-      for (int v = 0; v < 2; v++) {
-        float4 f = *reinterpret_cast<const float4*>(y0 + v * R);
-        const float4 d = *reinterpret_cast<const float4*>(y0 + v * R + ARRAY);
-        f.x += d.x; f.y += d.y; f.z += d.z; f.w += d.w;
+      for (int k = 0; k < 4; k++) {
+        float uf[2], zf[2];
+        unpack(uo[k], uf);
+        y[k][0] = fmaf(skip[0], uf[0], y[k][0]);
+        y[k][1] = fmaf(skip[1], uf[1], y[k][1]);
         if (has_z) {
-          const float4 g = *reinterpret_cast<const float4*>(y0 + v * R + 2 * ARRAY);
-          f.x *= g.x; f.y *= g.y; f.z *= g.z; f.w *= g.w;
+          unpack(zo[k], zf);
+          y[k][0] *= silu<T>(zf[0]);
+          y[k][1] *= silu<T>(zf[1]);
         }
-        y[0][v] = f.x; y[1][v] = f.y; y[2][v] = f.z; y[3][v] = f.w;
       }
       T* to = out;
-      if (async_x && left >= 4) {
+      if (ASYNC && have >= 4) {
 #pragma unroll
         for (int k = 0; k < 4; k++, to += p.ldo) *reinterpret_cast<P*>(to) = pack<T, 2>(y[k]);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++, to += p.ldo)
-          if (k < left) {
+          if (k < have) {
             to[0] = from_float<T>(y[k][0]);
             if (channels > 1) to[1] = from_float<T>(y[k][1]);
           }
@@ -337,33 +345,32 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
     }
     out += TILE * p.ldo;
   };
-  for (int i = 0; i < DEPTH - 1; i++) bring_tile(i);
-  for (int i = 0; i < tiles; i++) {
-    const int stage = i & 1;
+  auto tile = [&](int i, P (&ui)[4], P (&zi)[4], int stage) {
     const typename Rw::Slot& slot = raw.slot[i % DEPTH];
     asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 2) : "memory");
     asm volatile("bar.sync %0, %1;" ::"n"((int)BAR_HELPERS), "n"(HELPERS) : "memory");         // tile i is here, tile i - 1 has been read
     bring_tile(i + DEPTH - 1);
     if (i >= 2) {
       bar_sync(BAR_DONE + stage);
-      if constexpr (!LOCAL) store(i - 2);
+      if constexpr (!LOCAL) store(ui, zi, stage);
     }
     if (mine) {
-      const int left = w.tokens - i * TILE - j;
       const T* x = &slot.x[0][j][c];
       constexpr int X = TILE * Rw::XS;
-      float uf[4][2], df[4][2], zf[4][2];
+      float uf[4][2], df[4][2];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        unpack(*reinterpret_cast<const P*>(x + k * Rw::XS), uf[k]);
+        ui[k] = *reinterpret_cast<const P*>(x + k * Rw::XS);
+        unpack(ui[k], uf[k]);
         unpack(*reinterpret_cast<const P*>(x + k * Rw::XS + X), df[k]);
-        if (has_z) unpack(*reinterpret_cast<const P*>(x + k * Rw::XS + 2 * X), zf[k]);
+        if (has_z) zi[k] = *reinterpret_cast<const P*>(x + k * Rw::XS + 2 * X);
       }
 #pragma unroll
       for (int v = 0; v < 2; v++) {
+        F2 s01 = f2(df[0][v] + bias[v], df[1][v] + bias[v]), s23 = f2(df[2][v] + bias[v], df[3][v] + bias[v]);
         float s[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) s[k] = df[k][v] + bias[v];
+        split(s01, s[0], s[1]);
+        split(s23, s[2], s[3]);
         if (p.softplus) {
           split(softplus2(s[0], s[1]), s[0], s[1]);
           split(softplus2(s[2], s[3]), s[2], s[3]);
@@ -372,19 +379,20 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 #pragma unroll
           for (int k = 0; k < 4; k++)
             if (k >= left) s[k] = 0.0f;              // leaves the state as it is
+        s01 = f2(s[0], s[1]);
+        s23 = f2(s[2], s[3]);
         float* to = row + stage * TILE + v * R;
-        *reinterpret_cast<float4*>(to) = make_float4(s[0], s[1], s[2], s[3]);
-        *reinterpret_cast<float4*>(to + ARRAY) = make_float4(s[0] * uf[0][v], s[1] * uf[1][v], s[2] * uf[2][v], s[3] * uf[3][v]);
-        if constexpr (!LOCAL) *reinterpret_cast<float4*>(to + 3 * ARRAY) = make_float4(skip[v] * uf[0][v], skip[v] * uf[1][v], skip[v] * uf[2][v], skip[v] * uf[3][v]);
-        if (has_z) *reinterpret_cast<float4*>(to + 4 * ARRAY) = make_float4(silu<T>(zf[0][v]), silu<T>(zf[1][v]), silu<T>(zf[2][v]), silu<T>(zf[3][v]));
+        *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(s01, s23);
+        *reinterpret_cast<ulonglong2*>(to + ARRAY) = make_ulonglong2(mul2(s01, f2(uf[0][v], uf[1][v])), mul2(s23, f2(uf[2][v], uf[3][v])));
       }
     }
+    left -= TILE;
 #pragma unroll
     for (int e = 0; e < EB; e++) {
       int n, q;
       const int id = tid + e * HELPERS, second = id >= NA * QUADS;
       place(id % (NA * QUADS), NA, n, q);
-      if (id >= BBLOCKS) continue;
+      if (BBLOCKS % HELPERS != 0 && id >= BBLOCKS) continue;
       float f[4][2];
 #pragma unroll
       for (int k = 0; k < 4; k++) unpack(*reinterpret_cast<const P*>(&slot.bc[second][4 * q + k][2 * n]), f[k]);
@@ -393,10 +401,25 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
       *reinterpret_cast<float4*>(to + R) = make_float4(f[0][1], f[1][1], f[2][1], f[3][1]);
     }
     bar_arrive(BAR_FULL + stage);
+  };
+  for (int i = 0; i < DEPTH - 1; i++) bring_tile(i);
+  for (int i = 0; i < tiles; i += 2) {
+    tile(i, u[0], z[0], 0);
+    if (i + 1 < tiles) tile(i + 1, u[1], z[1], 1);
   }
-  for (int i = tiles > 2 ? tiles - 2 : 0; i < tiles; i++) {
-    bar_sync(BAR_DONE + (i & 1));
-    if constexpr (!LOCAL) store(i);
+  // the last two tiles' outputs, in order; `left` counts as if the tiles behind them were filled
+  if (tiles > 1) {
+    const int stage = tiles & 1;
+    bar_sync(BAR_DONE + stage);
+    if constexpr (!LOCAL) stage ? store(u[1], z[1], 1) : store(u[0], z[0], 0);
+    left -= TILE;
+  } else {
+    left -= TILE;
+  }
+  if (tiles > 0) {
+    const int stage = (tiles - 1) & 1;
+    bar_sync(BAR_DONE + stage);
+    if constexpr (!LOCAL) stage ? store(u[1], z[1], 1) : store(u[0], z[0], 0);
   }
 }
 
@@ -471,7 +494,7 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
 }
 
 // A sequence, or a piece of one, and up to CB channels of one group a block.
-template <typename T, int L, int S, bool LOCAL>
+template <typename T, int L, int S, bool LOCAL, bool ASYNC>
 __global__ void __launch_bounds__(SCAN_THREADS, 2) kda_selective_scan_kernel(const ScanParams p) {
   using Sh = ScanShared<L, S>;
   constexpr int CB = Sh::CB;
@@ -500,7 +523,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) kda_selective_scan_kernel(con
   if (w.piece + 1 < w.pieces) end = w.begin + p.piece;
   w.tokens = __reduce_max_sync(0xffffffffu, (int)(end - w.begin));       // the same in all lanes, and known to be: no divergence in the loops
   if (helper) {
-    help<T, L, S, LOCAL>(p, w, sh, raw, tid);
+    help<T, L, S, LOCAL, ASYNC>(p, w, sh, raw, tid);
     // rows behind the last sequence
     if (!LOCAL && w.seq == p.seq.N - 1 && w.piece + 1 == w.pieces && (rejected || p.zero_pad) && tid % CB < w.channels)
       for (long long t = end + tid / CB; t < p.seq.T; t += HELPERS / CB) reinterpret_cast<T*>(p.out)[t * p.ldo + w.d0 + tid % CB] = from_float<T>(0.0f);
@@ -686,15 +709,20 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
   *out = from_float<T>(y);
 }
 
-template <typename T, int L, int S, bool LOCAL>
-cudaError_t launch_pass(const ScanParams& p, long long pieces, cudaStream_t stream) {
+template <typename T, int L, int S, bool LOCAL, bool ASYNC>
+cudaError_t launch_copies(const ScanParams& p, long long pieces, cudaStream_t stream) {
   constexpr int bytes = sizeof(ScanShared<L, S>) + sizeof(RawShared<T, L, S>), CB = ScanShared<L, S>::CB;
   const long long blocks = (long long)((p.Dm / p.groups + CB - 1) / CB) * p.groups * pieces;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(kda_selective_scan_kernel<T, L, S, LOCAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const cudaError_t e = cudaFuncSetAttribute(kda_selective_scan_kernel<T, L, S, LOCAL, ASYNC>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  kda_selective_scan_kernel<T, L, S, LOCAL><<<(unsigned)blocks, SCAN_THREADS, bytes, stream>>>(p);
+  kda_selective_scan_kernel<T, L, S, LOCAL, ASYNC><<<(unsigned)blocks, SCAN_THREADS, bytes, stream>>>(p);
   return cudaGetLastError();
+}
+
+template <typename T, int L, int S, bool LOCAL>
+cudaError_t launch_pass(const ScanParams& p, long long pieces, cudaStream_t stream) {
+  return p.async ? launch_copies<T, L, S, LOCAL, true>(p, pieces, stream) : launch_copies<T, L, S, LOCAL, false>(p, pieces, stream);
 }
 
 template <typename T, int L, int S>
@@ -719,8 +747,8 @@ bool rows16(const void* p, long long ld, long long width) {
 template <typename T>
 cudaError_t launch_type(ScanParams p, cudaStream_t stream) {
   const long long per = p.Dm / p.groups;
-  p.async_x = rows16<T>(p.u, p.ldu, per) && rows16<T>(p.dt, p.lddt, per) && rows16<T>(p.z, p.ldz, per) && rows16<T>(p.out, p.ldo, per);
-  p.async_bc = rows16<T>(p.B, p.ldb, p.Ns) && rows16<T>(p.C, p.ldc, p.Ns);
+  p.async = rows16<T>(p.u, p.ldu, per) && rows16<T>(p.dt, p.lddt, per) && rows16<T>(p.z, p.ldz, per) && rows16<T>(p.out, p.ldo, per) &&
+            rows16<T>(p.B, p.ldb, p.Ns) && rows16<T>(p.C, p.ldc, p.Ns);
   if (p.Ns <= 4) return launch_lanes<T, 4, 1>(p, stream);
   if (p.Ns <= 8) return launch_lanes<T, 4, 2>(p, stream);
   if (p.Ns <= 16) return launch_lanes<T, 4, 4>(p, stream);
