@@ -4,6 +4,8 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -11,8 +13,7 @@ CSRC = PKG.parent / "csrc"
 LIB = PKG / "libkda_b200.so"
 SOURCES = ["kda_chunk_umma.cu", "kda_chunk_fwd.cu", "kda_plan.cu", "kda_cp.cu", "kda_conv.cu", "kda_sscan.cu", "kda_step.cu",
            "kda_pool.cu", "kda_capi.cu"]
-NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-              "-shared"]
+NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
 def nvcc_path() -> str:
@@ -33,13 +34,19 @@ def stale() -> bool:
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and not stale():
         return LIB
-    cmd = [nvcc_path(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", str(LIB),
-           *[str(CSRC / s) for s in SOURCES]]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    if verbose:
-        print(res.stderr)
+    def nvcc(*args):
+        res = subprocess.run([nvcc_path(), *NVCC_FLAGS, *args], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            print(res.stderr)
+
+    with tempfile.TemporaryDirectory() as tmp:         # the sources side by side: the instantiations of one take over a minute
+        objects = [str(Path(tmp) / (src + ".o")) for src in SOURCES]
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            list(pool.map(lambda job: nvcc(*(["-Xptxas", "-v"] if verbose else []), "-c", "-o", job[1], str(CSRC / job[0])),
+                          zip(SOURCES, objects)))
+        nvcc("-shared", "-o", str(LIB), *objects)
     return LIB
 
 
