@@ -93,7 +93,7 @@ struct RawShared {
   static constexpr int DEPTH = sizeof(T) == 4 ? 3 : 4;                   // what lets two blocks share an SM
 
   // rows of whole 16 bytes; 16-bit rows four apart fall into different halves of the banks
-  static constexpr int XS = SCAN_LANES / L + 8, NS = L * S + 8;
+  static constexpr int XS = SCAN_LANES / L + 8, NS = L * S < 8 ? 16 : L * S + 8;
   struct Slot {
     T x[3][TILE][XS];                                // u, dt, z
     T bc[2][TILE][NS];

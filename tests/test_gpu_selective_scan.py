@@ -76,6 +76,49 @@ def test_long_axes_on_few_channels(Dm, T, dtype, slow):
     check(a, init[:1], [T], y, final)
 
 
+@pytest.mark.parametrize("Dm,Ns,G,lens,dtype", [(40, 24, 2, [900, 0, 1, 350, 127, 129], BF), (36, 16, 4, [513], F), (64, 100, 1, [600, 5], HF),
+                                                (130, 3, 1, [640, 128], BF), (24, 33, 3, [256, 256, 256], F), (256, 8, 1, [1000, 200], HF)])
+def test_pieces_over_a_pool(Dm, Ns, G, lens, dtype):
+    """Long axes on few channels are cut into pieces: the slots in place, groups, odd state sizes, empty sequences, a repeated slot, rows
+    behind the last sequence."""
+    import kda_b200
+    gen, N, rest = generator(Ns), len(lens), 40
+    a = make(gen, sum(lens) + rest, Dm, Ns, G, dtype)
+    for n in ("u", "dt", "B", "C", "z"):
+        a[n][:, sum(lens):] = float("nan")
+    pool = randn(gen, N + 2, Dm, Ns)
+    slots = torch.randperm(N + 2, generator=torch.Generator().manual_seed(3))[:N].to(DEV)
+    before, status = pool.clone(), torch.zeros(1, dtype=torch.int32, device=DEV)
+    y, _ = kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu_of(lens), ssm_state_indices=slots, status=status)
+    assert int(status) == 0 and bool((y[:, sum(lens):] == 0).all())
+    check(a, before[slots], lens, y, pool[slots])
+    free = [i for i in range(N + 2) if i not in slots.tolist()]
+    assert torch.equal(pool[free], before[free])
+    if N > 1:                                                         # the last sequence names the first one's slot
+        slots[-1] = slots[0]
+        again = before.clone()
+        y2, _ = kda_b200.selective_scan(**a, initial_state=again, cu_seqlens=cu_of(lens), ssm_state_indices=slots, status=status)
+        init = before[slots].clone()
+        init[-1] = 0
+        assert int(status) == 2
+        want = [again[slots[i]] for i in range(N - 1)] + [kda_b200.selective_scan(**at(a, slice(sum(lens) - lens[-1], sum(lens))))[1][0]]
+        check(a, init, lens, y2, torch.stack(want))
+    status.zero_()
+    bad, keep = torch.tensor([0, *[5] * (N - 1), sum(lens) + rest + 1], device=DEV), before.clone()
+    y, _ = kda_b200.selective_scan(**a, initial_state=keep, cu_seqlens=bad, ssm_state_indices=torch.arange(N, device=DEV), status=status)
+    assert int(status) == 1 and bool((y == 0).all()) and torch.equal(keep, before)
+
+
+@pytest.mark.parametrize("N", [129, 300])
+def test_many_sequences(N):
+    import kda_b200
+    gen = generator(N)
+    lens = [(7 * i) % 23 for i in range(N)]
+    a, init = make(gen, sum(lens), 96, 16, 1, BF), randn(gen, N, 96, 16)
+    y, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of(lens))
+    check(a, init, lens, y, final)
+
+
 @pytest.mark.parametrize("leave", ["D", "z", "dt_bias", "all"])
 def test_what_may_be_left_out(leave):
     import kda_b200
