@@ -499,7 +499,7 @@ int conv_launch(const KdaConvArgs* a, bool step, void* stream) {
 
 int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
   if (a == nullptr || a->Dm < 1 || a->Ns < 1 || a->groups < 1 || a->Dm % a->groups || !known_type(a->type)) return KDA_ERR_ARG;
-  if (a->Ns > KDA_SCAN_MAX_STATE) return KDA_ERR_LIMIT;
+  if (a->Ns > KDA_SCAN_MAX_STATE || (step && a->seq.T > KDA_SCAN_MAX_ROWS)) return KDA_ERR_LIMIT;
   const int rc = check_sequences(a->seq, step);
   if (rc != KDA_OK) return rc;
   if (!a->A) return KDA_ERR_ARG;
@@ -577,6 +577,7 @@ int kda_selective_scan_step_launch(const KdaScanArgs* a, void* stream) { return 
 
 int kda_step_launch(const KdaStepArgs* a, void* stream) {
   if (a == nullptr || a->H < 1) return KDA_ERR_ARG;
+  if (a->H > 65535) return KDA_ERR_LIMIT;
   if (a->frontend != KDA_FRONTEND_RAW && a->frontend != KDA_FRONTEND_PLAIN) return KDA_ERR_ARG;
   const int rc = check_sequences(a->seq, true);
   if (rc != KDA_OK) return rc;

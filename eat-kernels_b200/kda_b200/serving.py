@@ -33,8 +33,9 @@ class _Ready:
     """A checked call: the argument block, where the pointers of the caller's tensors and of the ones made for this call go in it,
     and what it returns."""
 
-    def __init__(self, name, dev, args, given, fresh, result, written=(), aligned=()):
+    def __init__(self, name, dev, args, given, fresh, result, written=(), aligned=(), keep=()):
         self.name, self.dev, self.args = name, dev, args
+        self.keep = keep              # what the block points to, copies of the caller's tensors among it, until the launch
         self.given = given            # {index among the caller's tensors: names of pointer fields}
         self.fresh = fresh            # [(tensor made for this call, names of pointer fields)]
         self.result = result          # indices among the caller's tensors, or -1 - index in `fresh`
@@ -276,7 +277,7 @@ def _step_pool(dev, pool, inner, dtype, what="the pool"):
 
 def _slots(dev, slots, N):
     _cuda(dev, ssm_state_indices=slots)
-    return _table(slots, "ssm_state_indices", N, True)
+    return _table(slots, "ssm_state_indices", N, False)
 
 
 def _step_slots(dev, slots, N, pool):
@@ -327,7 +328,7 @@ def _conv(x, weight, bias, state, cu_seqlens, slots, out, status, activation, st
     fresh = ([(y, ["out"])] if out is None else []) + ([] if in_place else [(dst, ["dst"])])
     result = (6 if out is not None else -1, 3 if in_place else -len(fresh))
     name = None if step and not T else "kda_short_conv_step_launch" if step else "kda_short_conv_launch"
-    return _Ready(name, dev, args, given, fresh, result, [6] + [3] * in_place)
+    return _Ready(name, dev, args, given, fresh, result, [6] + [3] * in_place, keep=(x, weight, bias, src, cu, slots))
 
 
 def short_conv(x, weight, bias=None, initial_state=None, cu_seqlens=None, *, activation="silu", ssm_state_indices=None, out=None,
@@ -402,7 +403,7 @@ def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, slots, out, stat
     if ws is not None:
         fresh.append((ws, ["workspace"]))
     name = None if step and not T else "kda_selective_scan_step_launch" if step else "kda_selective_scan_launch"
-    return _Ready(name, dev, args, given, fresh, result, [11] + [8] * in_place)
+    return _Ready(name, dev, args, given, fresh, result, [11] + [8] * in_place, keep=(u, dt, A, B, C_, skip, z, dt_bias, src, cu, slots))
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=None, cu_seqlens=None, *, dt_softplus=True,
@@ -454,7 +455,8 @@ def _kda(q, k, v, g, beta, A_log, dt_bias, pool, slots, out, status, scale, raw)
                              float(scale), LOWER_BOUND, _cabi.FRONTEND_RAW if raw else _cabi.FRONTEND_PLAIN, H)
     given = {i: [f] for i, f in enumerate(("q", "k", "v", "g", "beta", "A_log", "dt_bias", "pool", "seq.slots", "out", "seq.status"))}
     fresh = [(y, ["out"])] if out is None else []
-    return _Ready("kda_step_launch" if N else None, dev, args, given, fresh, (9 if out is not None else -1, 7), [9, 7], [7])
+    return _Ready("kda_step_launch" if N else None, dev, args, given, fresh, (9 if out is not None else -1, 7), [9, 7], [7],
+                  keep=(q, k, v, g, beta, A_log, dt_bias, slots))
 
 
 def kda_step(q, k, v, g, beta, A_log, dt_bias, scale, pool, ssm_state_indices=None, *, out=None, status=None):

@@ -295,6 +295,7 @@ typedef struct KdaScanArgs {
   size_t workspace_bytes;
 } KdaScanArgs;
 #define KDA_SCAN_MAX_STATE 128
+#define KDA_SCAN_MAX_ROWS 262140      /* rows of a step */
 size_t kda_selective_scan_workspace_bytes(int64_t T, int32_t N, int32_t Dm, int32_t Ns);
 int kda_selective_scan_launch(const KdaScanArgs* args, void* stream);
 int kda_selective_scan_step_launch(const KdaScanArgs* args, void* stream);
@@ -312,7 +313,7 @@ typedef struct KdaStepArgs {
   int64_t ldq, ldk, ldv, ldg, ldbeta, ldo, slot_stride;
   KdaSequences seq;
   float scale, lower_bound;
-  int32_t frontend, H;
+  int32_t frontend, H;     /* H <= 65535 */
 } KdaStepArgs;
 int kda_step_launch(const KdaStepArgs* args, void* stream);
 

@@ -1,6 +1,9 @@
 """Calls with a layout that was checked before: other tensors, other addresses, other options, tensors that overlap or lie off 16 bytes,
 threads, inference mode, more layouts than are remembered."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -110,3 +113,42 @@ def test_more_layouts_than_are_remembered(monkeypatch):
         want = torch.nn.functional.silu(sum(padded[j:j + n] * w[:, j] for j in range(4)))
         torch.testing.assert_close(y[0], want, rtol=1e-4, atol=1e-5)
         assert len(serving._plans) <= 5
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, "eat-kernels_b200")
+import torch, kda_b200
+dev = "cuda:0"
+x, w, h = torch.ones(1, 3000, 64, device=dev), torch.ones(64, 4, device=dev), torch.zeros(4, 3, 64, device=dev)
+A, B, s = -torch.ones(64, 16, device=dev), torch.ones(1, 3000, 1, 16, device=dev), torch.zeros(4, 64, 16, device=dev)
+q, g, b = torch.ones(1, 4, 2, 128, device=dev, dtype=torch.bfloat16), torch.zeros(1, 4, 2, 128, device=dev), torch.ones(1, 4, 2, device=dev)
+S, used, none = torch.zeros(4, 2, 128, 128, device=dev), torch.zeros(4, dtype=torch.bool, device=dev), torch.tensor([-1, -1], device=dev)
+def calls():
+    slots = kda_b200.pool_fork([h, s, S], used, none)
+    y, _ = kda_b200.short_conv(x, w)
+    z, _ = kda_b200.selective_scan(y, x, A, B, B)
+    kda_b200.short_conv_step(x[:, :4], w, None, h)
+    kda_b200.selective_scan_step(x[:, :4], x[:, :4], A, B[:, :4], B[:, :4], None, None, None, s)
+    o, _ = kda_b200.kda_step_plain(q, q, q, g, b, 1.0, S)
+    kda_b200.pool_free(used, slots[:1])
+    return z, o, kda_b200.pool_compact([h, s, S], used)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = calls()
+graph.replay()
+torch.cuda.synchronize()
+first = [t.clone() for t in out] + [t.clone() for t in (h, s, S, used)]
+for t in (h, s, S, used):
+    t.zero_()
+eager = list(calls()) + [h, s, S, used]
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(first, eager))
+print("equal")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured():
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-2000:]

@@ -125,6 +125,25 @@ def test_bad_sequences_and_limits(lib):
     a = _scan()
     a.Ns = 129
     assert lib.kda_selective_scan_launch(a, None) == -4
+    a = _scan()
+    a.seq = _seq(262141, 262141)
+    assert lib.kda_selective_scan_step_launch(a, None) == -4
+    a = _step()
+    a.H = 65536
+    assert lib.kda_step_launch(a, None) == -4
+    for make, name in ((_conv, "kda_short_conv_step_launch"), (_scan, "kda_selective_scan_step_launch"), (_step, "kda_step_launch")):
+        a = make()
+        a.seq = _seq(2, 2, n_slots=1 << 31)
+        assert getattr(lib, name)(a, None) == -4
+    a = _scan()                                                      # a long axis on few channels needs a workspace
+    a.seq = _seq(1, 4096)
+    need = lib.kda_selective_scan_workspace_bytes(4096, 1, 64, 16)
+    assert need > 0 and lib.kda_selective_scan_launch(a, None) == -1
+    a.workspace, a.workspace_bytes = AT, need - 1
+    assert lib.kda_selective_scan_launch(a, None) == -2
+    a.workspace, a.workspace_bytes = AT + 8, need
+    assert lib.kda_selective_scan_launch(a, None) == -1
+    assert lib.kda_selective_scan_workspace_bytes(100, 1, 64, 16) == lib.kda_selective_scan_workspace_bytes(4096, 0, 64, 16) == 0
     a = _pool()
     a.workspace_bytes = lib.kda_pool_workspace_bytes(2, 8) - 1
     assert lib.kda_pool_copy_launch(a, None) == -2
