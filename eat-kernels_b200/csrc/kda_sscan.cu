@@ -18,7 +18,8 @@ namespace kda {
 
 namespace {
 
-constexpr int SCAN_LANES = 256;          // scan threads of a block
+constexpr int SCAN_LANES = 128;          // scan threads of a block
+constexpr int CH = 2;                    // channels of a lane
 constexpr int HELPERS = 128;
 constexpr int SCAN_THREADS = SCAN_LANES + HELPERS;
 constexpr int STEP_LANES = 128;          // threads of a single token's block
@@ -93,7 +94,7 @@ struct RawShared {
   static constexpr int DEPTH = sizeof(T) == 4 ? 3 : 4;                   // what lets two blocks share an SM
 
   // rows of whole 16 bytes; 16-bit rows four apart fall into different halves of the banks
-  static constexpr int XS = SCAN_LANES / L + 8, NS = L * S < 8 ? 16 : L * S + 8;
+  static constexpr int XS = CH * SCAN_LANES / L + 8, NS = L * S < 8 ? 16 : L * S + 8;
   struct Slot {
     T x[3][TILE][XS];                                // u, dt, z
     T bc[2][TILE][NS];
@@ -123,7 +124,7 @@ __device__ __forceinline__ void store_values(float* p, const Values<S>& v) {
 
 template <int L, int S>
 struct ScanShared {
-  static constexpr int CB = SCAN_LANES / L;          // channels of a block
+  static constexpr int CB = CH * SCAN_LANES / L;     // channels of a block; a lane has c and c + CB / CH
   static_assert(CB >= 8 && L * S <= 128, "layouts");
   static constexpr int NP = L * S;                   // state values, padded
   // a row of time, both stages: eight rows' 16 bytes at one time fall into different banks
@@ -427,67 +428,76 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 // four; tokens behind the last one leave the state as it is.
 // LOCAL: the state alone, and the sum of the steps.
 template <int L, int S, bool LOCAL>
-__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[S], float (&h)[S], float& sum) {
-  constexpr int R = ScanShared<L, S>::R;
-  constexpr int SUMS = 8;                            // tokens that are summed over the lanes at a time: exchanges that do not wait for each other
+__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[CH][S], float (&h)[CH][S], float (&sum)[CH]) {
+  constexpr int R = ScanShared<L, S>::R, NEXT = ScanShared<L, S>::CB / CH * R;
+  constexpr int SUMS = 4;                            // tokens that are summed over the lanes at a time
   const int lane = tid % L, c = tid / L;
   const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
-  F2 aa[S];
-#pragma unroll
-  for (int k = 0; k < S; k++) aa[k] = f2(a[k], a[k]);
   for (int i = 0; i < tiles; i++) {
     const int stage = i & 1;
     bar_sync(BAR_FULL + stage);
     const float *step = &sh.step[c][stage * TILE], *input = &sh.input[c][stage * TILE];
     const float *b = &sh.b[lane][stage * TILE], *cc = &sh.c[lane][stage * TILE];
-    float part[SUMS];
+    float* out = &sh.y[c][stage * TILE + lane * SUMS / L];
 #pragma unroll
     for (int j = 0; j < TILE; j += 4) {
-      const ulonglong2 st = *reinterpret_cast<const ulonglong2*>(step + j), in = *reinterpret_cast<const ulonglong2*>(input + j);
-      F2 y01, y23;
+      ulonglong2 st[CH], in[CH];
+      F2 y01[CH], y23[CH];
+#pragma unroll
+      for (int m = 0; m < CH; m++) {
+        st[m] = *reinterpret_cast<const ulonglong2*>(step + m * NEXT + j);
+        in[m] = *reinterpret_cast<const ulonglong2*>(input + m * NEXT + j);
+      }
 #pragma unroll
       for (int k = 0; k < S; k++) {
         const ulonglong2 bk = *reinterpret_cast<const ulonglong2*>(b + k * L * R + j);
-        float x0, x1, x2, x3, i0, i1, i2, i3;
-        split(mul2(st.x, aa[k]), x0, x1);
-        split(mul2(st.y, aa[k]), x2, x3);
-        split(mul2(in.x, bk.x), i0, i1);
-        split(mul2(in.y, bk.y), i2, i3);
-        const float h0 = fmaf(exp2_fast(x0), h[k], i0), h1 = fmaf(exp2_fast(x1), h0, i1), h2 = fmaf(exp2_fast(x2), h1, i2);
-        h[k] = fmaf(exp2_fast(x3), h2, i3);
-        if constexpr (LOCAL) continue;
-        const ulonglong2 ck = *reinterpret_cast<const ulonglong2*>(cc + k * L * R + j);
-        y01 = k == 0 ? mul2(ck.x, f2(h0, h1)) : fma2(ck.x, f2(h0, h1), y01);
-        y23 = k == 0 ? mul2(ck.y, f2(h2, h[k])) : fma2(ck.y, f2(h2, h[k]), y23);
-      }
-      if constexpr (LOCAL) {
-        float s0, s1, s2, s3;
-        split(st.x, s0, s1);
-        split(st.y, s2, s3);
-        sum += (s0 + s1) + (s2 + s3);
-        continue;
-      }
-      split(y01, part[j % SUMS], part[j % SUMS + 1]);
-      split(y23, part[j % SUMS + 2], part[j % SUMS + 3]);
-      if ((j + 4) % SUMS != 0) continue;
-      // a step of the exchange leaves half of the tokens with each lane: lane l ends with the sums of tokens l SUMS / L and on
-      // (L > SUMS: neighbours with the same one)
+        ulonglong2 ck = {0, 0};
+        if constexpr (!LOCAL) ck = *reinterpret_cast<const ulonglong2*>(cc + k * L * R + j);
 #pragma unroll
-      for (int m = L / 2, n = SUMS / 2; m >= 1; m /= 2, n /= 2) {
-        if (n >= 1) {
-#pragma unroll
-          for (int k = 0; k < n; k++) {
-            const bool up = lane & m;
-            const float give = up ? part[k] : part[n + k], keep = up ? part[n + k] : part[k];
-            part[k] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+        for (int m = 0; m < CH; m++) {
+          const F2 ak = f2(a[m][k], a[m][k]);
+          float x0, x1, x2, x3, i0, i1, i2, i3;
+          split(mul2(st[m].x, ak), x0, x1);
+          split(mul2(st[m].y, ak), x2, x3);
+          split(mul2(in[m].x, bk.x), i0, i1);
+          split(mul2(in[m].y, bk.y), i2, i3);
+          const float h0 = fmaf(exp2_fast(x0), h[m][k], i0), h1 = fmaf(exp2_fast(x1), h0, i1), h2 = fmaf(exp2_fast(x2), h1, i2);
+          h[m][k] = fmaf(exp2_fast(x3), h2, i3);
+          if constexpr (!LOCAL) {
+            y01[m] = k == 0 ? mul2(ck.x, f2(h0, h1)) : fma2(ck.x, f2(h0, h1), y01[m]);
+            y23[m] = k == 0 ? mul2(ck.y, f2(h2, h[m][k])) : fma2(ck.y, f2(h2, h[m][k]), y23[m]);
           }
-        } else {
-          part[0] += __shfl_xor_sync(0xffffffffu, part[0], m);
         }
       }
-      float* out = &sh.y[c][stage * TILE + j + 4 - SUMS + lane * SUMS / L];
-      if constexpr (L == 4) *reinterpret_cast<float2*>(out) = make_float2(part[0], part[1]);
-      else *out = part[0];
+#pragma unroll
+      for (int m = 0; m < CH; m++) {
+        if constexpr (LOCAL) {
+          float s0, s1, s2, s3;
+          split(st[m].x, s0, s1);
+          split(st[m].y, s2, s3);
+          sum[m] += (s0 + s1) + (s2 + s3);
+        } else {
+          float part[SUMS];
+          split(y01[m], part[0], part[1]);
+          split(y23[m], part[2], part[3]);
+          // a step of the exchange leaves half of the tokens with each lane: lane l ends with the sum of token l SUMS / L (L > SUMS:
+          // neighbours with the same one)
+#pragma unroll
+          for (int q = L / 2, n = SUMS / 2; q >= 1; q /= 2, n /= 2) {
+            if (n >= 1) {
+#pragma unroll
+              for (int k = 0; k < n; k++) {
+                const bool up = lane & q;
+                const float give = up ? part[k] : part[n + k], keep = up ? part[n + k] : part[k];
+                part[k] = keep + __shfl_xor_sync(0xffffffffu, give, q);
+              }
+            } else {
+              part[0] += __shfl_xor_sync(0xffffffffu, part[0], q);
+            }
+          }
+          out[m * NEXT + j] = part[0];
+        }
+      }
     }
     bar_arrive(BAR_DONE + stage);
   }
@@ -530,24 +540,35 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) kda_selective_scan_kernel(con
     return;
   }
   const int lane = tid % L, c = tid / L;
-  const bool mine = c < w.channels;
-  const long long at = (long long)(w.d0 + (mine ? c : 0)) * p.Ns + lane, rows = (long long)p.Dm * p.Ns;
+  const long long rows = (long long)p.Dm * p.Ns;
   float* const own = p.ws_state + w.at * rows;       // a piece's state: first what it adds to the state, then the state it starts from
   const float* from = w.pieces > 1 ? own : (p.src != nullptr && slot >= 0 ? p.src + slot * p.src_stride : nullptr);
-  float a[S], h[S], sum = 0.0f;
+  float a[CH][S], h[CH][S], sum[CH];
 #pragma unroll
-  for (int k = 0; k < S; k++) {
-    const bool on = mine && lane + k * L < p.Ns;
-    a[k] = on ? decay_rate(p.A[at + k * L]) : 0.0f;
-    h[k] = !LOCAL && on && from != nullptr ? from[at + k * L] : 0.0f;
+  for (int m = 0; m < CH; m++) {
+    const int cm = c + m * CB / CH;
+    const long long at = (long long)(w.d0 + cm) * p.Ns + lane;
+    sum[m] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      const bool on = cm < w.channels && lane + k * L < p.Ns;
+      a[m][k] = on ? decay_rate(p.A[at + k * L]) : 0.0f;
+      h[m][k] = !LOCAL && on && from != nullptr ? from[at + k * L] : 0.0f;
+    }
   }
   scan<L, S, LOCAL>(w, sh, tid, a, h, sum);
   float* to = LOCAL ? own : (w.piece + 1 == w.pieces && p.dst != nullptr && slot >= 0 ? p.dst + slot * p.dst_stride : nullptr);
-  if (to == nullptr || !mine) return;
+  if (to == nullptr) return;
 #pragma unroll
-  for (int k = 0; k < S; k++)
-    if (lane + k * L < p.Ns) to[at + k * L] = h[k];
-  if (LOCAL && lane == 0) p.ws_sum[(long long)w.at * p.Dm + w.d0 + c] = sum;
+  for (int m = 0; m < CH; m++) {
+    const int cm = c + m * CB / CH;
+    const long long at = (long long)(w.d0 + cm) * p.Ns + lane;
+    if (cm >= w.channels) break;
+#pragma unroll
+    for (int k = 0; k < S; k++)
+      if (lane + k * L < p.Ns) to[at + k * L] = h[m][k];
+    if (LOCAL && lane == 0) p.ws_sum[(long long)w.at * p.Dm + w.d0 + cm] = sum[m];
+  }
 }
 
 // Between the passes over pieces: from what each piece adds to the state (and exp(A sum of its steps), what it leaves of the
@@ -788,7 +809,7 @@ cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
 // card (two an SM): 0 = no cut, else the tokens of a piece.
 long long sscan_piece(long long T, int N, int Dm, int Ns) {
   const int lanes = Ns <= 16 ? 4 : (Ns <= 32 ? 8 : (Ns <= 64 ? 16 : 32));
-  const long long blocks = (Dm + SCAN_LANES / lanes - 1) / (SCAN_LANES / lanes), room = 2 * 148;
+  const long long blocks = (Dm + CH * SCAN_LANES / lanes - 1) / (CH * SCAN_LANES / lanes), room = 2 * 148;
   if (blocks * N >= room || N > room || T < 512) return 0;
   const long long piece = (T * blocks / (4 * room) + TILE - 1) / TILE * TILE;
   return piece < 128 ? 128 : piece;
