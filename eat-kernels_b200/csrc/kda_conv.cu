@@ -50,7 +50,7 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (
 // VEC channels a thread, a tile of tokens a block.  A sequence's first W - 1 tokens belong to the tile that holds its start,
 // even where they reach into the next tile: only that tile reads the slot's history, and it writes the new one after that,
 // so the pool is updated in place by one launch.  Bound by memory: the window slides in registers, a tile re-reads W - 1
-// rows of the tile before it (out of L2).
+// rows of the tile before it (out of L2); 55 846 tokens of 6144 channels, W = 4: 271 us, 5.1 TB/s.
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const ConvParams p) {
   constexpr int HW = W - 1;

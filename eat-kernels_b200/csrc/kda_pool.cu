@@ -184,7 +184,8 @@ __device__ __forceinline__ void copy_chunk(unsigned char* dst, const unsigned ch
   }
 }
 
-// Bound by memory.  The number of moves is known on the device only: the grid covers the card and takes chunk after chunk.
+// Bound by memory.  The number of moves is known on the device only: the grid covers the card and takes chunk after chunk.  64 rows
+// of 1.04 MB: 18 us behind 5 us of plan.
 __global__ void __launch_bounds__(COPY_THREADS) kda_pool_copy_kernel(const PoolRows r, const int* __restrict__ moves) {
   int chunks = 0;
   for (int k = 0; k < r.n; k++) chunks += (int)((r.bytes[k] + COPY_CHUNK - 1) / COPY_CHUNK);

@@ -2,16 +2,18 @@
 //   s = softplus(dt + dt_bias);  h[n] = exp(s A[d,n]) h[n] + s u B[n];  y = sum_n C[n] h[n] + D[d] u;  y *= silu(z)
 //
 // What bounds it: one exponential a token, channel and state value, 16 a clock and SM in the special-function unit, which is
-// two to three times the time of the tokens' bytes.  So everything else is kept away from that unit and from the instruction
-// stream and the shared memory of the warps that feed it:
-//   * a block has eight scan warps and four helper warps.  The helpers load the tokens, work out the step sizes, s u, D u and
-//     the gate, and write the outputs; the scan warps only see shared memory.  Two stages of tokens between them, handed over
-//     by named barriers.  A warp by itself issues every third cycle at best (fp32 multiply-adds that do not depend on one
-//     another: 2.7 cycles), so a state is spread over as many warps as keep their instruction count.
+// about three times the time of the tokens' bytes; behind it the shared-memory pipe (a 16-byte access of a warp takes four
+// cycles, also where lanes read the same) and the instructions issued.  So:
+//   * a block has four scan warps and four helper warps.  The helpers bring the tokens by asynchronous copies, work out the step
+//     sizes and s u, and write the outputs with D u and the gate; the scan warps only see shared memory.  Two stages of tokens
+//     between them, handed over by named barriers.
 //   * shared memory holds time rows: a lane takes four tokens in one access, and all products but the chain itself run two
 //     tokens an instruction, without a value copied to make a pair.
-//   * a channel's state lies over L lanes, S values each.  Sums over the lanes are taken for a group of tokens at once, each
-//     step of the exchange halving the tokens that a lane holds.
+//   * a lane has two channels, so that B and C are read once for both, and S state values of each; L lanes share a channel.
+//     Sums over the lanes are taken for four tokens at once, each step of an exchange halving the tokens that a lane holds.
+// Measured (bf16, 16 state values): 8 ragged prompts, 10 245 tokens of 4096 channels, 272 us, the exponentials' unit busy 66 % of
+// it (one channel a lane: 308 us, the shared-memory pipe at 84 %); one prompt of 32 768 tokens on 512 channels 207 us in pieces
+// (uncut 1725 us).
 #include "kda_serving.cuh"
 
 namespace kda {
@@ -505,7 +507,7 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
 
 // A sequence, or a piece of one, and up to CB channels of one group a block.
 template <typename T, int L, int S, bool LOCAL, bool ASYNC>
-__global__ void __launch_bounds__(SCAN_THREADS, 2) kda_selective_scan_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(SCAN_THREADS, LOCAL ? 3 : 2) kda_selective_scan_kernel(const ScanParams p) {
   using Sh = ScanShared<L, S>;
   constexpr int CB = Sh::CB;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -608,7 +610,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(c
   }
 }
 
-// One token a row, ROWS rows a block for one load of A.  L lanes hold a channel's state, S consecutive values each; lane r works out
+// One token a row, ROWS rows a block for one load of A (256 rows of 4096 channels, 16 values: 39 us, 3.7 TB/s; a row a block with
+// every lane working out its step 57 us).  L lanes hold a channel's state, S consecutive values each; lane r works out
 // the step, the gate and the output of row r and hands the step round.  Bound by memory: the states of all rows are asked for before
 // anything else, and go through once.
 constexpr int ROWS = 4;
@@ -805,13 +808,15 @@ cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
 }  // namespace
 
 // Where whole sequences would leave SMs without work, they are cut: a first pass over the pieces finds what each adds to the
-// state, the states are joined, a second pass computes the outputs.  That is about 1.6 times the work, for blocks that fill the
-// card (two an SM): 0 = no cut, else the tokens of a piece.
+// state, the states are joined, a second pass computes the outputs.  That is about 1.6 times the work, for two rounds of blocks
+// that fill the card (two an SM): 0 = no cut, else the tokens of a piece.  The lengths lie on the device, so the rule goes by the
+// number of sequences.  32 768 tokens on 512 channels: one round of pieces 1725 us (uncut), two 207 us, four 218 us, eight 241 us;
+// 8192 tokens on 4096 channels (64 blocks uncut, 160 cycles a token: some 690 us) 378 us.
 long long sscan_piece(long long T, int N, int Dm, int Ns) {
   const int lanes = Ns <= 16 ? 4 : (Ns <= 32 ? 8 : (Ns <= 64 ? 16 : 32));
   const long long blocks = (Dm + CH * SCAN_LANES / lanes - 1) / (CH * SCAN_LANES / lanes), room = 2 * 148;
   if (blocks * N >= room || N > room || T < 512) return 0;
-  const long long piece = (T * blocks / (4 * room) + TILE - 1) / TILE * TILE;
+  const long long piece = (T * blocks / (2 * room) + TILE - 1) / TILE * TILE;
   return piece < 128 ? 128 : piece;
 }
 

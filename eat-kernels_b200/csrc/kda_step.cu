@@ -17,7 +17,8 @@ __device__ __forceinline__ float sigmoid_exact(float x) { return 1.0f / (1.0f + 
 // Value rows do not depend on one another, so a head is split over four blocks by value channels.  Value first (raw front-end): a warp
 // holds 8 rows of 128 keys, 4 keys a lane, and sums over its lanes.  Key first (plain): 8 lanes hold 32 value columns, the
 // 16 groups of lanes 8 keys each, and sum over shuffles and shared memory.  Bound by memory: 128 bytes a thread are in flight before the
-// token's operands are needed.
+// token's operands are needed and before the slots are looked through for repeats (48 rows of 64 heads: 70 us, 5.8 TB/s; with the
+// look in front of the loads 80 us).
 template <bool RAW>
 __global__ void __launch_bounds__(STEP_THREADS) kda_step_kernel(const StepParams p) {
   constexpr bool KEY_FIRST = !RAW;

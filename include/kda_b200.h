@@ -1,4 +1,5 @@
-/* C ABI of the B200 KDA-prefill library (libkda_b200.so).
+/* C ABI of the B200 KDA-prefill library (libkda_b200.so): the prefill, and the operators of a server of recurrent layers around
+ * it (short convolution, selective scan, single-token steps, slot pools; from KdaSequences on).
  *
  * Plain pointers and sizes only; every pointer marked "device" is a CUDA device address on the current device.
  * Every entry point returns 0 or a negative KDA_ERR_* code, never throws, never synchronises the device and never
@@ -234,7 +235,8 @@ int kda_state_rows_copy(void* dst, int64_t dst_row_stride, int32_t dst_is_bf16, 
 /* ---- the operators around the prefill in a recurrent layer.  No counterpart in the reference, which stops at the prefill.
  * Token tensors are packed as there: [T] rows of one token, ld* = elements between consecutive rows (>= the row), values of a
  * row consecutive.  16-byte alignment is not needed, but rows that all start on 16 bytes are read fastest.  Written buffers
- * may not overlap anything else (a state buffer may be source and destination at once).  One kernel launch each. */
+ * may not overlap anything else (a state buffer may be source and destination at once).  One kernel launch each, three for a
+ * scan that is cut into pieces. */
 enum { KDA_TYPE_BF16 = 0, KDA_TYPE_FP16 = 1, KDA_TYPE_FP32 = 2 };
 
 /* Further bits of `status` in these calls, which OR them in (the caller clears it): KDA_STATUS_BAD_CU (every sequence taken as
