@@ -607,7 +607,9 @@ int kda_step_launch(const KdaStepArgs* a, void* stream) {
 
 size_t kda_pool_workspace_bytes(int64_t n, int64_t P) {
   if (n < 0 || P < 1) return 0;
-  return sizeof(int) * (size_t)(4 + (3 * n > P + 2 ? 3 * n : P + 2));   // pairs and free slots of n entries, or P / 2 moves
+  // P / 2 moves (compact); pairs and free slots of n entries (fork); pairs of n entries and two tables of slots (copy)
+  const int64_t compact = P + 2, fork = 3 * n, copy = 2 * n + 2 * P;
+  return sizeof(int) * (size_t)(4 + (n == 0 ? compact : (fork > copy ? fork : copy)));
 }
 
 int kda_pool_copy_launch(const KdaPoolArgs* a, void* stream) {

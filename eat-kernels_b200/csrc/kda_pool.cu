@@ -43,26 +43,41 @@ __device__ __forceinline__ void share_of(long long n, long long& first, long lon
 
 // dst[i] <- src[i].  A destination that an earlier entry names, or that some entry reads, would make the result depend on the
 // order: such entries are left out, as are those out of range.  A negative destination is padding, a negative source zeros.
+// Each slot that is named has the first entry that writes it, and whether one reads it, in two tables behind the moves.
 __global__ void __launch_bounds__(PLAN_THREADS, 1) kda_pool_copy_plan_kernel(const PoolPlan p) {
   __shared__ int s_count;
+  int *first = p.moves + 4 + 2 * p.n, *read = first + p.P;
   if (threadIdx.x == 0) s_count = 0;
+  // an entry of a table: -1 negative, P out of range
+  auto entry = [&](const void* table, int is64, long long i) {
+    const long long d = table_at(table, is64, i);
+    return d < 0 ? -1 : (int)min(d, p.P);
+  };
+  for (long long i = threadIdx.x; i < p.n; i += PLAN_THREADS) {
+    const int d = entry(p.dst, p.dst_is64, i);
+    if (d >= 0 && d < p.P) {
+      first[d] = 0x7fffffff;
+      read[d] = 0;
+    }
+  }
   __syncthreads();
   for (long long i = threadIdx.x; i < p.n; i += PLAN_THREADS) {
-    const long long d = table_at(p.dst, p.dst_is64, i), s = table_at(p.src, p.src_is64, i);
-    if (d < 0 || d == s) {
-      if (d >= p.P) report(p.status, SEQ_BAD_SLOT);
+    const int d = entry(p.dst, p.dst_is64, i), s = entry(p.src, p.src_is64, i);
+    if (d < 0) continue;
+    if (d < p.P) atomicMin(&first[d], (int)i);
+    if (s >= 0 && s < p.P) read[s] = 1;
+  }
+  __syncthreads();
+  for (long long i = threadIdx.x; i < p.n; i += PLAN_THREADS) {
+    const int d = entry(p.dst, p.dst_is64, i), s = entry(p.src, p.src_is64, i);
+    if (d < 0 || (d == s && d < p.P)) continue;      // padding; a row onto itself
+    if (d >= p.P || s >= p.P || first[d] != (int)i || read[d] != 0) {
+      report(p.status, SEQ_BAD_SLOT);
       continue;
     }
-    bool ok = d < p.P && s < p.P;
-    for (long long j = 0; j < p.n && ok; j++) {
-      const long long dj = table_at(p.dst, p.dst_is64, j);
-      if (j < i && dj == d) ok = false;
-      if (dj >= 0 && table_at(p.src, p.src_is64, j) == d) ok = false;
-    }
-    if (!ok) { report(p.status, SEQ_BAD_SLOT); continue; }
     const int at = atomicAdd(&s_count, 1);
-    p.moves[4 + 2 * at] = s < 0 ? -1 : (int)s;
-    p.moves[5 + 2 * at] = (int)d;
+    p.moves[4 + 2 * at] = s;
+    p.moves[5 + 2 * at] = d;
   }
   __syncthreads();
   if (threadIdx.x == 0) p.moves[0] = s_count;

@@ -71,7 +71,7 @@ struct PoolPlan {
   long long table_n[TABLES_MAX];
   int table_is64[TABLES_MAX];
   int n_tables;
-  int* moves;              // [0] count, then pairs from [4]
+  int* moves;              // the workspace: [0] count, pairs from [4], a plan's own tables behind them
   int* status;
   long long P;
 };

@@ -143,7 +143,8 @@ struct Work {                                        // a block's share
   long long begin;                                   // first token
 };
 
-constexpr int RANKED = 128;                          // up to so many sequences the longest goes first
+constexpr int RANKED = 128;                          // up to so many sequences the longest goes first, where not all blocks have room at once
+constexpr int ROOM = 2 * 148;
 
 // Pieces that a sequence is cut into (empty sequences have one, for their state).
 __device__ __forceinline__ int pieces_of(const ScanParams& p, bool rejected, int seq) {
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, LOCAL ? 3 : 2) kda_selective_sca
   if (p.piece > 0) {
     if (!find_piece(p, rejected, w.at, w) || (LOCAL && w.piece + 1 == w.pieces)) return;
   } else {
-    w.seq = p.seq.N > 1 && p.seq.N <= RANKED && !rejected ? by_length(p, w.at) : w.at;
+    w.seq = p.seq.N > 1 && p.seq.N <= RANKED && gridDim.x > ROOM && !rejected ? by_length(p, w.at) : w.at;
     w.piece = 0;
     w.pieces = 1;
   }
@@ -814,9 +815,9 @@ cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
 // 8192 tokens on 4096 channels (64 blocks uncut, 160 cycles a token: some 690 us) 378 us.
 long long sscan_piece(long long T, int N, int Dm, int Ns) {
   const int lanes = Ns <= 16 ? 4 : (Ns <= 32 ? 8 : (Ns <= 64 ? 16 : 32));
-  const long long blocks = (Dm + CH * SCAN_LANES / lanes - 1) / (CH * SCAN_LANES / lanes), room = 2 * 148;
-  if (blocks * N >= room || N > room || T < 512) return 0;
-  const long long piece = (T * blocks / (2 * room) + TILE - 1) / TILE * TILE;
+  const long long blocks = (Dm + CH * SCAN_LANES / lanes - 1) / (CH * SCAN_LANES / lanes);
+  if (blocks * N >= ROOM || N > ROOM || T < 512) return 0;
+  const long long piece = (T * blocks / (2 * ROOM) + TILE - 1) / TILE * TILE;
   return piece < 128 ? 128 : piece;
 }
 

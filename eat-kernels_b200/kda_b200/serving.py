@@ -133,7 +133,7 @@ def _call(check, tensors, *options):
     try:
         key = (check, options, *[t if t is None else (t.dtype, t.shape, t.stride(), t.device) for t in tensors])
         plan = _plans.get(key)
-    except (AttributeError, TypeError):                # not tensors: the checks say so
+    except (AttributeError, TypeError, RuntimeError):  # not tensors, or without strides: the checks say so
         key = plan = None
     if plan is not None:
         result = plan.run(tensors)

@@ -137,6 +137,30 @@ def test_copies_that_depend_on_the_order_are_left_out(status):
     assert int(status) == 2 and pool[:, 0].tolist() == [0, 1, 2, 2, 4, 5, 6, 4, 9, 9]
 
 
+@pytest.mark.parametrize("n", [1, 1023, 1025, 2600])
+def test_copies_by_long_tables(n, status):
+    """Random tables against the rule entry by entry: repeats, chains, rows onto themselves, padding, entries out of range."""
+    import kda_b200
+    host = torch.Generator().manual_seed(n)
+    P = 3 * n + 5
+    pool = torch.arange(float(P), device=DEV)[:, None].clone()
+    src, dst = torch.randint(-2, P + 2, (n,), generator=host), torch.randint(-2, P + 2, (n,), generator=host)
+    some = torch.rand(n, generator=host) < 0.05
+    dst[some] = src[some]
+    want, seen, reads, bad = list(range(P)), set(), {s for s, d in zip(src.tolist(), dst.tolist()) if d >= 0}, False
+    for s, d in zip(src.tolist(), dst.tolist()):
+        if d < 0 or (d == s and d < P):
+            seen |= {d}
+            continue
+        if d >= P or s >= P or d in seen or d in reads:
+            bad = True
+        else:
+            want[d] = float(max(s, 0)) if s >= 0 else 0.0
+        seen |= {d}
+    kda_b200.pool_copy([pool], src.to(DEV), dst.to(torch.int32).to(DEV), status=status)
+    assert pool[:, 0].tolist() == want and int(status) == (2 if bad else 0)
+
+
 def test_strided_pools_keep_what_lies_between_their_slots():
     import kda_b200
     gen = generator(10)
