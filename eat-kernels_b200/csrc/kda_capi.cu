@@ -535,7 +535,7 @@ int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
 // The parts of the argument block that a call uses, checked; fills the kernels' parameters.
 int pool_params(const KdaPoolArgs* a, bool used, bool src, bool copies, kda::PoolPlan& p, kda::PoolRows& r) {
   if (a == nullptr || a->slots < 1 || a->n < 0) return KDA_ERR_ARG;
-  if (a->slots > 0x7fffffffLL || a->n > 0x3fffffffLL) return KDA_ERR_LIMIT;
+  if (a->slots > 0x3fffffffLL || a->n > 0x1fffffffLL) return KDA_ERR_LIMIT;
   if ((used && !a->used) || (src && a->n > 0 && !a->src)) return KDA_ERR_ARG;
   if (!whole_table(a->src, a->src_is64) || !whole_table(a->dst, a->dst_is64) || !whole_table(a->status, 0) || !whole_table(a->slots_out, 0) ||
       !whole_table(a->remap, 0)) return KDA_ERR_ARG;

@@ -99,10 +99,10 @@ __device__ __forceinline__ void row_slots(const SeqTable& s, int row0, int rows,
   }
 }
 
-// Then, called by the whole block: -1 for a slot that an earlier row has claimed too.
+// Then, called by the whole block: -1 for a slot that an earlier row has claimed too.  Says whether any row is at -1 now.
 template <int R>
-__device__ __forceinline__ void drop_repeats(const SeqTable& s, int row0, int (&slot)[R]) {
-  if (s.slots == nullptr) return;
+__device__ __forceinline__ bool drop_repeats(const SeqTable& s, int row0, int (&slot)[R]) {
+  if (s.slots == nullptr) return false;
   int bad = 0;
   for (int j = threadIdx.x; j < row0; j += blockDim.x) {
     const int d = slot_entry(s, j);
@@ -117,11 +117,12 @@ __device__ __forceinline__ void drop_repeats(const SeqTable& s, int row0, int (&
     for (int q = 0; q < r; q++)
       if (slot[r] >= 0 && slot[r] == slot[q]) bad |= 1 << r;
   }
-  if (__syncthreads_or(bad) == 0) return;
+  if (__syncthreads_or(bad) == 0) return false;
 #pragma unroll
   for (int r = 0; r < R; r++)
     if (__syncthreads_or(bad >> r & 1)) slot[r] = -1;
   if (threadIdx.x == 0) report(s.status, SEQ_BAD_SLOT);
+  return true;
 }
 
 // ---- token types

@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(c
   }
 }
 
-// One token a row, ROWS rows a block for one load of A (256 rows of 4096 channels, 16 values: 39 us, 3.7 TB/s; a row a block with
+// One token a row, ROWS rows a block for one load of A (256 rows of 4096 channels, 16 values: 37 us, 3.8 TB/s; a row a block with
 // every lane working out its step 57 us).  L lanes hold a channel's state, S consecutive values each; lane r works out
 // the step, the gate and the output of row r and hands the step round.  Bound by memory: the states of all rows are asked for before
 // anything else, and go through once.
@@ -628,14 +628,24 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
   int slot[ROWS];
   row_slots(p.seq, row0, rows, slot);
   const long long at = (long long)dc * p.Ns + n;
-  // S consecutive values of which `left` there are: one access where WIDE
+  // S consecutive values of a row of states: one access where WIDE
   auto values = [&](const float* q) {
     Values<S> v;
     if constexpr (WIDE) {
-      v = n < p.Ns ? load_values<S>(q) : Values<S>();
+      v = load_values<S>(q);
     } else {
 #pragma unroll
       for (int k = 0; k < S; k++) v.v[k] = n + k < p.Ns ? q[k] : 0.0f;
+    }
+    return v;
+  };
+  auto tokens = [&](const T* q) {
+    Pack<T, S> v;
+    if constexpr (WIDE) {
+      v = *reinterpret_cast<const Pack<T, S>*>(q);
+    } else {
+#pragma unroll
+      for (int k = 0; k < S; k++) v.v[k] = n + k < p.Ns ? q[k] : from_float<T>(0.0f);
     }
     return v;
   };
@@ -643,26 +653,17 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
 #pragma unroll
   for (int r = 0; r < ROWS; r++)
     if (slot[r] >= 0) h[r] = values(p.src + slot[r] * p.src_stride + at);
+  // what a row of padding brings is worked on like the rest, and dropped
   Pack<T, S> rb[ROWS], rc[ROWS];
+  const T* B = reinterpret_cast<const T*>(p.B) + row0 * p.ldb + (long long)group * p.Ns + n;
+  const T* C = reinterpret_cast<const T*>(p.C) + row0 * p.ldc + (long long)group * p.Ns + n;
 #pragma unroll
   for (int r = 0; r < ROWS; r++) {
-    const T* B = reinterpret_cast<const T*>(p.B) + (long long)(row0 + r) * p.ldb + (long long)group * p.Ns + n;
-    const T* C = reinterpret_cast<const T*>(p.C) + (long long)(row0 + r) * p.ldc + (long long)group * p.Ns + n;
-#pragma unroll
-    for (int k = 0; k < S; k++) rb[r].v[k] = rc[r].v[k] = from_float<T>(0.0f);
-    if (slot[r] == -2) continue;
-    if constexpr (WIDE) {
-      if (n < p.Ns) {
-        rb[r] = *reinterpret_cast<const Pack<T, S>*>(B);
-        rc[r] = *reinterpret_cast<const Pack<T, S>*>(C);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < S; k++)
-        if (n + k < p.Ns) {
-          rb[r].v[k] = B[k];
-          rc[r].v[k] = C[k];
-        }
+    rb[r] = tokens(B);
+    rc[r] = tokens(C);
+    if (r + 1 < rows) {
+      B += p.ldb;
+      C += p.ldc;
     }
   }
   // lane r: row r
@@ -676,27 +677,27 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
   for (int k = 0; k < S; k++) a.v[k] *= LOG2E_F;
   if (p.softplus) s = softplus(s);
   const float su = s * u;
-  drop_repeats(p.seq, row0, slot);
+  if (drop_repeats(p.seq, row0, slot)) {
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+      if (slot[r] < 0) h[r] = Values<S>();
+  }
   float part[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; r++) {
     const float sr = __shfl_sync(0xffffffffu, s, r, L), sur = __shfl_sync(0xffffffffu, su, r, L);
-    part[r] = 0.0f;
-    if (slot[r] == -2) continue;
-    if (slot[r] == -1) h[r] = Values<S>();
     float b[S], c[S];
     unpack(rb[r], b);
     unpack(rc[r], c);
 #pragma unroll
     for (int k = 0; k < S; k++) {
-      if (!WIDE && n + k >= p.Ns) continue;
       h[r].v[k] = fmaf(exp2_fast(sr * a.v[k]), h[r].v[k], sur * b[k]);
-      part[r] = fmaf(c[k], h[r].v[k], part[r]);
+      part[r] = k == 0 ? c[k] * h[r].v[k] : fmaf(c[k], h[r].v[k], part[r]);
     }
     if (slot[r] >= 0 && mine) {
       float* to = p.dst + slot[r] * p.dst_stride + at;
       if constexpr (WIDE) {
-        if (n < p.Ns) store_values<S>(to, h[r]);
+        store_values<S>(to, h[r]);
       } else {
 #pragma unroll
         for (int k = 0; k < S; k++)
@@ -788,10 +789,10 @@ cudaError_t launch_step(const ScanParams& p, cudaStream_t stream) {
   if (rows == 0) return cudaSuccess;
   if (rows > 65535) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((p.Dm + STEP_LANES / L - 1) / (STEP_LANES / L)), (unsigned)rows);
-  // one access for S values where all start on as many
+  // one access for S values where all start on as many and no lane has fewer
   const uintptr_t f = reinterpret_cast<uintptr_t>(p.src) | reinterpret_cast<uintptr_t>(p.A) | (uintptr_t)(p.src_stride * 4);
   const uintptr_t t = reinterpret_cast<uintptr_t>(p.B) | reinterpret_cast<uintptr_t>(p.C) | (uintptr_t)((p.ldb | p.ldc) * (long long)sizeof(T));
-  if ((f & (S * 4 - 1)) == 0 && (t & (S * sizeof(T) - 1)) == 0 && p.Ns % S == 0) kda_selective_scan_step_kernel<T, L, S, true><<<grid, STEP_LANES, 0, stream>>>(p);
+  if ((f & (S * 4 - 1)) == 0 && (t & (S * sizeof(T) - 1)) == 0 && p.Ns == L * S) kda_selective_scan_step_kernel<T, L, S, true><<<grid, STEP_LANES, 0, stream>>>(p);
   else kda_selective_scan_step_kernel<T, L, S, false><<<grid, STEP_LANES, 0, stream>>>(p);
   return cudaGetLastError();
 }

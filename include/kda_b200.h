@@ -326,14 +326,14 @@ int kda_step_launch(const KdaStepArgs* args, void* stream);
 typedef struct KdaPoolArgs {
   void* base[KDA_MAX_POOLS];
   int64_t stride[KDA_MAX_POOLS], bytes[KDA_MAX_POOLS];
-  int64_t slots;           /* P, of every pool; at most 2^31 - 1 */
+  int64_t slots;           /* P, of every pool; at most 2^30 - 1 */
   int32_t n_pools;
   int32_t n_tables;        /* compact: tables to rewrite */
   uint8_t* used;           /* device [P]: 0 = free (not for copy) */
   const void* src;         /* device [n]: copy: source slots, negative = zeros; fork: parents, negative = none (zeros); free: slots,
                               negative = padding */
   const void* dst;         /* device [n]: copy: destination slots, negative = padding */
-  int64_t n;               /* entries of src / dst */
+  int64_t n;               /* entries of src / dst; at most 2^29 - 1 */
   int32_t src_is64, dst_is64;
   int32_t* slots_out;      /* fork: device [n], the new slots (-1: none) */
   int32_t* remap;          /* compact: device [P], where each slot went (-1: was free) */
