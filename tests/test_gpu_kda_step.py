@@ -129,6 +129,16 @@ def test_the_token_after_a_prompt(raw):
     ko.check_close(pool, final, "final state")
 
 
+def test_other_types_are_cast_as_in_the_prefill():
+    import kda_b200
+    gen = generator(37)
+    a, pool = make(gen, 3, 2, True), randn(gen, 3, 2, 128, 128, scale=0.25)
+    one, two = pool.clone(), pool.clone()
+    y, _ = kda_b200.kda_step(**a, scale=0.1, pool=one)
+    z, _ = kda_b200.kda_step(**{n: t.double() if n in ("A_log", "dt_bias") else t.float() for n, t in a.items()}, scale=0.1, pool=two)
+    assert torch.equal(y, z) and torch.equal(one, two) and z.dtype == BF
+
+
 def test_captured_calls_follow_their_table():
     gen, N = generator(34), 4
     for raw in (True, False):

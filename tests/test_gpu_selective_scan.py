@@ -321,6 +321,39 @@ def test_captured_calls_follow_their_tables():
     check(a, torch.zeros(N, 96, 16, device=DEV), [90, 0, 0, 0, 0, 0], z, final)
 
 
+def test_captured_pieces_follow_their_tables():
+    """A long axis on few channels is cut by its size alone: a replay may have any layout of as many sequences."""
+    import kda_b200
+    gen, N, T = generator(23), 5, 1200
+    a, pool = make(gen, T, 48, 16, 1, BF), randn(gen, 8, 48, 16)
+    cu, slots = cu_of([240] * N), torch.arange(N, device=DEV)
+    kda_b200.selective_scan(**a, initial_state=pool.clone(), cu_seqlens=cu, ssm_state_indices=slots)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(kda_b200.selective_scan(**a, initial_state=pool, cu_seqlens=cu, ssm_state_indices=slots)[0])
+    for lens, ids in (([1200, 0, 0, 0, 0], [4, 1, 2, 3, 0]), ([1, 128, 129, 0, 942], [7, 0, 3, 5, 6]), ([240] * N, [0, 1, 2, 3, 4]), ([0, 0, 0, 0, 300], [5, 6, 7, 0, 1])):
+        cu.copy_(cu_of(lens))
+        slots.copy_(torch.tensor(ids))
+        for graph, y in zip(graphs, outs):
+            before = pool.clone()
+            graph.replay()
+            check(a, before[slots], lens, y, pool[slots])
+            assert bool((y[:, sum(lens):] == 0).all())
+
+
+def test_states_and_rates_in_other_orders():
+    import kda_b200
+    gen, lens = generator(24), [30, 20]
+    a = make(gen, 50, 64, 16, 1, F)
+    init = randn(gen, 2, 16, 64).transpose(1, 2)
+    a["A"] = a["A"].t().contiguous().t()
+    for _ in range(2):
+        y, final = kda_b200.selective_scan(**a, initial_state=init, cu_seqlens=cu_of(lens).cpu())
+        check(a, init, lens, y, final)
+
+
 def test_offsets_behind_32_bits():
     import kda_b200
     Dm, T = 8192, 270_000
