@@ -8,7 +8,7 @@ namespace kda {
 namespace {
 
 constexpr int CONV_THREADS = 128;
-constexpr int GROUP = 8;                 // rows in flight
+constexpr int GROUP = 4;                 // tokens whose rows are asked for together
 
 // N consecutive values, in 8-byte accesses where they start on 8 bytes
 template <typename T, int N>
@@ -50,9 +50,9 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (
 // VEC channels a thread, a tile of tokens a block.  A sequence's first W - 1 tokens belong to the tile that holds its start,
 // even where they reach into the next tile: only that tile reads the slot's history, and it writes the new one after that,
 // so the pool is updated in place by one launch.  Bound by memory: the window slides in registers, a tile re-reads W - 1
-// rows of the tile before it (out of L2); 55 846 tokens of 6144 channels, W = 4: 271 us, 5.1 TB/s.
+// rows of the tile before it (out of L2); 55 846 tokens of 6144 channels, W = 4: 259 us, 5.3 TB/s.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const ConvParams p) {
+__global__ void __launch_bounds__(CONV_THREADS, 7) kda_short_conv_kernel(const ConvParams p) {
   constexpr int HW = W - 1;
   using P = Pack<T, VEC>;
   const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
@@ -91,14 +91,24 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_kernel(const Conv
     }
     *reinterpret_cast<P*>(out + t * p.ldo) = pack<T, VEC>(y);
   };
-  // tokens in groups: a group's rows are all on their way before the first is used
+  // tokens in groups: a group's rows are on their way while the group in front is worked on (two groups of four: 259 us on the
+  // batch above, one of eight at a time 272, two of eight 271, two of two 300)
   auto run = [&](long long from, long long to, float (&win)[HW][VEC]) {
-    for (; from + GROUP <= to; from += GROUP) {
-      P rows[GROUP];
+    if (from + GROUP <= to) {
+      P rows[GROUP], next[GROUP];
 #pragma unroll
       for (int g = 0; g < GROUP; g++) rows[g] = *reinterpret_cast<const P*>(x + (from + g) * p.ldx);
+      for (; from + GROUP <= to; from += GROUP) {
+        const bool more = from + 2 * GROUP <= to;
+        if (more) {
 #pragma unroll
-      for (int g = 0; g < GROUP; g++) token(from + g, rows[g], win);
+          for (int g = 0; g < GROUP; g++) next[g] = *reinterpret_cast<const P*>(x + (from + GROUP + g) * p.ldx);
+        }
+#pragma unroll
+        for (int g = 0; g < GROUP; g++) token(from + g, rows[g], win);
+#pragma unroll
+        for (int g = 0; g < GROUP; g++) rows[g] = next[g];
+      }
     }
     for (; from < to; from++) token(from, *reinterpret_cast<const P*>(x + from * p.ldx), win);
   };
@@ -207,7 +217,7 @@ __global__ void __launch_bounds__(CONV_THREADS) kda_short_conv_step_kernel(const
 }
 
 // Four channels an access where every row starts on as many, single values elsewhere.  Eight 16-bit channels take 187 registers, which
-// leaves two blocks an SM: 471 us for 56 k tokens of 6144 channels against 273 us with four.
+// leaves two blocks an SM: 471 us for 56 k tokens of 6144 channels against 273 us with four (before the groups of four).
 constexpr int WIDE = 4;
 template <typename T>
 bool wide(const ConvParams& p) {
@@ -242,7 +252,7 @@ template <typename T>
 cudaError_t launch_type(ConvParams p, bool step, cudaStream_t stream) {
   const bool w = wide<T>(p);
   const long long cblocks = (p.C / (w ? WIDE : 1) + CONV_THREADS - 1) / CONV_THREADS;
-  p.tile = step ? tile_of(p.seq.T, cblocks, 1, STEP_ROWS) : tile_of(p.seq.T, cblocks, 8, 128);
+  p.tile = step ? tile_of(p.seq.T, cblocks, 1, STEP_ROWS) : tile_of(p.seq.T, cblocks, 8, 64);
   return w ? launch_width<T, WIDE>(p, step, stream) : launch_width<T, 1>(p, step, stream);
 }
 
