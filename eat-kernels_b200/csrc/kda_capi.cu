@@ -553,7 +553,6 @@ int pool_params(const KdaPoolArgs* a, bool used, bool src, bool copies, kda::Poo
     if (a->workspace_bytes < kda_pool_workspace_bytes(a->n, a->slots)) return KDA_ERR_WORKSPACE;
   }
   r.n = a->n_pools;
-  r.slots = a->slots;
   p.used = a->used; p.src = a->src; p.dst = a->dst; p.src_is64 = a->src_is64; p.dst_is64 = a->dst_is64; p.n = a->n;
   p.slots_out = a->slots_out; p.remap = a->remap; p.moves = reinterpret_cast<int*>(a->workspace); p.status = a->status; p.P = a->slots;
   return KDA_OK;

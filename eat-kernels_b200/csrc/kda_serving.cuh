@@ -16,7 +16,7 @@ struct ConvParams {
   SeqTable seq;
   long long ldx, ldo, src_stride, dst_stride;
   int C, W, silu, weight_type, zero_pad;
-  int tile, vec;           // set by the launcher
+  int tile;                // rows of a block, set by the launcher
 };
 cudaError_t launch_conv(ConvParams p, int type, cudaStream_t stream);
 cudaError_t launch_conv_step(ConvParams p, int type, cudaStream_t stream);
@@ -56,7 +56,6 @@ struct PoolRows {          // the pools that share one table of slots
   unsigned char* base[POOLS_MAX];
   long long stride[POOLS_MAX], bytes[POOLS_MAX];
   int n;
-  long long slots;
 };
 // Copies named by a table: plan -> `moves` (source, destination; source -1: zeros), then the bytes.
 struct PoolPlan {
