@@ -430,8 +430,12 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 // The scan warps' half: lane l of a channel holds the state values l + k L.  A tile is one run of instructions, four tokens after
 // four; tokens behind the last one leave the state as it is.
 // LOCAL: the state alone, and the sum of the steps.
-template <int L, int S, bool LOCAL>
-__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, const float (&a)[CH][S], float (&h)[CH][S], float (&sum)[CH]) {
+// PADDED: there are only `states` of the L S state values.  The places behind them hold B = C = 0, which an infinite step or s u turns
+// into NaN (0 times inf): the sums take them as zeros, and nothing else reads them.  The
+// lower half of a lane's places always has values.
+template <int L, int S, bool LOCAL, bool PADDED>
+__device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, int states, const float (&a)[CH][S], float (&h)[CH][S],
+                                     float (&sum)[CH]) {
   constexpr int R = ScanShared<L, S>::R, NEXT = ScanShared<L, S>::CB / CH * R;
   constexpr int SUMS = 4;                            // tokens that are summed over the lanes at a time
   const int lane = tid % L, c = tid / L;
@@ -467,8 +471,10 @@ __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int ti
           const float h0 = fmaf(exp2_fast(x0), h[m][k], i0), h1 = fmaf(exp2_fast(x1), h0, i1), h2 = fmaf(exp2_fast(x2), h1, i2);
           h[m][k] = fmaf(exp2_fast(x3), h2, i3);
           if constexpr (!LOCAL) {
-            y01[m] = k == 0 ? mul2(ck.x, f2(h0, h1)) : fma2(ck.x, f2(h0, h1), y01[m]);
-            y23[m] = k == 0 ? mul2(ck.y, f2(h2, h[m][k])) : fma2(ck.y, f2(h2, h[m][k]), y23[m]);
+            F2 h01 = f2(h0, h1), h23 = f2(h2, h[m][k]);
+            if (PADDED && k >= S / 2 && lane + k * L >= states) h01 = h23 = 0;
+            y01[m] = k == 0 ? mul2(ck.x, h01) : fma2(ck.x, h01, y01[m]);
+            y23[m] = k == 0 ? mul2(ck.y, h23) : fma2(ck.y, h23, y23[m]);
           }
         }
       }
@@ -559,7 +565,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, LOCAL ? 3 : 2) kda_selective_sca
       h[m][k] = !LOCAL && on && from != nullptr ? from[at + k * L] : 0.0f;
     }
   }
-  scan<L, S, LOCAL>(w, sh, tid, a, h, sum);
+  if (!LOCAL && p.Ns < L * S) scan<L, S, LOCAL, !LOCAL>(w, sh, tid, p.Ns, a, h, sum);
+  else scan<L, S, LOCAL, false>(w, sh, tid, p.Ns, a, h, sum);
   float* to = LOCAL ? own : (w.piece + 1 == w.pieces && p.dst != nullptr && slot >= 0 ? p.dst + slot * p.dst_stride : nullptr);
   if (to == nullptr) return;
 #pragma unroll
@@ -693,6 +700,13 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
     for (int k = 0; k < S; k++) {
       h[r].v[k] = fmaf(exp2_fast(sr * a.v[k]), h[r].v[k], sur * b[k]);
       part[r] = k == 0 ? c[k] * h[r].v[k] : fmaf(c[k], h[r].v[k], part[r]);
+    }
+    // places behind the state values hold B = C = 0, which an infinite s u turns into NaN (0 times inf): a sum without them
+    if (!WIDE && !(fabsf(sur) < INFINITY)) {
+      part[r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S; k++)
+        if (n + k < p.Ns) part[r] = fmaf(c[k], h[r].v[k], part[r]);
     }
     if (slot[r] >= 0 && mine) {
       float* to = p.dst + slot[r] * p.dst_stride + at;

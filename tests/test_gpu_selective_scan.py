@@ -373,3 +373,43 @@ def test_offsets_behind_32_bits():
     y, _ = kda_b200.selective_scan_step(**tok, pool=pool, ssm_state_indices=torch.tensor([16_999, 3], device=DEV))
     check(tok, torch.zeros(2, Dm, 16, device=DEV), [1, 1], y, pool[[16_999, 3]])
     assert int((pool != 0).any(-1).any(-1).sum()) == 2
+
+
+def same(got, want, what):
+    """Equal where `want` is infinite or not a number; nothing is said about the rest."""
+    got, want = got.double(), want.to(got.device)
+    assert torch.equal(got.isnan(), want.isnan()), what
+    assert torch.equal(torch.where(want.isinf(), want, 0.0), torch.where(got.isinf(), got, 0.0)), what
+
+
+@pytest.mark.parametrize("dtype,Ns", [(F, 1), (BF, 3), (HF, 13), (BF, 16), (F, 24), (BF, 24), (F, 33), (HF, 100)])
+@pytest.mark.parametrize("how", ["whole", "pieces", "step"])
+def test_infinite_tokens_reach_no_state_that_does_not_exist(dtype, Ns, how):
+    """An infinite u (channel 0) or dt (channel 1) makes the states and outputs from there on infinite, not NaN, whatever the number of
+    state values (B, C, D positive, so that no infinities cancel); the other channels stay as they are."""
+    import kda_b200
+    gen, T = generator(30 + Ns), 600 if how == "pieces" else 40
+    a = make(gen, T, 24, Ns, 1, dtype, gate=False)
+    for n in "BC":
+        a[n] = a[n].abs() + 0.5
+    a["A"] = a["A"] / Ns                                              # no single step's decay is zero in fp32
+    a["u"][..., :2] = a["u"][..., :2].abs()
+    a["D"][:2] = 1.0
+    a["u"][0, 21, 0] = a["dt"][0, 9, 1] = float("inf")
+    lens = [1] * T if how == "step" else [T]
+    init = torch.zeros(len(lens), 24, Ns, device=DEV)
+    if how == "step":
+        final = init.clone()
+        y, _ = kda_b200.selective_scan_step(**a, pool=final)
+    else:
+        y, final = kda_b200.selective_scan(**a, initial_state=init)
+    rest = {n: t[..., 2:] if n in ("u", "dt") else t[2:] if n in ("A", "D", "dt_bias") else t for n, t in a.items() if t is not None}
+    check(dict(rest, z=None), init[:, 2:], lens, y[..., 2:], final[:, 2:])
+    t = 0
+    for i, n in enumerate(lens):
+        s = at(a, slice(t, t + n))
+        want, _, h, _ = scan64(s["u"][0], s["dt"][0], a["A"], s["B"][0], s["C"][0], a["D"], None, a["dt_bias"], init[i], True)
+        assert not bool(want.isnan().any()) and not bool(h.isnan().any())
+        same(y[0, t:t + n, :2], want[:, :2], f"sequence {i}")
+        same(final[i, :2], h[:2], f"state {i}")
+        t += n
