@@ -285,7 +285,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
   constexpr int CA = Sh::CB / 2;
   static_assert(CA * QUADS <= HELPERS, "one block of two channels and four tokens a helper");
   constexpr int NA = Sh::NP / 2, BBLOCKS = (LOCAL ? 1 : 2) * NA * QUADS, EB = (BBLOCKS + HELPERS - 1) / HELPERS;     // blocks of B, then of C
-  const bool has_z = !LOCAL && p.z != nullptr;
+  const bool has_z = !LOCAL && p.z != nullptr, has_skip = p.D != nullptr;
   const int tiles = (int)(((long long)w.tokens + TILE - 1) / TILE);
   Bring<T, Sh::CB, Rw::XS, 3, ASYNC> bx({p.u, p.dt, p.z}, {p.ldu, p.lddt, p.ldz}, w.begin, w.d0, w.channels, w.tokens, tid);
   Bring<T, Sh::NP, Rw::NS, 2, ASYNC> bbc({p.B, p.C}, {p.ldb, p.ldc}, w.begin, (long long)w.group * p.Ns, p.Ns, w.tokens, tid);
@@ -308,7 +308,7 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 #pragma unroll
   for (int v = 0; v < 2; v++) {
     const int d = w.d0 + (v < channels ? c + v : 0);
-    skip[v] = p.D != nullptr ? p.D[d] : 0.0f;
+    skip[v] = has_skip ? p.D[d] : 0.0f;
     bias[v] = p.dt_bias != nullptr ? p.dt_bias[d] : 0.0f;
   }
   float* const row = mine ? &sh.step[c][j] : &sh.step[0][0];               // step, input, y lie CB rows apart
@@ -322,12 +322,18 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
       const float4 f0 = *reinterpret_cast<const float4*>(row + stage * TILE + 2 * ARRAY);
       const float4 f1 = *reinterpret_cast<const float4*>(row + stage * TILE + 2 * ARRAY + R);
       float y[4][2] = {{f0.x, f1.x}, {f0.y, f1.y}, {f0.z, f1.z}, {f0.w, f1.w}};
+      if (has_skip) {                                // 0 times an infinite u would be NaN
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          float uf[2];
+          unpack(uo[k], uf);
+          y[k][0] = fmaf(skip[0], uf[0], y[k][0]);
+          y[k][1] = fmaf(skip[1], uf[1], y[k][1]);
+        }
+      }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        float uf[2], zf[2];
-        unpack(uo[k], uf);
-        y[k][0] = fmaf(skip[0], uf[0], y[k][0]);
-        y[k][1] = fmaf(skip[1], uf[1], y[k][1]);
+        float zf[2];
         if (has_z) {
           unpack(zo[k], zf);
           y[k][0] *= silu<T>(zf[0]);
@@ -744,7 +750,7 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
     if (p.zero_pad) *out = from_float<T>(0.0f);
     return;
   }
-  y = fmaf(skip, u, y);
+  y = fmaf(skip, fabsf(u) < INFINITY || p.D != nullptr ? u : 0.0f, y);       // 0 times an infinite u would be NaN
   if (p.z != nullptr) y *= silu<T>(z);
   *out = from_float<T>(y);
 }

@@ -413,3 +413,27 @@ def test_infinite_tokens_reach_no_state_that_does_not_exist(dtype, Ns, how):
         same(y[0, t:t + n, :2], want[:, :2], f"sequence {i}")
         same(final[i, :2], h[:2], f"state {i}")
         t += n
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_without_a_skip_an_infinite_token_is_not_multiplied_by_it(step):
+    """D left out adds nothing, also where u is infinite: the output is the infinite sum of C h (B, C positive)."""
+    import kda_b200
+    gen, T = generator(31), 40
+    a = make(gen, T, 64, 16, 1, BF, gate=False)
+    a.update(D=None, B=a["B"].abs() + 0.5, C=a["C"].abs() + 0.5)
+    a["u"][0, 21, 0] = float("inf")
+    a["u"][0, 33, 1] = -float("inf")
+    lens = [1] * T if step else [T]
+    init = torch.zeros(len(lens), 64, 16, device=DEV)
+    if step:
+        y, _ = kda_b200.selective_scan_step(**a, pool=init.clone())
+    else:
+        y, _ = kda_b200.selective_scan(**a)
+    t = 0
+    for n in lens:
+        s = at(a, slice(t, t + n))
+        want = scan64(s["u"][0], s["dt"][0], a["A"], s["B"][0], s["C"][0], None, None, a["dt_bias"], init[0], True)[0]
+        assert not bool(want.isnan().any())
+        same(y[0, t:t + n], want, f"token {t}")
+        t += n
