@@ -50,10 +50,11 @@ __device__ __forceinline__ float softplus(float x) {
   return fmaxf(x, 0.0f) + q * e;
 }
 
-// A in powers of two; finite, since -inf times a step of zero (behind the last token) would be NaN
+// A in powers of two; finite, since an infinite rate times a step of zero (that of the places behind the last token, too) would be NaN:
+// it keeps the state at such a step and forgets it at every other
 __device__ __forceinline__ float decay_rate(float a) {
   a *= LOG2E_F;
-  return a < -3.0e38f ? -3.0e38f : a;
+  return a < -3.0e38f ? -3.0e38f : (a > 3.0e38f ? 3.0e38f : a);
 }
 
 // two fp32 values an instruction
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
   const float skip = p.D != nullptr ? p.D[dc] : 0.0f;
   Values<S> a = values(p.A + at);
 #pragma unroll
-  for (int k = 0; k < S; k++) a.v[k] *= LOG2E_F;
+  for (int k = 0; k < S; k++) a.v[k] = decay_rate(a.v[k]);
   if (p.softplus) s = softplus(s);
   const float su = s * u;
   if (drop_repeats(p.seq, row0, slot)) {

@@ -437,3 +437,28 @@ def test_without_a_skip_an_infinite_token_is_not_multiplied_by_it(step):
         assert not bool(want.isnan().any())
         same(y[0, t:t + n], want, f"token {t}")
         t += n
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_rates_that_are_infinite(step, sign):
+    """A of -inf forgets the state at every positive step and keeps it at a step of zero, for prompts (of a length that ends inside a
+    tile) as for single tokens; +inf does so with negative steps.  In 64 bits: a rate of 1e30, since exp(-1e30 s) is 0 for every step
+    here but zero."""
+    import kda_b200
+    gen, T = generator(32), 41
+    a = make(gen, T, 48, 16, 1, F)
+    a.update(dt=-sign * (a["dt"].abs() + 0.01), dt_bias=None)
+    a["dt"][:, 10:14] = 0.0
+    a["dt"][:, -1] = 0.0
+    a["A"][:4] = sign * float("inf")
+    a["dt"][..., 4:] = a["dt"][..., 4:].abs()
+    finite = dict(a, A=a["A"].clamp(-1e30, 1e30))
+    lens = [1] * T if step else [T]
+    init = randn(gen, len(lens), 48, 16)
+    if step:
+        final = init.clone()
+        y, _ = kda_b200.selective_scan_step(**a, pool=final, dt_softplus=False)
+    else:
+        y, final = kda_b200.selective_scan(**a, initial_state=init, dt_softplus=False)
+    check(finite, init, lens, y, final, False)
