@@ -591,6 +591,18 @@ __global__ void __launch_bounds__(SCAN_THREADS, LOCAL ? 3 : 2) kda_selective_sca
 // Between the passes over pieces: from what each piece adds to the state (and exp(A sum of its steps), what it leaves of the
 // state in front) to the state that each starts from.  A thread follows one state value through its sequence.
 constexpr int JOIN_THREADS = 256;
+
+// 2^x h + add where the product does not tell: step by step a state of zero stays zero however far the exponential is beyond fp32's
+// range, an infinite one stays infinite however small it is, and a small state grows into the range.
+__device__ __forceinline__ float join_rare(float x, float h, float add) {
+  if (h != 0.0f && !isinf(h))
+    for (int i = 0; i < 3; i++) {                    // 2^300 lifts the least state out of the range
+      const float part = x > 100.0f ? 100.0f : x;
+      h *= exp2_fast(part);
+      x -= part;
+    }
+  return h + add;
+}
 __global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(const ScanParams p) {
   const long long rows = (long long)p.Dm * p.Ns;
   const int blocks = (int)((rows + JOIN_THREADS - 1) / JOIN_THREADS), seq = blockIdx.x / blocks;
@@ -609,18 +621,31 @@ __global__ void __launch_bounds__(JOIN_THREADS) kda_selective_scan_join_kernel(c
   float *state = p.ws_state + first * rows + at, *sums = p.ws_sum + (long long)first * p.Dm + d;
   constexpr int AHEAD = 8;
   for (int i0 = 0; i0 < n; i0 += AHEAD) {
-    float add[AHEAD], keep[AHEAD];
+    float add[AHEAD], keep[AHEAD], x[AHEAD];
+    const float h0 = h;
+    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) {
       const bool on = i0 + i + 1 < n;                // the last piece adds nothing here
       add[i] = on ? state[(i0 + i) * rows] : 0.0f;
-      keep[i] = on ? exp2_fast(a * sums[(long long)(i0 + i) * p.Dm]) : 0.0f;
+      x[i] = on ? a * sums[(long long)(i0 + i) * p.Dm] : 0.0f;
+      keep[i] = exp2_fast(x[i]);
+      most = fmaxf(most, x[i]);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
       if (i0 + i < n) {
         state[(i0 + i) * rows] = h;
         h = fmaf(keep[i], h, add[i]);
+      }
+    // finite exponentials and a finite state behind them: none of these steps was 0 times inf (inf and NaN stay, once in the state)
+    if (fabsf(h) < INFINITY && most <= 127.0f) continue;
+    h = h0;                                          // once more with care
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (i0 + i < n) {
+        state[(i0 + i) * rows] = h;
+        h = h == 0.0f || isinf(h) || x[i] > 127.0f ? join_rare(x[i], h, add[i]) : fmaf(keep[i], h, add[i]);
       }
   }
 }

@@ -462,3 +462,27 @@ def test_rates_that_are_infinite(step, sign):
     else:
         y, final = kda_b200.selective_scan(**a, initial_state=init, dt_softplus=False)
     check(finite, init, lens, y, final, False)
+
+
+def test_pieces_with_states_and_growth_that_fp32_products_do_not_hold():
+    """What a piece leaves of the state in front of it is one exponential of many steps: it may be beyond fp32's range where the state
+    is zero or small, and zero where the state is infinite.  Channels 0-1: a zero state that nothing enters, growing; 2-3: 1e-30 times
+    e^96 within the first piece; 4-5: an infinite state that decays (B, C positive); the rest as ever."""
+    import kda_b200
+    gen, T = generator(33), 3000
+    a = make(gen, T, 16, 16, 1, F, gate=False)
+    a.update(B=a["B"].abs() + 0.5, C=a["C"].abs() + 0.5, dt=a["dt"].abs() * 0.1, dt_bias=None)
+    a["A"][:4], a["A"][4:6] = 1.0, -1.0
+    a["u"][..., :4] = 0.0
+    a["dt"][..., :2] = 1.0
+    a["dt"][..., 2:4] = 0.0
+    a["dt"][:, :128, 2:4] = 0.75
+    a["dt"][..., 4:6] = 1.0
+    init = randn(gen, 1, 16, 16)
+    init[:, :2], init[:, 2:4], init[:, 4:6] = 0.0, 1e-30, float("inf")
+    y, final = kda_b200.selective_scan(**a, initial_state=init, dt_softplus=False)
+    assert bool((final[0, :2] == 0).all()) and bool((y[..., :2] == 0).all())
+    assert bool((final[0, 4:6] == float("inf")).all()) and bool((y[..., 4:6] == float("inf")).all())
+    keep = [2, 3, *range(6, 16)]
+    part = {n: t[..., keep] if n in ("u", "dt") else t[keep] if n in ("A", "D") else t for n, t in a.items()}
+    check(part, init[:, keep], [T], y[..., keep], final[:, keep], False)
