@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _cabi, _err, _reject_aliasing
-from .serving import _call, _pool_rows, _ptr, _Ready
+from .serving import _call, _pool_rows, _ptr, _Ready, _status
 
 
 def _index(t, name, dev=None):
@@ -49,12 +49,9 @@ def _args(pools, used, status, dev, slots, written, read):
         if not (used.dtype == torch.bool and used.is_contiguous()):
             raise _err(f"used must be a contiguous bool tensor [{slots}], got {used.dtype} {list(used.shape)}")
         a.used = used.data_ptr()
-    if status is not None:
-        if not (torch.is_tensor(status) and status.dtype == torch.int32 and status.device == dev and status.numel() >= 1):
-            raise _err(f"status must be an int32 tensor on {dev}")
-        a.status = status.data_ptr()
     a.slots, a.n_pools = slots, len(pools)
-    _reject_aliasing(_extents(a) + [("used", used)] + written, read)
+    _reject_aliasing(_extents(a) + [("used", used), _status(dev, status)] + written, read)
+    a.status = _ptr(status)
     return a, dev
 
 
@@ -107,7 +104,7 @@ def _copy(src, dst, status, *pools):
     ws = _workspace(a, src.numel(), dev)
     a.src, a.src_is64, a.dst, a.dst_is64 = _ptr(src), src.dtype == torch.int64, _ptr(dst), dst.dtype == torch.int64
     return _ready("kda_pool_copy_launch" if src.numel() else None, dev, a, 3, {0: ["src"], 1: ["dst"], 2: ["status"]}, [(ws, ["workspace"])], (),
-                  len(pools), [])
+                  len(pools), [2])
 
 
 def pool_copy(pools, src, dst, *, status=None):
@@ -125,7 +122,7 @@ def _fork(used, parents, status, *pools):
     ws = _workspace(a, parents.numel(), dev)
     a.src, a.src_is64, a.slots_out = _ptr(parents), parents.dtype == torch.int64, _ptr(slots)
     return _ready("kda_pool_fork_launch" if parents.numel() else None, dev, a, 3, {0: ["used"], 1: ["src"], 2: ["status"]},
-                  [(slots, ["slots_out"]), (ws, ["workspace"])], (-1,), len(pools), [0])
+                  [(slots, ["slots_out"]), (ws, ["workspace"])], (-1,), len(pools), [0, 2])
 
 
 def pool_fork(pools, used, parents, *, status=None):
@@ -140,7 +137,7 @@ def _free(used, slots, status):
     _index(slots, "slots", dev)
     a, dev = _args([], used, status, dev, P, [], [("slots", slots)])
     a.n, a.src, a.src_is64 = slots.numel(), _ptr(slots), slots.dtype == torch.int64
-    return _ready("kda_pool_free_launch" if slots.numel() else None, dev, a, 3, {0: ["used"], 1: ["src"], 2: ["status"]}, [], (), 0, [0])
+    return _ready("kda_pool_free_launch" if slots.numel() else None, dev, a, 3, {0: ["used"], 1: ["src"], 2: ["status"]}, [], (), 0, [0, 2])
 
 
 def pool_free(used, slots, *, status=None):
@@ -162,7 +159,7 @@ def _compact(*tensors):
     ws = _workspace(a, 0, dev)
     given = {0: ["used"], 1: ["status"], **{2 + i: [f"tables[{i}]"] for i in range(len(tables))}}
     return _ready("kda_pool_compact_launch", dev, a, 2 + len(tables), given, [(remap, ["remap"]), (ws, ["workspace"])], (-1,), len(pools),
-                  [0, *range(2, 2 + len(tables))])
+                  [0, 1, *range(2, 2 + len(tables))])
 
 
 def pool_compact(pools, used, tables=(), *, status=None):

@@ -14,8 +14,8 @@ None: zeros), is left alone, and a new final state is returned.  Steps: row i is
 
 Tables are read on the device where they lie; every call enqueues its launches on the current stream of the tensors' device, reads
 nothing on the host and can be captured in a CUDA graph.  Rows of the output that no sequence owns (behind the last sequence,
-padding) are zeros, or stay as they are in a caller's `out`.  `status`: an int32 CUDA tensor whose first entry collects (ORs) the
-bits 1 = rejected cu_seqlens (all sequences taken as empty, output rows zero) and 2 = slot out of range or named before (that
+padding) are zeros, or stay as they are in a caller's `out`.  `status`: an int32 CUDA tensor, apart from every other operand, whose
+first entry collects (ORs) the bits 1 = rejected cu_seqlens (all sequences taken as empty, output rows zero) and 2 = slot out of range or named before (that
 sequence starts from zeros and its state is not stored)."""
 from __future__ import annotations
 
@@ -230,10 +230,16 @@ def _pool_rows(t, name, inner):
     return t.stride(0) if t.shape[0] > 1 else n
 
 
-def _sequences(dev, T, N, cu, slots, n_slots, status, zero_rest):
-    if status is not None and not (torch.is_tensor(status) and status.dtype == torch.int32 and status.is_cuda and status.numel() >= 1
-                                   and status.device == dev):
+def _status(dev, status):
+    """Checks `status`; returns the bytes of it that a call writes, named."""
+    if status is None:
+        return "status", None
+    if not (torch.is_tensor(status) and status.dtype == torch.int32 and status.device == dev and status.numel() >= 1):
         raise _err(f"status must be an int32 tensor on {dev}")
+    return "status", (status.data_ptr(), status.data_ptr() + 4)
+
+
+def _sequences(T, N, cu, slots, n_slots, status, zero_rest):
     return _cabi.KdaSequences(_ptr(cu), _ptr(slots), n_slots, T, _ptr(status), int(cu is not None and cu.dtype == torch.int64),
                               int(slots is not None and slots.dtype == torch.int64), N, zero_rest)
 
@@ -317,18 +323,18 @@ def _conv(x, weight, bias, state, cu_seqlens, slots, out, status, activation, st
     x, ldx = _rows(x)
     y = _out(out, x)
     in_place = src is dst
-    if in_place or out is not None:
-        _reject_aliasing([("out", y), ("the pool", dst)], [("x", x), ("weight", weight), ("bias", bias), ("cu_seqlens", cu),
+    if in_place or out is not None or status is not None:
+        _reject_aliasing([("out", y), ("the pool", dst), _status(dev, status)], [("x", x), ("weight", weight), ("bias", bias), ("cu_seqlens", cu),
                          ("ssm_state_indices", slots), ("initial_state", None if in_place else src)])
     args = _cabi.KdaConvArgs(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(src), _ptr(dst), ldx, _rows(y)[1], src_stride, dst_stride,
-                             _sequences(dev, T, N, cu, slots, n_slots, status, int(out is None)), channels, W, TYPES[x.dtype],
+                             _sequences(T, N, cu, slots, n_slots, status, int(out is None)), channels, W, TYPES[x.dtype],
                              TYPES[weight.dtype], int(activation is not None))
     given = {0: ["x"], 1: ["weight"], 2: ["bias"], 4: ["seq.cu_seqlens"], 5: ["seq.slots"], 6: ["out"], 7: ["seq.status"]}
     given[3] = ["src", "dst"] if in_place else ["src"]
     fresh = ([(y, ["out"])] if out is None else []) + ([] if in_place else [(dst, ["dst"])])
     result = (6 if out is not None else -1, 3 if in_place else -len(fresh))
     name = None if step and not T else "kda_short_conv_step_launch" if step else "kda_short_conv_launch"
-    return _Ready(name, dev, args, given, fresh, result, [6] + [3] * in_place, keep=(x, weight, bias, src, cu, slots))
+    return _Ready(name, dev, args, given, fresh, result, [6, 7] + [3] * in_place, keep=(x, weight, bias, src, cu, slots))
 
 
 def short_conv(x, weight, bias=None, initial_state=None, cu_seqlens=None, *, activation="silu", ssm_state_indices=None, out=None,
@@ -386,14 +392,14 @@ def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, slots, out, stat
         z, ldz = _rows(z)
     y = _out(out, u)
     in_place = src is dst
-    if in_place or out is not None:
-        _reject_aliasing([("out", y), ("the pool", dst)], [("u", u), ("dt", dt), ("A", A), ("B", B), ("C", C_), ("D", skip), ("z", z),
+    if in_place or out is not None or status is not None:
+        _reject_aliasing([("out", y), ("the pool", dst), _status(dev, status)], [("u", u), ("dt", dt), ("A", A), ("B", B), ("C", C_), ("D", skip), ("z", z),
                          ("dt_bias", dt_bias), ("cu_seqlens", cu), ("ssm_state_indices", slots), ("initial_state", None if in_place else src)])
     ws_bytes = 0 if step else _cabi.lib().kda_selective_scan_workspace_bytes(T, N, channels, size)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     args = _cabi.KdaScanArgs(_ptr(u), _ptr(dt), _ptr(B), _ptr(C_), _ptr(z), _ptr(y), _ptr(A), _ptr(skip), _ptr(dt_bias), _ptr(src), _ptr(dst),
                              ldu, lddt, ldb, ldc, ldz, _rows(y)[1], src_stride, dst_stride,
-                             _sequences(dev, T, N, cu, slots, n_slots, status, int(out is None)), channels, size, groups, TYPES[u.dtype],
+                             _sequences(T, N, cu, slots, n_slots, status, int(out is None)), channels, size, groups, TYPES[u.dtype],
                              int(bool(softplus)), _ptr(ws), ws_bytes)
     given = {i: [f] for i, f in enumerate(("u", "dt", "A", "B", "C", "D", "z", "dt_bias"))}
     given.update({9: ["seq.cu_seqlens"], 10: ["seq.slots"], 11: ["out"], 12: ["seq.status"]})
@@ -403,7 +409,7 @@ def _scan(u, dt, A, B, C_, skip, z, dt_bias, state, cu_seqlens, slots, out, stat
     if ws is not None:
         fresh.append((ws, ["workspace"]))
     name = None if step and not T else "kda_selective_scan_step_launch" if step else "kda_selective_scan_launch"
-    return _Ready(name, dev, args, given, fresh, result, [11] + [8] * in_place, keep=(u, dt, A, B, C_, skip, z, dt_bias, src, cu, slots))
+    return _Ready(name, dev, args, given, fresh, result, [11, 12] + [8] * in_place, keep=(u, dt, A, B, C_, skip, z, dt_bias, src, cu, slots))
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=None, cu_seqlens=None, *, dt_softplus=True,
@@ -448,14 +454,14 @@ def _kda(q, k, v, g, beta, A_log, dt_bias, pool, slots, out, status, scale, raw)
     slots = _step_slots(dev, slots, N, pool)
     (q, ldq), (k, ldk), (v, ldv), (g, ldg), (beta, ldbeta) = map(_rows, (q, k, v, g, beta))
     y = _out(out, q)
-    _reject_aliasing([("out", y), ("the pool", pool)], [("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("A_log", A_log),
+    _reject_aliasing([("out", y), ("the pool", pool), _status(dev, status)], [("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("A_log", A_log),
                      ("dt_bias", dt_bias), ("ssm_state_indices", slots)])
     args = _cabi.KdaStepArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(y), _ptr(A_log), _ptr(dt_bias), _ptr(pool), ldq, ldk, ldv,
-                             ldg, ldbeta, _rows(y)[1], stride, _sequences(dev, N, N, None, slots, pool.shape[0], status, int(out is None)),
+                             ldg, ldbeta, _rows(y)[1], stride, _sequences(N, N, None, slots, pool.shape[0], status, int(out is None)),
                              float(scale), LOWER_BOUND, _cabi.FRONTEND_RAW if raw else _cabi.FRONTEND_PLAIN, H)
     given = {i: [f] for i, f in enumerate(("q", "k", "v", "g", "beta", "A_log", "dt_bias", "pool", "seq.slots", "out", "seq.status"))}
     fresh = [(y, ["out"])] if out is None else []
-    return _Ready("kda_step_launch" if N else None, dev, args, given, fresh, (9 if out is not None else -1, 7), [9, 7], [7],
+    return _Ready("kda_step_launch" if N else None, dev, args, given, fresh, (9 if out is not None else -1, 7), [9, 10, 7], [7],
                   keep=(q, k, v, g, beta, A_log, dt_bias, slots))
 
 

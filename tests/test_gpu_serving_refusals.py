@@ -113,3 +113,26 @@ def test_written_buffers_that_overlap_are_refused():
     h = zeros(4, 64, 16)
     with pytest.raises(ValueError, match="overlap"):
         kda_b200.selective_scan_step(zeros(1, 2, 64), zeros(1, 2, 64), h[0], zeros(1, 2, 1, 16), zeros(1, 2, 1, 16), None, None, None, h)
+
+
+def test_status_that_overlaps_an_operand_is_refused():
+    """The kernels OR bits into it while other blocks read the tables.  Nothing is reported in these calls, so that they only write
+    where they may."""
+    import kda_b200
+    cu, slots = ints(0, 5, 8), ints(0, 1)
+    for call, operand in ((conv, dict(cu_seqlens=cu)), (conv, dict(ssm_state_indices=slots)), (conv_step, dict(ssm_state_indices=slots)),
+                          (scan, dict(cu_seqlens=cu)), (scan_step, dict(ssm_state_indices=slots)), (step, dict(ssm_state_indices=slots))):
+        for _ in range(2):
+            call(**operand, status=ints(0))
+            with pytest.raises(ValueError, match="overlap"):
+                call(**operand, status=next(iter(operand.values()))[:1])
+    src, used, slots = ints(0), zeros(4, dtype=torch.bool), ints(-1)
+    for call, operand in ((lambda s: copy(src=src, status=s), src), (lambda s: fork(used=used, parents=slots, status=s), slots),
+                          (lambda s: kda_b200.pool_free(used, slots, status=s), slots), (lambda s: compact(tables=[slots], status=s), slots)):
+        for _ in range(2):
+            call(ints(0))
+            with pytest.raises(ValueError, match="overlap"):
+                call(operand)
+    with pytest.raises(ValueError, match="overlap"):
+        kda_b200.short_conv(zeros(1, 8, 64), zeros(64, 4), None, None, cu, status=cu[1:])
+    torch.cuda.synchronize()
