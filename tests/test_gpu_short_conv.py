@@ -240,3 +240,22 @@ def test_offsets_behind_32_bits():
     y, _ = kda_b200.short_conv_step(x[:, -1:].clone(), w, None, pool, torch.tensor([pool.shape[0] - 1], device=DEV))
     assert bool(torch.isfinite(y).all())
     assert torch.equal(pool[-1, -1], pool.view(-1, C)[-1])
+
+
+def test_single_tokens_in_slots_behind_32_bits():
+    """Slots further than 2^31 elements from the base: values, new histories, and every other slot as it was."""
+    import kda_b200
+    gen, C, W = generator(12), 8192, 4
+    P = 2 ** 31 // ((W - 1) * C) + 1000
+    pool = torch.full((P, W - 1, C), 5.0, dtype=BF, device=DEV)
+    ids = [P - 1, 3, 2 ** 31 // ((W - 1) * C) + 1, 0]
+    at = torch.tensor(ids, device=DEV)
+    x, w = randn(gen, 1, 4, C, dtype=BF), randn(gen, C, W, dtype=BF)
+    pool[at] = randn(gen, 4, W - 1, C, dtype=BF)
+    before = pool[at].clone()
+    y, got = kda_b200.short_conv_step(x, w, None, pool, at)
+    assert got is pool
+    check(x, w, None, before, [1] * 4, y, pool[at])
+    assert not torch.equal(pool[at], before)
+    pool[at] = 5.0
+    assert all(bool((part == 5.0).all()) for part in pool.split(4096))
