@@ -692,7 +692,8 @@ __global__ void __launch_bounds__(STEP_LANES) kda_selective_scan_step_kernel(con
 #pragma unroll
   for (int r = 0; r < ROWS; r++)
     if (slot[r] >= 0) h[r] = values(p.src + slot[r] * p.src_stride + at);
-  // what a row of padding brings is worked on like the rest, and dropped
+  // what a row of padding brings is worked on like the rest, and dropped: tokens that wait for the slots cost 43 us for the 256 rows
+  // above instead of 37
   Pack<T, S> rb[ROWS], rc[ROWS];
   const T* B = reinterpret_cast<const T*>(p.B) + row0 * p.ldb + (long long)group * p.Ns + n;
   const T* C = reinterpret_cast<const T*>(p.C) + row0 * p.ldc + (long long)group * p.Ns + n;

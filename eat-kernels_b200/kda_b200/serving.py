@@ -10,13 +10,13 @@
 Tokens are packed as in the prefill, [1, T, ...].  Prompts: sequences by `cu_seqlens` (None: one); with `ssm_state_indices` the
 state buffer is a pool of slots that is updated in place and returned, without it `initial_state` has one entry a sequence (or is
 None: zeros), is left alone, and a new final state is returned.  Steps: row i is the next token of a sequence of its own, in slot
-`ssm_state_indices[i]` (None: slot i); a negative entry marks a row of padding, of which nothing is read or stored.
+`ssm_state_indices[i]` (None: slot i); a negative entry marks a row of padding, of which nothing is used or stored.
 
 Tables are read on the device where they lie; every call enqueues its launches on the current stream of the tensors' device, reads
 nothing on the host and can be captured in a CUDA graph.  Rows of the output that no sequence owns (behind the last sequence,
 padding) are zeros, or stay as they are in a caller's `out`.  `status`: an int32 CUDA tensor, apart from every other operand, whose
-first entry collects (ORs) the bits 1 = rejected cu_seqlens (all sequences taken as empty, output rows zero) and 2 = slot out of range or named before (that
-sequence starts from zeros and its state is not stored)."""
+first entry collects (ORs) the bits 1 = rejected cu_seqlens (all sequences taken as empty, output rows zero) and 2 = slot out of
+range or named before (that sequence starts from zeros and its state is not stored)."""
 from __future__ import annotations
 
 import ctypes as C

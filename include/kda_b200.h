@@ -248,7 +248,8 @@ enum { KDA_STATUS_POOL_FULL = 32 };   /* kda_pool_fork: no slot was left for som
 typedef struct KdaSequences {
   const void* cu_seqlens;  /* device int32/int64 [N+1], or NULL: one sequence [0, T].  Unused in a step: row i is sequence i */
   const void* slots;       /* device int32/int64 [N], or NULL: sequence i uses slot i.  In a step a negative entry stands for
-                              a row of padding: nothing of it is read, computed or stored */
+                              a row of padding: nothing of it is used or stored, and no state read for it (its
+                              tokens must lie in memory like any other row's: the scan's step loads them) */
   int64_t n_slots;         /* slots of the state buffers (range check; >= N without a table, at most 2^31 - 1) */
   int64_t T;               /* token rows; at most 2^31 - 1 */
   int32_t* status;         /* device int32, or NULL */

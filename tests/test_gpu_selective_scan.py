@@ -486,3 +486,24 @@ def test_pieces_with_states_and_growth_that_fp32_products_do_not_hold():
     keep = [2, 3, *range(6, 16)]
     part = {n: t[..., keep] if n in ("u", "dt") else t[keep] if n in ("A", "D") else t for n, t in a.items()}
     check(part, init[:, keep], [T], y[..., keep], final[:, keep], False)
+
+
+@pytest.mark.parametrize("dtype,Dm,Ns", [(BF, 256, 16), (F, 72, 13), (HF, 40, 64), (F, 24, 128)])
+@pytest.mark.parametrize("fill", ["nan", "inf", "-inf"])
+def test_nothing_of_a_row_of_padding_is_used(dtype, Dm, Ns, fill):
+    """Four rows of a step share a block: whatever lies in the rows of padding among them, in every tensor, the others, the pool and a
+    caller's output rows of padding stay bit for bit."""
+    import kda_b200
+    gen, N = generator(25), 13
+    a, pool = make(gen, N, Dm, Ns, 1, dtype), randn(gen, 11, Dm, Ns)
+    dead = [1, 2, 3, 6, 12]
+    slots = torch.tensor([5, -1, -9, -1, 0, 10, -2, 3, 4, 1, 2, 8, -1], device=DEV)
+    outs, pools = [], []
+    for value in (0.0, float(fill)):
+        for n in ("u", "dt", "B", "C", "z"):
+            a[n][:, dead] = value
+        pools.append(pool.clone())
+        outs.append(torch.full((1, N, Dm), 3.0, dtype=dtype, device=DEV))
+        kda_b200.selective_scan_step(**a, pool=pools[-1], ssm_state_indices=slots, out=outs[-1])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(pools[0], pools[1])
+    assert bool((outs[1][0, dead] == 3.0).all()) and bool(torch.isfinite(outs[1]).all()) and torch.equal(pools[1][[6, 7, 9]], pool[[6, 7, 9]])
