@@ -9,6 +9,10 @@ namespace {
 
 constexpr int CONV_THREADS = 128;
 constexpr int GROUP = 4;                 // tokens whose rows are asked for together
+// Blocks an SM that the prompt kernel's registers leave room for: two groups of rows in 16 bits fit 72 registers, in 32 bits 96 (W = 4, 3, 2
+// on the batch below: 480, 454 and 438 us; with 72 registers, spilling 296 bytes, 565, 460 and 546; 80: 467, 524, 432; 128: 502, 494, 438).
+template <typename T>
+constexpr int BLOCKS_AN_SM = sizeof(T) == 4 ? 5 : 7;
 
 // N consecutive values, in 8-byte accesses where they start on 8 bytes
 template <typename T, int N>
@@ -50,9 +54,9 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (
 // VEC channels a thread, a tile of tokens a block.  A sequence's first W - 1 tokens belong to the tile that holds its start,
 // even where they reach into the next tile: only that tile reads the slot's history, and it writes the new one after that,
 // so the pool is updated in place by one launch.  Bound by memory: the window slides in registers, a tile re-reads W - 1
-// rows of the tile before it (out of L2); 55 846 tokens of 6144 channels, W = 4: 259 us, 5.3 TB/s.
+// rows of the tile before it (out of L2); 55 846 tokens of 6144 channels, W = 4: 258-261 us in bf16, 5.3 TB/s, 480 us in fp32, 5.7 TB/s.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(CONV_THREADS, 7) kda_short_conv_kernel(const ConvParams p) {
+__global__ void __launch_bounds__(CONV_THREADS, BLOCKS_AN_SM<T>) kda_short_conv_kernel(const ConvParams p) {
   constexpr int HW = W - 1;
   using P = Pack<T, VEC>;
   const int cblocks = (p.C / VEC + CONV_THREADS - 1) / CONV_THREADS;
@@ -91,8 +95,8 @@ __global__ void __launch_bounds__(CONV_THREADS, 7) kda_short_conv_kernel(const C
     }
     *reinterpret_cast<P*>(out + t * p.ldo) = pack<T, VEC>(y);
   };
-  // tokens in groups: a group's rows are on their way while the group in front is worked on (two groups of four: 259 us on the
-  // batch above, one of eight at a time 272, two of eight 271, two of two 300)
+  // tokens in groups: a group's rows are on their way while the group in front is worked on (two groups of four: 258 us on the
+  // batch above in bf16, 252 in fp16, one of eight at a time 270 and 252, two of eight 271, two of two 300)
   auto run = [&](long long from, long long to, float (&win)[HW][VEC]) {
     if (from + GROUP <= to) {
       P rows[GROUP], next[GROUP];

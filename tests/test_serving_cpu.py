@@ -177,3 +177,16 @@ def test_host_tensors_are_refused():
                  lambda: kda_b200.pool_compact([pool], torch.zeros(4, dtype=torch.bool))):
         with pytest.raises(ValueError, match="KDA kernel"):
             call()
+
+
+def test_registers_of_the_convolution_fit():
+    """No type or width spills more than a few registers in the prompt kernel (one cap for all types left 296 bytes in fp32)."""
+    import re
+    import subprocess
+
+    from kda_b200 import _build
+    r = subprocess.run([_build.nvcc_path(), *_build.NVCC_FLAGS, "-Xptxas", "-v", "-cubin", "-o", "/dev/null", str(_build.CSRC / "kda_conv.cu")],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    spills = re.findall(r"Function properties for \S*kda_short_conv_kernel\S*\n.*?(\d+) bytes spill loads", r.stderr)
+    assert len(spills) == 18 and max(map(int, spills)) <= 64, spills
