@@ -12,9 +12,9 @@
 //   * a lane has two channels, so that B and C are read once for both, and S state values of each; L lanes share a channel.
 //     Sums over the lanes are taken for four tokens at once, each step of an exchange halving the tokens that a lane holds.
 // Measured (16 state values): 8 ragged prompts, 10 245 tokens of 4096 channels, in bf16 270 us, the exponentials' unit busy 65 % of
-// it (one channel a lane: 308 us, the shared-memory pipe at 84 %), in fp32 300 us; one prompt of 32 768 tokens on 512 channels 208 us
+// it (one channel a lane: 308 us, the shared-memory pipe at 84 %), in fp32 299 us; one prompt of 32 768 tokens on 512 channels 207 us
 // in pieces (uncut 1725 us).  Rows that do not all start on 16 bytes are read value by value: the ragged prompts with 4095 channels
-// 331 us, with 4 and 13 state values (B and C rows of 8 and 26 bytes, all tensors on that path) 333 and 340 us.
+// 330 us, with 4 and 13 state values (B and C rows of 8 and 26 bytes, all tensors on that path) 332 and 336 us.
 #include "kda_serving.cuh"
 
 namespace kda {
@@ -440,9 +440,8 @@ __device__ __forceinline__ void help(const ScanParams& p, const Work& w, ScanSha
 // four; tokens behind the last one leave the state as it is.
 // LOCAL: the state alone, and the sum of the steps.
 // PADDED: there are only `states` of the L S state values.  The places behind them hold B = C = 0, which an infinite step or s u turns
-// into NaN (0 times inf): the sums take them as zeros, and nothing else reads them (the ragged prompts with 13 and, on 2048 channels,
-// 24 values: 340 and 283 us, without the care 335 and 279).  The
-// lower half of a lane's places always has values.
+// into NaN (0 times inf): the sums take them as zeros, and nothing else reads them.  The lower half of a lane's places always has values.
+// The ragged prompts with 13 values, and with 24 on 2048 channels: 336 and 286 us, without the care 335 and 279.
 template <int L, int S, bool LOCAL, bool PADDED>
 __device__ __forceinline__ void scan(const Work& w, ScanShared<L, S>& sh, int tid, int states, const float (&a)[CH][S], float (&h)[CH][S],
                                      float (&sum)[CH]) {
@@ -575,8 +574,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, LOCAL ? 3 : 2) kda_selective_sca
       h[m][k] = !LOCAL && on && from != nullptr ? from[at + k * L] : 0.0f;
     }
   }
-  if (!LOCAL && p.Ns < L * S) scan<L, S, LOCAL, !LOCAL>(w, sh, tid, p.Ns, a, h, sum);
-  else scan<L, S, LOCAL, false>(w, sh, tid, p.Ns, a, h, sum);
+  if (LOCAL || p.Ns == L * S) scan<L, S, LOCAL, false>(w, sh, tid, p.Ns, a, h, sum);
+  else scan<L, S, LOCAL, !LOCAL>(w, sh, tid, p.Ns, a, h, sum);
   float* to = LOCAL ? own : (w.piece + 1 == w.pieces && p.dst != nullptr && slot >= 0 ? p.dst + slot * p.dst_stride : nullptr);
   if (to == nullptr) return;
 #pragma unroll
@@ -863,7 +862,7 @@ cudaError_t launch_step_type(const ScanParams& p, cudaStream_t stream) {
 // state, the states are joined, a second pass computes the outputs.  That is about 1.6 times the work, for two rounds of blocks
 // that fill the card (two an SM): 0 = no cut, else the tokens of a piece.  The lengths lie on the device, so the rule goes by the
 // number of sequences, and by all channels together: groups that end inside a block launch more blocks than it counts, so that
-// small groups get shorter pieces than two rounds.  32 768 tokens on 512 channels: uncut 1725 us, two rounds of pieces 208 us, four 218 us,
+// small groups get shorter pieces than two rounds.  32 768 tokens on 512 channels: uncut 1725 us, two rounds of pieces 207 us, four 218 us,
 // eight 241 us; 8192 tokens on 4096 channels (64 blocks uncut, 160 cycles a token: some 690 us) 379 us.
 long long sscan_piece(long long T, int N, int Dm, int Ns) {
   const int lanes = Ns <= 16 ? 4 : (Ns <= 32 ? 8 : (Ns <= 64 ? 16 : 32));
