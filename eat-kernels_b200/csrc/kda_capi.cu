@@ -418,11 +418,14 @@ size_t kda_abi_struct_bytes(int which) {
     case 3: return sizeof(KdaScanArgs);
     case 4: return sizeof(KdaStepArgs);
     case 5: return sizeof(KdaPoolArgs);
+    case 6: return sizeof(KdaGatedScanArgs);
+    case 7: return sizeof(KdaGatedScanGradArgs);
+    case 8: return sizeof(KdaGroupNormArgs);
     default: return 0;
   }
 }
 
-const char* kda_version(void) { return "kda_b200 5 sm_100a"; }
+const char* kda_version(void) { return "kda_b200 6 sm_100a"; }
 
 int kda_prefill_plan_counts(const KdaPrefillArgs* a, int32_t* counts, void* stream_) {
   if (a == nullptr || counts == nullptr || a->workspace == nullptr || a->H <= 0 || a->N < 1) return KDA_ERR_ARG;
@@ -447,7 +450,8 @@ int kda_debug_configure(int64_t wait_limit_us, int32_t flags, void* prof_counter
 
 }  // extern "C"
 
-// ---- the operators around the prefill (kernels: kda_conv.cu, kda_sscan.cu, kda_step.cu, kda_pool.cu)
+// ---- the operators around the prefill (kernels: kda_conv.cu, kda_sscan.cu, kda_step.cu, kda_gscan.cu, kda_gscan_grad.cu, kda_gnorm.cu,
+// kda_pool.cu)
 namespace {
 
 bool known_type(int type) { return type >= KDA_TYPE_BF16 && type <= KDA_TYPE_FP32; }
@@ -532,6 +536,60 @@ int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
   return launched(step ? kda::launch_sscan_step(p, a->type, s) : kda::launch_sscan(p, a->type, s));
 }
 
+static_assert(KDA_GATED_SCAN_TILE == kda::GATED_SCAN_TILE && KDA_GROUP_NORM_MAX_WIDTH == kda::GROUP_NORM_MAX_WIDTH, "limits as documented");
+
+int gated_scan_launch(const KdaGatedScanArgs* a, bool step, void* stream) {
+  if (a == nullptr || a->C < 1 || !known_type(a->type)) return KDA_ERR_ARG;
+  const int rc = check_sequences(a->seq, step);
+  if (rc != KDA_OK) return rc;
+  if (!whole(a->type, a->x, a->r, a->i, a->out)) return KDA_ERR_ARG;
+  if (!whole(KDA_TYPE_FP32, a->rate, a->r_bias, a->i_bias, a->src, a->dst, a->tiles)) return KDA_ERR_ARG;
+  if (a->seq.T > 0) {
+    if (a->i_bias && !a->i) return KDA_ERR_ARG;
+    if (!a->x || !a->r || !a->out || a->ldx < a->C || a->ldr < a->C || (a->i && a->ldi < a->C) || a->ldo < a->C) return KDA_ERR_ARG;
+  }
+  if ((a->src && a->src_slot_stride < a->C) || (a->dst && a->dst_slot_stride < a->C)) return KDA_ERR_ARG;
+  if (step && a->seq.T > 0 && (!a->dst || a->src != a->dst || a->src_slot_stride != a->dst_slot_stride)) return KDA_ERR_ARG;
+  kda::GatedScanParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x; p.r = a->r; p.i = a->seq.T > 0 ? a->i : nullptr; p.out = a->out;
+  p.rate = a->rate; p.r_bias = a->r_bias; p.i_bias = a->i_bias; p.src = a->src; p.dst = a->dst; p.tiles = a->tiles;
+  p.seq = seq_table(a->seq);
+  p.ldx = a->ldx; p.ldr = a->ldr; p.ldi = a->i ? a->ldi : 0; p.ldo = a->ldo; p.src_stride = a->src_slot_stride; p.dst_stride = a->dst_slot_stride;
+  p.rate_scale = a->rate_scale; p.C = a->C; p.zero_pad = a->seq.zero_rest != 0;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return launched(step ? kda::launch_gated_scan_step(p, a->type, s) : kda::launch_gated_scan(p, a->type, s));
+}
+
+int group_norm_launch(const KdaGroupNormArgs* a, bool grad, void* stream) {
+  if (a == nullptr || a->T < 0 || a->G < 1 || a->D < 1 || !known_type(a->type) || a->act < KDA_ACT_NONE || a->act > KDA_ACT_SIGMOID) return KDA_ERR_ARG;
+  if (a->D > KDA_GROUP_NORM_MAX_WIDTH || a->T > 0x7fffffffLL || (int64_t)a->G * a->D > 0x7fffffffLL / 2) return KDA_ERR_LIMIT;
+  const int64_t width = (int64_t)a->G * a->D;
+  if (a->T > 0) {
+    if (!a->x || !a->out || a->ldx < width || a->ldo < width || (a->z && a->ldz < width)) return KDA_ERR_ARG;
+    if (grad && (!a->dy || a->lddy < width || (a->z && (!a->dz || a->lddz < width)))) return KDA_ERR_ARG;
+  }
+  if (!whole(a->type, a->x, a->z, a->out) || !whole(KDA_TYPE_FP32, a->weight, a->bias)) return KDA_ERR_ARG;
+  kda::GroupNormParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x; p.z = a->z; p.out = a->out; p.weight = a->weight; p.bias = a->bias;
+  p.T = a->T; p.ldx = a->ldx; p.ldz = a->z ? a->ldz : 0; p.ldo = a->ldo;
+  p.eps = a->eps; p.G = a->G; p.D = a->D; p.act = a->act; p.center = a->center != 0; p.shared = a->shared != 0;
+  if (grad) {
+    if (!whole(a->type, a->dy, a->dz) || !whole(KDA_TYPE_FP32, a->dweight, a->dbias)) return KDA_ERR_ARG;
+    p.dy = a->dy; p.lddy = a->lddy;
+    if (a->z) { p.dz = a->dz; p.lddz = a->lddz; }
+    p.dweight = a->dweight; p.dbias = a->dbias;
+    if (a->dweight || a->dbias) {
+      if (!a->workspace || !aligned16(a->workspace)) return KDA_ERR_ARG;
+      if (a->workspace_bytes < kda_group_norm_workspace_bytes(a->T, a->G, a->D, a->type, a->shared)) return KDA_ERR_WORKSPACE;
+      p.partial = reinterpret_cast<float*>(a->workspace);
+    }
+  }
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return launched(grad ? kda::launch_group_norm_grad(p, a->type, s) : kda::launch_group_norm(p, a->type, s));
+}
+
 // The parts of the argument block that a call uses, checked; fills the kernels' parameters.
 int pool_params(const KdaPoolArgs* a, bool used, bool src, bool copies, kda::PoolPlan& p, kda::PoolRows& r) {
   if (a == nullptr || a->slots < 1 || a->n < 0) return KDA_ERR_ARG;
@@ -603,6 +661,41 @@ int kda_step_launch(const KdaStepArgs* a, void* stream) {
   p.scale = a->scale; p.lower_bound = a->lower_bound; p.H = a->H; p.raw = raw; p.zero_pad = a->seq.zero_rest != 0;
   return launched(kda::launch_kda_step(p, reinterpret_cast<cudaStream_t>(stream)));
 }
+
+int kda_gated_scan_launch(const KdaGatedScanArgs* a, void* stream) { return gated_scan_launch(a, false, stream); }
+int kda_gated_scan_step_launch(const KdaGatedScanArgs* a, void* stream) { return gated_scan_launch(a, true, stream); }
+
+int kda_gated_scan_grad_launch(const KdaGatedScanGradArgs* a, void* stream) {
+  if (a == nullptr || a->C < 1 || !known_type(a->type) || a->seq.slots) return KDA_ERR_ARG;
+  KdaSequences seq = a->seq;
+  seq.n_slots = seq.N;                               // one state a sequence
+  const int rc = check_sequences(seq, false);
+  if (rc != KDA_OK) return rc;
+  if (!whole(a->type, a->x, a->r, a->i, a->dy, a->dx, a->dr, a->di)) return KDA_ERR_ARG;
+  if (!whole(KDA_TYPE_FP32, a->rate, a->r_bias, a->i_bias, a->tiles, a->src, a->dfinal, a->dsrc, a->drate, a->dr_bias, a->di_bias)) return KDA_ERR_ARG;
+  if (a->drate && !a->rate) return KDA_ERR_ARG;
+  if (seq.T > 0) {
+    if ((a->i_bias || a->di || a->di_bias) && !a->i) return KDA_ERR_ARG;
+    if (!a->x || !a->r || !a->dx || !a->dr || !a->tiles || a->ldx < a->C || a->ldr < a->C || a->lddx < a->C || a->lddr < a->C) return KDA_ERR_ARG;
+    if ((a->dy && a->lddy < a->C) || (a->i && (!a->di || a->ldi < a->C || a->lddi < a->C))) return KDA_ERR_ARG;
+  }
+  kda::GatedScanGradParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x; p.r = a->r; p.i = a->i; p.dy = a->dy; p.dx = a->dx; p.dr = a->dr; p.di = a->di;
+  p.rate = a->rate; p.r_bias = a->r_bias; p.i_bias = a->i_bias; p.tiles = a->tiles; p.src = a->src; p.dfinal = a->dfinal; p.dsrc = a->dsrc;
+  p.drate = a->drate; p.dr_bias = a->dr_bias; p.di_bias = a->di_bias;
+  p.seq = seq_table(seq);
+  p.ldx = a->ldx; p.ldr = a->ldr; p.ldi = a->i ? a->ldi : 0; p.lddy = a->dy ? a->lddy : 0; p.lddx = a->lddx; p.lddr = a->lddr; p.lddi = a->i ? a->lddi : 0;
+  p.rate_scale = a->rate_scale; p.C = a->C;
+  return launched(kda::launch_gated_scan_grad(p, a->type, reinterpret_cast<cudaStream_t>(stream)));
+}
+
+size_t kda_group_norm_workspace_bytes(int64_t T, int32_t G, int32_t D, int32_t type, int32_t shared) {
+  if (T < 0 || G < 1 || D < 1 || D > KDA_GROUP_NORM_MAX_WIDTH || !known_type(type)) return 0;
+  return sizeof(float) * (size_t)kda::group_norm_partial_floats(T, G, D, type, shared != 0);
+}
+int kda_group_norm_launch(const KdaGroupNormArgs* a, void* stream) { return group_norm_launch(a, false, stream); }
+int kda_group_norm_grad_launch(const KdaGroupNormArgs* a, void* stream) { return group_norm_launch(a, true, stream); }
 
 size_t kda_pool_workspace_bytes(int64_t n, int64_t P) {
   if (n < 0 || P < 1) return 0;

@@ -163,4 +163,35 @@ __device__ __forceinline__ float silu(float x) {
   return x * r;
 }
 
+__device__ __forceinline__ float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float min_or_nan(float a, float b) {       // NaN if one of them is
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// sigmoid(x + bias) and 1 minus it, both to relative accuracy.  16-bit tokens: the approximate exponential and reciprocal, some
+// 2^-21 off, with `bias` scaled by -log2(e).  e^-x stops at 2^126, behind which the sigmoid is 2^-126 and its product with e^-x still 1.
+template <typename T>
+__device__ __forceinline__ void sigmoid_pair(float x, float bias, float& s, float& n) {
+  float e;
+  if constexpr (sizeof(T) == 4) {
+    e = expf(min_or_nan(-(x + bias), 87.0f));
+    s = 1.0f / (1.0f + e);
+  } else {
+    e = ex2_fast(min_or_nan(fmaf(x, -1.4426950408889634f, bias), 126.0f));
+    s = rcp_fast(1.0f + e);
+  }
+  n = e * s;
+}
+
 }  // namespace kda

@@ -51,6 +51,58 @@ struct StepParams {
 };
 cudaError_t launch_kda_step(const StepParams& p, cudaStream_t stream);
 
+constexpr int GATED_SCAN_TILE = 64;      // a training pass keeps the states in front of every so many tokens
+struct GatedScanParams {
+  const void *x, *r, *i;   // [T][C]; i may be nullptr
+  void* out;
+  const float *rate, *r_bias, *i_bias;   // [C]; each may be nullptr, rate: the form without it
+  const float* src;        // states [slot][C]; nullptr: zeros
+  float* dst;              // may be src; nullptr: not stored
+  float* tiles;            // [tiles of T][C]: the states in front of them; nullptr: not kept
+  SeqTable seq;
+  long long ldx, ldr, ldi, ldo, src_stride, dst_stride;
+  float rate_scale;
+  int C, zero_pad;
+  int tile;                // step: rows of a block, set by the launcher
+};
+cudaError_t launch_gated_scan(const GatedScanParams& p, int type, cudaStream_t stream);
+cudaError_t launch_gated_scan_step(const GatedScanParams& p, int type, cudaStream_t stream);
+
+struct GatedScanGradParams {
+  const void *x, *r, *i, *dy;            // i and dy may be nullptr
+  void *dx, *dr, *di;      // [T][C]; di with i
+  const float *rate, *r_bias, *i_bias;
+  const float* tiles;      // of the forward pass
+  const float* src;        // its initial states [N][C]; nullptr: zeros
+  const float* dfinal;     // [N][C]; nullptr: zeros
+  float* dsrc;             // [N][C]; nullptr: not wanted
+  float *drate, *dr_bias, *di_bias;      // [C]; each nullptr: not wanted
+  SeqTable seq;            // without slots
+  long long ldx, ldr, ldi, lddy, lddx, lddr, lddi;
+  float rate_scale;
+  int C;
+};
+cudaError_t launch_gated_scan_grad(const GatedScanGradParams& p, int type, cudaStream_t stream);
+
+// Norm of each group of D channels of a token, with an activation: of the gate z, or of the normalised value.
+struct GroupNormParams {
+  const void *x, *z, *dy;  // [T][G D]; z may be nullptr; dy: gradients only
+  void* out;               // y, or dx
+  void* dz;                // gradients with z
+  const float *weight, *bias;            // [G D], or [D] with `shared`; may be nullptr
+  float *dweight, *dbias;  // their gradients' sums; nullptr: not wanted
+  float* partial;          // gradients: the workspace
+  long long T, ldx, ldz, lddy, ldo, lddz;
+  float eps;
+  int G, D, act, center, shared;         // act: ACT_*
+  int lanes, parts;        // set by the launcher: threads of a group, blocks along the rows
+};
+enum { ACT_NONE = 0, ACT_SILU = 1, ACT_SIGMOID = 2 };
+constexpr int GROUP_NORM_MAX_WIDTH = 16384;
+cudaError_t launch_group_norm(const GroupNormParams& p, int type, cudaStream_t stream);
+cudaError_t launch_group_norm_grad(const GroupNormParams& p, int type, cudaStream_t stream);
+long long group_norm_partial_floats(long long T, int G, int D, int type, bool shared);
+
 constexpr int POOLS_MAX = 8, TABLES_MAX = 8;
 struct PoolRows {          // the pools that share one table of slots
   unsigned char* base[POOLS_MAX];

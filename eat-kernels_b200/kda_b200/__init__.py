@@ -17,7 +17,7 @@ cu_seqlens [N+1] int32/int64 or None (one sequence).  Gate, beta sigmoid and q/k
 key-first [N, H, K, V]).
 
 The operators around it in a recurrent layer (short convolution, selective scan, the single-token steps) are in `serving.py`, the
-upkeep of the slot pools in `pool.py`.
+gated linear recurrence and the norm of groups of channels, with their gradients, in `gated.py`, the upkeep of the slot pools in `pool.py`.
 
 All compute goes through the C ABI of libkda_b200.so (include/kda_b200.h); this module only checks arguments,
 owns output / workspace tensors and passes raw device pointers.  There is no CPU or eager fallback.
@@ -37,7 +37,7 @@ LOWER_BOUND = -5.0   # the reference fixes the gate's lower bound (kda/b200/csrc
 
 __all__ = ["kda_prefill", "run", "prepare", "status_bits", "chunk_kda", "prepare_plain",
            "short_conv", "short_conv_step", "selective_scan", "selective_scan_step", "kda_step", "kda_step_plain",
-           "pool_copy", "pool_fork", "pool_free", "pool_compact"]
+           "gated_scan", "gated_scan_step", "group_norm", "pool_copy", "pool_fork", "pool_free", "pool_compact"]
 
 
 def default_kernel():
@@ -424,6 +424,7 @@ def chunk_kda(q, k, v, g, beta, scale=None, initial_state=None, output_final_sta
     return (o if dt == torch.bfloat16 else o.to(dt), *res[1:])
 
 
+from .gated import gated_scan, gated_scan_step, group_norm  # noqa: E402
 from .pool import pool_compact, pool_copy, pool_fork, pool_free  # noqa: E402
 from .serving import (kda_step, kda_step_plain, selective_scan, selective_scan_step, short_conv,  # noqa: E402
                       short_conv_step)

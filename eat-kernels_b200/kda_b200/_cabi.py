@@ -17,9 +17,13 @@ EXPORTS = ["kda_prefill_workspace_bytes", "kda_prefill_workspace_bytes_cuts", "k
            "kda_fixup_launch", "kda_fixup_tiles_launch", "kda_segment_tiles", "kda_state_rows_copy", "kda_error_string", "kda_abi_struct_bytes", "kda_version",
            "kda_debug_configure", "kda_short_conv_launch", "kda_short_conv_step_launch", "kda_selective_scan_workspace_bytes",
            "kda_selective_scan_launch", "kda_selective_scan_step_launch", "kda_step_launch", "kda_pool_workspace_bytes",
-           "kda_pool_copy_launch", "kda_pool_fork_launch", "kda_pool_free_launch", "kda_pool_compact_launch"]
+           "kda_pool_copy_launch", "kda_pool_fork_launch", "kda_pool_free_launch", "kda_pool_compact_launch",
+           "kda_gated_scan_launch", "kda_gated_scan_step_launch", "kda_gated_scan_grad_launch", "kda_group_norm_workspace_bytes",
+           "kda_group_norm_launch", "kda_group_norm_grad_launch"]
 TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
 SCAN_MAX_STATE, MAX_POOLS, MAX_TABLES = 128, 8, 8
+GATED_SCAN_TILE, GROUP_NORM_MAX_WIDTH = 64, 16384
+ACT_NONE, ACT_SILU, ACT_SIGMOID = 0, 1, 2
 
 
 class KdaPrefillArgs(C.Structure):
@@ -107,7 +111,43 @@ class KdaPoolArgs(C.Structure):
     ]
 
 
-STRUCTS = [KdaPrefillArgs, KdaSegmentArgs, KdaConvArgs, KdaScanArgs, KdaStepArgs, KdaPoolArgs]
+class KdaGatedScanArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("r", C.c_void_p), ("i", C.c_void_p), ("out", C.c_void_p), ("rate", C.c_void_p),
+        ("r_bias", C.c_void_p), ("i_bias", C.c_void_p), ("src", C.c_void_p), ("dst", C.c_void_p), ("tiles", C.c_void_p),
+        ("ldx", C.c_int64), ("ldr", C.c_int64), ("ldi", C.c_int64), ("ldo", C.c_int64), ("src_slot_stride", C.c_int64),
+        ("dst_slot_stride", C.c_int64),
+        ("seq", KdaSequences),
+        ("rate_scale", C.c_float), ("C", C.c_int32), ("type", C.c_int32),
+    ]
+
+
+class KdaGatedScanGradArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("r", C.c_void_p), ("i", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p), ("dr", C.c_void_p),
+        ("di", C.c_void_p), ("rate", C.c_void_p), ("r_bias", C.c_void_p), ("i_bias", C.c_void_p), ("tiles", C.c_void_p),
+        ("src", C.c_void_p), ("dfinal", C.c_void_p), ("dsrc", C.c_void_p), ("drate", C.c_void_p), ("dr_bias", C.c_void_p),
+        ("di_bias", C.c_void_p),
+        ("ldx", C.c_int64), ("ldr", C.c_int64), ("ldi", C.c_int64), ("lddy", C.c_int64), ("lddx", C.c_int64),
+        ("lddr", C.c_int64), ("lddi", C.c_int64),
+        ("seq", KdaSequences),
+        ("rate_scale", C.c_float), ("C", C.c_int32), ("type", C.c_int32),
+    ]
+
+
+class KdaGroupNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("z", C.c_void_p), ("dy", C.c_void_p), ("out", C.c_void_p), ("dz", C.c_void_p), ("weight", C.c_void_p),
+        ("bias", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("T", C.c_int64), ("ldx", C.c_int64), ("ldz", C.c_int64), ("lddy", C.c_int64), ("ldo", C.c_int64), ("lddz", C.c_int64),
+        ("eps", C.c_float), ("G", C.c_int32), ("D", C.c_int32), ("act", C.c_int32), ("center", C.c_int32), ("shared", C.c_int32),
+        ("type", C.c_int32),
+    ]
+
+
+STRUCTS = [KdaPrefillArgs, KdaSegmentArgs, KdaConvArgs, KdaScanArgs, KdaStepArgs, KdaPoolArgs, KdaGatedScanArgs, KdaGatedScanGradArgs,
+           KdaGroupNormArgs]
 _lib = None
 
 
@@ -159,11 +199,16 @@ def lib():
         L.kda_abi_struct_bytes.restype = C.c_size_t
         for name, block in (("short_conv", KdaConvArgs), ("short_conv_step", KdaConvArgs), ("selective_scan", KdaScanArgs),
                             ("selective_scan_step", KdaScanArgs), ("step", KdaStepArgs), ("pool_copy", KdaPoolArgs),
-                            ("pool_fork", KdaPoolArgs), ("pool_free", KdaPoolArgs), ("pool_compact", KdaPoolArgs)):
+                            ("pool_fork", KdaPoolArgs), ("pool_free", KdaPoolArgs), ("pool_compact", KdaPoolArgs),
+                            ("gated_scan", KdaGatedScanArgs), ("gated_scan_step", KdaGatedScanArgs),
+                            ("gated_scan_grad", KdaGatedScanGradArgs), ("group_norm", KdaGroupNormArgs),
+                            ("group_norm_grad", KdaGroupNormArgs)):
             entry = getattr(L, f"kda_{name}_launch")
             entry.argtypes, entry.restype = [C.POINTER(block), C.c_void_p], C.c_int
         L.kda_selective_scan_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
         L.kda_selective_scan_workspace_bytes.restype = C.c_size_t
+        L.kda_group_norm_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+        L.kda_group_norm_workspace_bytes.restype = C.c_size_t
         L.kda_pool_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
         L.kda_pool_workspace_bytes.restype = C.c_size_t
         if any(L.kda_abi_struct_bytes(i) != C.sizeof(block) for i, block in enumerate(STRUCTS)):

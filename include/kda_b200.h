@@ -320,6 +320,73 @@ typedef struct KdaStepArgs {
 } KdaStepArgs;
 int kda_step_launch(const KdaStepArgs* args, void* stream);
 
+/* Gated linear recurrence, per channel, states fp32:
+ *   s = sigmoid(r + r_bias), g = sigmoid(i + i_bias) (1 without i);
+ *   with rate: f = exp(-rate_scale softplus(rate) s), gain = sqrt(1 - f^2);  without: f = s, gain = 1 - s;
+ *   h = f h + gain g x;  out = h
+ * One kernel launch. */
+typedef struct KdaGatedScanArgs {
+  const void *x, *r;       /* [T][C] */
+  const void* i;           /* [T][C] or NULL; all of one type */
+  void* out;               /* [T][C] */
+  const float* rate;       /* [C] or NULL */
+  const float* r_bias;     /* [C] or NULL */
+  const float* i_bias;     /* [C] or NULL; only with i */
+  const float* src;        /* [slot][C]; NULL = zeros */
+  float* dst;              /* NULL = not stored; may be src.  A step needs src == dst */
+  float* tiles;            /* [(T + 63) / 64][C], packed: the states that a later kda_gated_scan_grad_launch starts from; or NULL.
+                              Unused in a step */
+  int64_t ldx, ldr, ldi, ldo, src_slot_stride, dst_slot_stride;
+  KdaSequences seq;
+  float rate_scale;
+  int32_t C, type;
+} KdaGatedScanArgs;
+#define KDA_GATED_SCAN_TILE 64
+int kda_gated_scan_launch(const KdaGatedScanArgs* args, void* stream);
+int kda_gated_scan_step_launch(const KdaGatedScanArgs* args, void* stream);
+
+/* Its gradients, from those of out and of the final states.  Rows behind the last sequence get zeros, and with a rejected cu_seqlens
+ * (KDA_STATUS_BAD_CU) all rows and sums; an empty sequence's dsrc is its dfinal.  Sums do not depend on timing.  One kernel launch. */
+typedef struct KdaGatedScanGradArgs {
+  const void *x, *r, *i;   /* as given to the forward call, rate, r_bias, i_bias, src, cu_seqlens and rate_scale too */
+  const void* dy;          /* [T][C], or NULL: zeros */
+  void *dx, *dr, *di;      /* [T][C]; di with i */
+  const float *rate, *r_bias, *i_bias;
+  const float* tiles;      /* what the forward call left there */
+  const float* src;        /* [N][C], packed; NULL = zeros */
+  const float* dfinal;     /* [N][C], packed; NULL = zeros */
+  float* dsrc;             /* [N][C], packed, or NULL */
+  float *drate, *dr_bias, *di_bias;    /* [C] or NULL */
+  int64_t ldx, ldr, ldi, lddy, lddx, lddr, lddi;
+  KdaSequences seq;        /* no slots */
+  float rate_scale;
+  int32_t C, type;
+} KdaGatedScanGradArgs;
+int kda_gated_scan_grad_launch(const KdaGatedScanGradArgs* args, void* stream);
+
+/* Norm of each group of D channels of a token, with an activation: xh = (x - mean) / sqrt(mean((x - mean)^2) + eps), mean = 0 without
+ * `center`;  n = xh weight + bias;  out = n act(z), or act(n) without z.  One kernel launch, two for the gradients of the weights. */
+enum { KDA_ACT_NONE = 0, KDA_ACT_SILU = 1, KDA_ACT_SIGMOID = 2 };
+typedef struct KdaGroupNormArgs {
+  const void *x, *z;       /* [T][G][D]; z may be NULL; all tensors of one type */
+  const void* dy;          /* gradients: [T][G][D] */
+  void* out;               /* [T][G][D]: y; gradients: dx */
+  void* dz;                /* gradients with z: [T][G][D] */
+  const float *weight, *bias;          /* [G][D], or [D] with `shared`; NULL: ones, zeros */
+  float *dweight, *dbias;  /* gradients: like them; NULL: not wanted */
+  void* workspace;         /* gradients with dweight or dbias: kda_group_norm_workspace_bytes(..) bytes, 16-byte aligned; contents need
+                              not survive, but concurrent calls must not share it */
+  size_t workspace_bytes;
+  int64_t T, ldx, ldz, lddy, ldo, lddz;
+  float eps;
+  int32_t G, D;            /* D <= KDA_GROUP_NORM_MAX_WIDTH */
+  int32_t act, center, shared, type;
+} KdaGroupNormArgs;
+#define KDA_GROUP_NORM_MAX_WIDTH 16384
+size_t kda_group_norm_workspace_bytes(int64_t T, int32_t G, int32_t D, int32_t type, int32_t shared);
+int kda_group_norm_launch(const KdaGroupNormArgs* args, void* stream);
+int kda_group_norm_grad_launch(const KdaGroupNormArgs* args, void* stream);
+
 /* Upkeep of pools that share one table of slots (states, convolution histories, ...).  Row s of pool k: bytes [base[k] +
  * s * stride[k], + bytes[k]).  Two launches (kda_pool_free_launch: one); nothing is read on the host. */
 #define KDA_MAX_POOLS 8
@@ -361,8 +428,8 @@ int kda_pool_compact_launch(const KdaPoolArgs* args, void* stream);
 /* Text of a KDA_ERR_* code; for KDA_ERR_LAUNCH the last CUDA error string seen by this thread. */
 const char* kda_error_string(int code);
 
-/* sizeof of KdaPrefillArgs (which = 0), KdaSegmentArgs (1), KdaConvArgs (2), KdaScanArgs (3), KdaStepArgs (4) or KdaPoolArgs (5)
- * as the library was compiled: lets a foreign
+/* sizeof of KdaPrefillArgs (which = 0), KdaSegmentArgs (1), KdaConvArgs (2), KdaScanArgs (3), KdaStepArgs (4), KdaPoolArgs (5),
+ * KdaGatedScanArgs (6), KdaGatedScanGradArgs (7) or KdaGroupNormArgs (8) as the library was compiled: lets a foreign
  * binding check its struct layout before the first call. */
 size_t kda_abi_struct_bytes(int which);
 
