@@ -16,11 +16,8 @@ namespace kda {
 namespace gscan {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int S = 8;                     // tokens of a slice
-constexpr int TILE = WARPS * S;
 constexpr int MAX_CLUSTER = 8;
 constexpr long long NEVER = 0x7fffffffffffffffLL;
-static_assert(TILE == GATED_SCAN_TILE, "the states that a training pass keeps are those in front of the tiles");
 
 // A product of decays that underflows to zero is taken as the smallest positive number, so that an infinite state stays infinite, as it
 // does token by token (a finite one is not changed by that).  Where a decay is NaN, so is the map's constant.
@@ -40,17 +37,6 @@ __device__ __forceinline__ float bias_of(const float* p, int c) {
   return sizeof(T) == 4 ? b : -LOG2E_F * b;
 }
 
-// -(e^y - 1) for y = 2 ln2 l <= 0, e = 2^l given: near zero by a polynomial for (e^y - 1) / y on [-1/2, 0] (relative minimax, found by
-// linear programming: 1.0e-7 off in fp32), which 1 - e e would lose its digits for
-__device__ __forceinline__ float one_minus_square(float l, float e) {
-  const float y = l * (2.0f * LN2_F);
-  float q = fmaf(y, 0.006771687883883715f, 0.0410030297935009f);
-  q = fmaf(y, q, 0.1665491908788681f);
-  q = fmaf(y, q, 0.4999926686286926f);
-  q = fmaf(y, q, 0.9999999403953552f);
-  return y > -0.5f ? -y * q : fmaf(-e, e, 1.0f);
-}
-
 // softplus in full precision, once a channel
 __device__ __forceinline__ float softplus_exact(float x) { return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))); }
 
@@ -62,41 +48,20 @@ __device__ __forceinline__ float decay_factor(const float* rate, int c, float sc
   return k < -3.0e38f ? -3.0e38f : k;
 }
 
-// A token's values of one channel.  `l` (POWER) is log f, natural for 32-bit tokens, else base 2; s, n: of the decay's gate; inv: 1 / gain.
-struct Gates {
-  float f, gain, s, n, l, inv;
-};
-template <typename T, bool POWER>
-__device__ __forceinline__ Gates decay(float r, float bias, float k) {
-  Gates a;
-  sigmoid_pair<T>(r, bias, a.s, a.n);
-  if constexpr (!POWER) {
-    a.f = a.s; a.gain = a.n; a.l = a.inv = 0.0f;
-  } else {
-    a.l = k * a.s;
-    if constexpr (sizeof(T) == 4) {
-      a.f = expf(a.l);
-      a.gain = sqrtf(-expm1f(2.0f * a.l));
-      a.inv = 1.0f / fmaxf(a.gain, 1.0e-19f);
-    } else {
-      a.f = ex2_fast(a.l);
-      const float q = one_minus_square(a.l, a.f);
-      a.inv = rsqrt_fast(fmaxf(q, 1.0e-38f));          // l times it is 0 where l is
-      a.gain = q * a.inv;
-    }
-  }
-  return a;
-}
-
 // ---- sequences
-// Called by a warp: the first entry from j on that is >= t (N + 1: none)
-__device__ __forceinline__ int seek(const SeqTable& s, int j, long long t) {
+// Called by a warp: the first of the entries [lo, hi) that is >= t, hi where none is.  32 entries are looked at at a time.
+__device__ __forceinline__ int lower(const SeqTable& s, int lo, int hi, long long t) {
   const int lane = threadIdx.x % 32;
-  for (; j <= s.N; j += 32) {
-    const unsigned at = __ballot_sync(0xffffffffu, j + lane > s.N || cu_at(s, j + lane) >= t);
-    if (at != 0) return min(j + __ffs(at) - 1, s.N + 1);
+  while (lo < hi) {
+    const int part = (hi - lo + 31) / 32;
+    const long long at = (long long)lo + (long long)(lane + 1) * part - 1;
+    const unsigned found = __ballot_sync(0xffffffffu, cu_at(s, at < hi ? at : hi - 1) >= t);
+    if (found == 0) return hi;
+    const int first = __ffs(found) - 1;
+    hi = min(hi - 1, lo + (first + 1) * part - 1);
+    lo = lo + first * part;
   }
-  return s.N + 1;
+  return lo;
 }
 
 // Called by a warp: the slot of sequence i, or -1 where its entry is out of range or repeats an earlier one
@@ -124,39 +89,199 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void put_remote(void* own, uint32_t rank, float v) {        // at the address of `own` in another block
+// at the address of `own` in another block
+__device__ __forceinline__ void put_remote(const void* own, uint32_t rank, float4 v) {
+  const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
+  asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.v4.f32 [t], {%2, %3, %4, %5};\n}" ::"r"(a), "r"(rank), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void put_remote(const void* own, uint32_t rank, float v) {
   const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.f32 [t], %2;\n}" ::"r"(a), "r"(rank), "f"(v) : "memory");
 }
-__device__ __forceinline__ void put_remote(uint32_t* own, uint32_t rank, uint32_t v) {
+__device__ __forceinline__ void put_remote(const void* own, uint32_t rank, uint32_t v) {
   const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.u32 [t], %2;\n}" ::"r"(a), "r"(rank), "r"(v) : "memory");
 }
 
-// ---- tokens
-// Channels of a lane: two 16-bit ones in an access of 4 bytes, or one
-template <typename T, bool WIDE>
-constexpr int CHANNELS = WIDE ? 4 / (int)sizeof(T) : 1;
-
-// The rows of a slice, as they lie in memory, for one tensor: asked for a round ahead
-template <typename T, int V>
-struct Rows {
-  Pack<T, V> v[S];
-  __device__ __forceinline__ void ask(const void* base, long long ld, long long t0, int n, int c, bool mine) {
-    const T* p = reinterpret_cast<const T*>(base) + c + t0 * ld;
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-      if (mine && s < n) v[s] = *reinterpret_cast<const Pack<T, V>*>(p + s * ld);
-      else
-#pragma unroll
-        for (int k = 0; k < V; k++) v[s].v[k] = from_float<T>(0.0f);
-    }
-  }
+// ---- one or two channels at once (two: one instruction)
+template <int V>
+struct Vec {
+  float v[V];
 };
+template <int V>
+__device__ __forceinline__ Vec<V> vec(float a) {
+  Vec<V> r;
+#pragma unroll
+  for (int k = 0; k < V; k++) r.v[k] = a;
+  return r;
+}
+__device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v[0], b.v[0], c.v[0])}; }
+__device__ __forceinline__ Vec<1> mul(Vec<1> a, Vec<1> b) { return {a.v[0] * b.v[0]}; }
+__device__ __forceinline__ Vec<1> add(Vec<1> a, Vec<1> b) { return {a.v[0] + b.v[0]}; }
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) {
+  Vec<2> d;
+  asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2,%3};\n mov.b64 rb, {%4,%5};\n mov.b64 rc, {%6,%7};\n fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0,%1}, rd;\n}"
+      : "=f"(d.v[0]), "=f"(d.v[1]) : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]), "f"(c.v[0]), "f"(c.v[1]));
+  return d;
+}
+__device__ __forceinline__ Vec<2> mul(Vec<2> a, Vec<2> b) {
+  Vec<2> d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2,%3};\n mov.b64 rb, {%4,%5};\n mul.rn.f32x2 rd, ra, rb;\n mov.b64 {%0,%1}, rd;\n}"
+      : "=f"(d.v[0]), "=f"(d.v[1]) : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+  return d;
+}
+__device__ __forceinline__ Vec<2> add(Vec<2> a, Vec<2> b) {
+  Vec<2> d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2,%3};\n mov.b64 rb, {%4,%5};\n add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0,%1}, rd;\n}"
+      : "=f"(d.v[0]), "=f"(d.v[1]) : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+  return d;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> least(Vec<V> a) {        // at least LEAST
+#pragma unroll
+  for (int k = 0; k < V; k++) a.v[k] = fmaxf(a.v[k], LEAST);
+  return a;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> pick(bool first, Vec<V> a, Vec<V> b) {
+#pragma unroll
+  for (int k = 0; k < V; k++) a.v[k] = first ? a.v[k] : b.v[k];
+  return a;
+}
 
+// ---- tokens
+// Channels of a lane: two 16-bit ones where rows start on 16 bytes, else one
+template <typename T, bool ASYNC>
+constexpr int CHANNELS = ASYNC ? 4 / (int)sizeof(T) : 1;
+
+template <int S>
 __device__ __forceinline__ int count(long long t0, long long end) {        // tokens of the slice at t0
   const long long n = end - t0;
   return n < 0 ? 0 : (n > S ? S : (int)n);
+}
+
+// A warp's slice of one tensor.  ASYNC: S rows of 128 bytes in shared memory, by copies of 16 bytes that are asked for rounds ahead;
+// places behind the last token or channel are zeros.  Otherwise S registers, asked for a round ahead.
+template <typename T, int S>
+struct Slice {
+  Pack<T, 4 / sizeof(T)> row[S][32];
+
+  __device__ __forceinline__ void ask(const void* base, long long ld, long long t0, int n, int c0, int C) {
+    const int lane = threadIdx.x % 32, chunk = lane % 8;
+    const int c = c0 + chunk * (16 / (int)sizeof(T));
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(this)) + (uint32_t)(lane / 8 * 128 + chunk * 16);
+    const T* from = reinterpret_cast<const T*>(base) + (t0 + lane / 8) * ld + c;
+#pragma unroll
+    for (int q = 0; q < S / 4; q++) {
+      const bool on = c < C && lane / 8 + 4 * q < n;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512u * q), "l"(on ? (const void*)from : base), "r"(on ? 16 : 0) : "memory");
+      from += 4 * ld;
+    }
+  }
+  // the first n rows to memory; the warp has written them
+  __device__ __forceinline__ void store(void* base, long long ld, long long t0, int n, int c0, int C) const {
+    const int lane = threadIdx.x % 32, chunk = lane % 8;
+    const int c = c0 + chunk * (16 / (int)sizeof(T));
+    T* to = reinterpret_cast<T*>(base) + (t0 + lane / 8) * ld + c;
+#pragma unroll
+    for (int q = 0; q < S / 4; q++) {
+      if (c < C && lane / 8 + 4 * q < n) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(this) + lane / 8 * 128 + chunk * 16 + 512 * q);
+      to += 4 * ld;
+    }
+  }
+};
+template <typename T, int S>
+struct Registers {
+  T row[S];
+  __device__ __forceinline__ void ask(const void* base, long long ld, long long t0, int n, int c, int C) {
+    const T* from = reinterpret_cast<const T*>(base) + t0 * ld + c;
+    if (c < C && n == S) {
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        row[s] = *from;
+        from += ld;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        row[s] = from_float<T>(0.0f);
+        if (c < C && s < n) row[s] = *from;
+        from += ld;
+      }
+    }
+  }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<V> values(const Pack<T, V>& p) {
+  Vec<V> r;
+#pragma unroll
+  for (int k = 0; k < V; k++) r.v[k] = to_float(p.v[k]);
+  return r;
+}
+
+// Of V channels: sigmoid and 1 minus it
+template <typename T, int V>
+__device__ __forceinline__ void sigmoids(Vec<V> x, Vec<V> bias, Vec<V>& s, Vec<V>& n) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < V; k++) sigmoid_pair<T>(x.v[k], bias.v[k], s.v[k], n.v[k]);
+  } else {
+    Vec<V> e = fma(x, vec<V>(-LOG2E_F), bias);
+#pragma unroll
+    for (int k = 0; k < V; k++) e.v[k] = ex2_fast(min_or_nan(e.v[k], 126.0f));
+    s = add(e, vec<V>(1.0f));
+#pragma unroll
+    for (int k = 0; k < V; k++) s.v[k] = rcp_fast(s.v[k]);
+    n = mul(e, s);
+  }
+}
+
+// A token's values.  `l` (POWER) is log f, natural for 32-bit tokens, else base 2; s, n: of the decay's gate; inv: 1 / gain.
+template <int V>
+struct Gates {
+  Vec<V> f, gain, s, n, l, inv;
+};
+template <typename T, bool POWER, int V>
+__device__ __forceinline__ Gates<V> decay(Vec<V> r, Vec<V> bias, Vec<V> k_) {
+  Gates<V> a;
+  sigmoids<T, V>(r, bias, a.s, a.n);
+  if constexpr (!POWER) {
+    a.f = a.s; a.gain = a.n; a.l = a.inv = vec<V>(0.0f);
+  } else {
+    a.l = mul(k_, a.s);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        a.f.v[k] = expf(a.l.v[k]);
+        a.gain.v[k] = sqrtf(-expm1f(2.0f * a.l.v[k]));
+        a.inv.v[k] = 1.0f / fmaxf(a.gain.v[k], 1.0e-19f);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; k++) a.f.v[k] = ex2_fast(a.l.v[k]);
+      // 1 - f^2 = -(e^y - 1), y = 2 ln2 l <= 0: near zero by a polynomial for (e^y - 1) / y on [-1/2, 0] (relative minimax, found by linear
+      // programming, 1.0e-7 off in fp32), as the difference would lose its digits there
+      const Vec<V> y = mul(a.l, vec<V>(2.0f * LN2_F));
+      Vec<V> q = fma(y, vec<V>(0.006771687883883715f), vec<V>(0.0410030297935009f));
+      q = fma(y, q, vec<V>(0.1665491908788681f));
+      q = fma(y, q, vec<V>(0.4999926686286926f));
+      q = fma(y, q, vec<V>(0.9999999403953552f));
+      q = mul(q, y);
+      const Vec<V> d = fma(a.f, a.f, vec<V>(-1.0f));
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float m = y.v[k] > -0.5f ? -q.v[k] : -d.v[k];
+        a.inv.v[k] = rsqrt_fast(fmaxf(m, 1.0e-38f));     // l times it is 0 where l is
+        a.gain.v[k] = m * a.inv.v[k];
+      }
+    }
+  }
+  return a;
 }
 
 // Rows [end, T) of an output are zeros, spread over the blocks of a cluster
@@ -171,18 +296,23 @@ __device__ __forceinline__ void zero_rest(void* out, long long ld, long long end
 }
 
 // Blocks along time: as many as give the card two blocks an SM, no more than the batch has tiles
-inline int cluster_of(long long slabs, long long T) {
+inline int cluster_of(long long slabs, long long T, int tile) {
   int size = 1;
-  while (size < MAX_CLUSTER && slabs * size < 2 * 148 && (long long)size * TILE < T) size *= 2;
+  while (size < MAX_CLUSTER && slabs * size * 2 <= 2 * 148 && (long long)size * tile < T) size *= 2;
   return size;
 }
 
 template <typename K, typename P>
-cudaError_t launch_clusters(K kernel, const P& p, long long slabs, int size, cudaStream_t stream) {
+cudaError_t launch_clusters(K kernel, const P& p, long long slabs, int size, int bytes, cudaStream_t stream) {
   if (slabs * size > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(slabs * size));
   cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
