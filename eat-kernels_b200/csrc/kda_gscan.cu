@@ -7,17 +7,36 @@ namespace {
 
 using namespace gscan;
 
-// Stores the final states of the sequences that end at t: those of entries j and behind.  h: the state in front of t.
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int DEPTH = 2;                 // rounds of tokens on their way or worked on
+constexpr int S = 12, TILE = WARPS * S;  // tokens of a slice, of a block: 16 a slice do not fit 128 registers with all that a ragged batch takes
+static_assert(TILE == GATED_SCAN_TILE, "the states that a training pass keeps are those in front of the tiles");
+
+// One round's maps of the warps' slices, {F, U} of a lane's channels, double-buffered against warps (blocks) that are a round ahead.
 template <int V>
-__device__ __noinline__ void finish(const GatedScanParams& p, int j, long long t, bool all_empty, int c, bool mine, float h0, float h1) {
+struct Shared {
+  Vec<2 * V> map[2][WARPS][32];
+  float4 tile[2][MAX_CLUSTER][32];       // of the cluster's tiles, sent by their blocks: {F, F, U, U}; F < 0: the map is constant
+  unsigned long long sent[2];            // barriers: the tiles' maps have arrived
+  uint32_t starts[2][WARPS];             // whether a sequence starts there: the map is constant
+  Tables<true> tables;
+};
+
+struct Steps {             // bytes from a row to the fourth behind it
+  long long x, r, i, y;
+};
+
+// Stores the final states of the sequences that end at t.  h: the state in front of t.
+template <int V>
+__device__ __forceinline__ void finish(const GatedScanParams& p, const Layout<true> l, uint32_t t, bool all_empty, int c, bool mine, float h0, float h1) {
   if (p.dst == nullptr) return;
   const float h[2] = {h0, h1};
-  for (; j <= p.seq.N; j++) {
-    if (!all_empty && cu_at(p.seq, j) != t) return;
+  for (int j = all_empty ? 1 : lower(l, 0, p.seq.N + 1, t); j <= p.seq.N; j++) {
+    if (!all_empty && l.at(j) != t) return;
     if (j == 0) continue;
-    const bool empty = all_empty || cu_at(p.seq, j - 1) == t;
+    const bool empty = all_empty || l.at(j - 1) == t;
     if (empty && p.src == p.dst) continue;
-    const long long slot = claim(p.seq, j - 1);
+    const long long slot = claim(l, j - 1);
     if (slot < 0 || !mine) continue;
 #pragma unroll
     for (int k = 0; k < V; k++)
@@ -25,46 +44,36 @@ __device__ __noinline__ void finish(const GatedScanParams& p, int j, long long t
   }
 }
 
-constexpr int DEPTH = 2;                 // rounds of tokens on their way or worked on
-
-template <typename T, bool ASYNC>
-constexpr int TOKENS = ASYNC ? 16 : 8;   // of a slice
-
-// One round's maps of the warps' slices, {F, U} of a lane's channels, double-buffered against warps (blocks) that are a round ahead.
-template <int V>
-struct Shared {
-  Vec<2 * V> map[2][WARPS][32];
-  float4 tile[2][MAX_CLUSTER][32];       // of the cluster's tiles, written by their blocks: {F, F, U, U}
-  uint32_t starts[2][WARPS], tile_starts[2][MAX_CLUSTER];          // whether a sequence starts there: the map is constant
-};
-
 template <typename T, bool ASYNC, bool POWER, bool GATED>
-__global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid_constant__ GatedScanParams p) {
-  constexpr int V = CHANNELS<T, ASYNC>, S = TOKENS<T, ASYNC>, TILE = WARPS * S, NT = GATED ? 3 : 2;
+__global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid_constant__ GatedScanParams p, const __grid_constant__ Steps g) {
+  constexpr int V = CHANNELS<T, ASYNC>, NT = GATED ? 3 : 2;
   __shared__ Shared<V> sm;
   extern __shared__ __align__(128) unsigned char raw[];              // ASYNC: [DEPTH][WARPS][NT] slices
   using Tokens = Slice<T, S>;
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int c0 = (int)(blockIdx.x / size) * 32 * V, c = c0 + lane * V;
-  const bool mine = c < p.C;
+  const bool mine = c < p.C, chunk = c0 + lane % 8 * (16 / (int)sizeof(T)) < p.C;
+  if (threadIdx.x == 0)
+    for (int b = 0; b < 2; b++) bar_init(&sm.sent[b]);
   if (size > 1) cluster_arrive();                    // blocks write into one another: all of them have to be there
   const bool rejected = cu_rejected(p.seq);
-  const long long end = rejected ? 0 : cu_at(p.seq, p.seq.N);
-  const long long step = (long long)size * TILE;
-  const int rounds = end > 0 ? (int)((end + step - 1) / step) : 1;
+  const Layout<true> tables = rejected ? Layout<true>{p.seq, nullptr} : layout_of(p.seq, sm.tables);
+  const uint32_t end = rejected ? 0 : (uint32_t)cu_at(p.seq, p.seq.N);       // tokens fit 31 bits, and a round more 32
+  const uint32_t step = size * TILE;
+  const int rounds = end > 0 ? (int)(((long long)end + step - 1) / step) : 1;
 
-  long long t0 = (long long)rank * TILE + warp * S;
+  uint32_t t0 = rank * TILE + warp * S;
   Registers<T, S> rx, rr, ri;
   auto slice = [&](int slot, int k) -> Tokens& { return reinterpret_cast<Tokens*>(raw)[(slot * WARPS + warp) * NT + k]; };
   auto ask = [&](int ahead, int slot) {              // the tokens of a later round
-    const long long t = t0 + ahead * step;
+    const uint32_t t = t0 + ahead * step;
     const int m = count<S>(t, end);
     if constexpr (ASYNC) {
       if (m > 0) {
-        slice(slot, 0).ask(p.x, p.ldx, t, m, c0, p.C);
-        slice(slot, 1).ask(p.r, p.ldr, t, m, c0, p.C);
-        if (GATED) slice(slot, 2).ask(p.i, p.ldi, t, m, c0, p.C);
+        Cursor<T, S>(p.x, p.ldx, t, c0).ask(slice(slot, 0), g.x, m, chunk, p.x);
+        Cursor<T, S>(p.r, p.ldr, t, c0).ask(slice(slot, 1), g.r, m, chunk, p.r);
+        if (GATED) Cursor<T, S>(p.i, p.ldi, t, c0).ask(slice(slot, 2), g.i, m, chunk, p.i);
       }
       copies_commit();
     } else if (m > 0) {
@@ -74,85 +83,67 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
     }
   };
 #pragma unroll
-  for (int k = 0; k < (ASYNC ? DEPTH - 1 : 1); k++) ask(k, k);
+  for (int k = 0; k < (ASYNC ? 2 : 1); k++) ask(k, k);
   Vec<V> rb, ib, k_;
 #pragma unroll
   for (int k = 0; k < V; k++) {
     rb.v[k] = mine ? bias_of<T>(p.r_bias, c + k) : 0.0f;
     ib.v[k] = GATED && mine ? bias_of<T>(p.i_bias, c + k) : 0.0f;
-    k_.v[k] = POWER && mine ? decay_factor<T>(p.rate, c + k, p.rate_scale) : 0.0f;
+    k_.v[k] = POWER && mine ? decay_factor(p.rate, c + k, p.rate_scale) : 0.0f;
   }
-  int j = 0;                                         // first entry of cu_seqlens that is >= t0, once looked for
-  long long next = 0;                                // that entry
-  Vec<V> carry = vec<V>(0.0f);
+  uint32_t next = 0;                                 // the first entry of cu_seqlens that is not in front of the round's slice
+  int early = -1;                                    // the first sequence that starts in it, where its state has been asked for
+  Vec<V> carry = vec<V>(0.0f);                       // the state in front of a round
+  bool lost = false;
+
+  Vec<V> f[S], u[S];                                 // decays and terms of a round
+  auto gates = [&](int s, const Tokens& x, const Tokens& r, const Tokens& i) {
+    Vec<V> xs, rs, is;
+    if constexpr (ASYNC) {
+      xs = values(x.row[s][lane]); rs = values(r.row[s][lane]); is = values(i.row[s][lane]);
+    } else {
+      xs = vec<V>(to_float(rx.row[s])); rs = vec<V>(to_float(rr.row[s])); is = vec<V>(to_float(ri.row[s]));
+    }
+    token_terms<T, POWER, GATED, V>(xs, rs, is, rb, ib, k_, f[s], u[s]);
+  };
+  auto look = [&](uint32_t t, int buf) {             // for sequences that start in the slice at t, which is next; their place is that of its map
+    early = -1;
+    if (next < t) {
+      const int j = lower(tables, 0, p.seq.N + 1, t);
+      next = j <= p.seq.N ? tables.at(j) : NEVER;
+    }
+    if (next >= t + S || next >= end || p.src == nullptr) return;
+    early = lower(tables, 0, p.seq.N + 1, next + 1) - 1;
+    const long long from = claim(tables, early);
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      const bool here = from >= 0 && mine;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.map[buf][warp][lane].v[k]))),
+                   "l"(here ? p.src + from * p.src_stride + c + k : p.src), "r"(here ? 4 : 0) : "memory");
+    }
+  };
+  __syncthreads();                                   // the copies of the tables
+  if (!rejected) look(t0, 0);
+  if (ASYNC) {
+    copies_wait<1>();
+    __syncwarp();
+  }
+#pragma unroll
+  for (int s = 0; s < S; s++) gates(s, slice(0, 0), slice(0, 1), slice(0, NT - 1));
+  if (ASYNC) __syncwarp();
+  if (ASYNC) ask(2, 0);
+  else ask(1, 0);
   if (size > 1) cluster_wait();
 
-  int slot = 0;
-  for (int round = 0; round < rounds; round++) {
+  for (int round = 0; round < rounds; round++, t0 += step) {
     const int buf = round & 1, n = count<S>(t0, end);
-    if (next < t0) {
-      j = lower(p.seq, j, p.seq.N + 1, t0);
-      next = j <= p.seq.N ? cu_at(p.seq, j) : NEVER;
-    }
-    const bool begins = !rejected && next < t0 + n;  // some sequence starts in the slice
-    Vec<V> f[S], u[S];
-    if constexpr (ASYNC) {
-      copies_wait<DEPTH - 2>();
-      __syncwarp();                                  // the warp's copies have landed; the slot of the round before is no longer read
-      const Tokens &x = slice(slot, 0), &r = slice(slot, 1), &i = slice(slot, NT - 1);
-#pragma unroll
-      for (int s = 0; s < S; s++) {
-        const Gates<V> a = decay<T, POWER, V>(values(r.row[s][lane]), rb, k_);
-        f[s] = a.f;
-        u[s] = mul(a.gain, values(x.row[s][lane]));
-        if constexpr (GATED) {
-          Vec<V> g, ng;
-          sigmoids<T, V>(values(i.row[s][lane]), ib, g, ng);
-          u[s] = mul(u[s], g);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < S; s++) {
-        const Gates<V> a = decay<T, POWER, V>(vec<V>(to_float(rr.row[s])), rb, k_);
-        f[s] = a.f;
-        u[s] = mul(a.gain, vec<V>(to_float(rx.row[s])));
-        if constexpr (GATED) {
-          Vec<V> g, ng;
-          sigmoids<T, V>(vec<V>(to_float(ri.row[s])), ib, g, ng);
-          u[s] = mul(u[s], g);
-        }
-      }
-    }
-    // the next tokens: ASYNC into the slot of the round before
-    if (ASYNC) ask(DEPTH - 1, slot == 0 ? DEPTH - 1 : slot - 1);
-    else ask(1, 0);
-    if (n < S) {
-#pragma unroll
-      for (int s = 0; s < S; s++)
-        if (s >= n) { f[s] = vec<V>(1.0f); u[s] = vec<V>(0.0f); }
-    }
-    // sequences that start in the slice: the state they enter with joins the first token's term
+    if (size > 1 && threadIdx.x == 0) bar_expect(&sm.sent[buf], size * 512);
+    const bool begins = !rejected && next < t0 + n, plain = !begins && n == S;        // begins: some sequence starts in the slice
+    Vec<V> F, U;                                     // the slice's map
     uint32_t starts = 0;
-    if (begins) {
-      for (int q = j; q < p.seq.N; q++) {
-        const long long t = cu_at(p.seq, q);
-        if (t >= t0 + n) break;
-        if (cu_at(p.seq, q + 1) == t) continue;
-        const long long from = claim(p.seq, q);
-        const int at = (int)(t - t0);
-        starts |= 1u << at;
-        Vec<V> h0 = vec<V>(0.0f);
-#pragma unroll
-        for (int k = 0; k < V; k++)
-          if (p.src != nullptr && from >= 0 && mine) h0.v[k] = p.src[from * p.src_stride + c + k];
-#pragma unroll
-        for (int s = 0; s < S; s++)
-          if (s == at) u[s] = fma(f[s], h0, u[s]);
-      }
-    }
-    Vec<V> F = f[0], U = u[0];
-    if (starts == 0) {
+    if (plain) {
+      F = f[0];
+      U = u[0];
 #pragma unroll
       for (int s = 1; s < S; s++) {
         U = fma(f[s], U, u[s]);
@@ -160,7 +151,34 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
       }
     } else {
 #pragma unroll
-      for (int s = 1; s < S; s++) {
+      for (int s = 0; s < S; s++)
+        if (s >= n) { f[s] = vec<V>(1.0f); u[s] = vec<V>(0.0f); }
+      // sequences that start in the slice: the state they enter with joins the first token's term
+      if (begins) copies_wait<0>();                  // of `look`
+      for (int q = begins ? lower(tables, 0, p.seq.N + 1, t0) : p.seq.N; q < p.seq.N; q++) {
+        const uint32_t b = tables.at(q);
+        if (b >= t0 + n) break;
+        if (tables.at(q + 1) == b) continue;
+        const int at = (int)(b - t0);
+        starts |= 1u << at;
+        Vec<V> h0 = vec<V>(0.0f);
+        if (q == early) {
+#pragma unroll
+          for (int k = 0; k < V; k++) h0.v[k] = sm.map[buf][warp][lane].v[k];
+        } else if (p.src != nullptr) {
+          const long long from = claim(tables, q);
+#pragma unroll
+          for (int k = 0; k < V; k++)
+            if (from >= 0 && mine) h0.v[k] = p.src[from * p.src_stride + c + k];
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++)
+          if (s == at) u[s] = fma(f[s], h0, u[s]);
+      }
+      F = vec<V>(1.0f);
+      U = vec<V>(0.0f);
+#pragma unroll
+      for (int s = 0; s < S; s++) {
         U = pick(starts >> s & 1, u[s], fma(f[s], U, u[s]));
         F = mul(F, f[s]);
       }
@@ -172,103 +190,112 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
     sm.map[buf][warp][lane] = map;
     if (lane == 0) sm.starts[buf][warp] = starts;
     const bool some = __syncthreads_or(starts != 0);
-    auto slice_map = [&](int w, Vec<V>& Fw, Vec<V>& Uw) {
-      const Vec<2 * V> m = sm.map[buf][w][lane];
-#pragma unroll
-      for (int k = 0; k < V; k++) { Fw.v[k] = m.v[k]; Uw.v[k] = m.v[V + k]; }
-    };
     // the slices in front of this one
     Vec<V> Fb = vec<V>(1.0f), Ub = vec<V>(0.0f);
     bool cut = false;
 #pragma unroll
-    for (int w = 0; w < WARPS - 1; w++) {
-      if (w >= warp) break;
-      Vec<V> Fw, Uw;
-      slice_map(w, Fw, Uw);
-      const bool constant = some && sm.starts[buf][w] != 0;
-      cut |= constant;
-      Ub = constant ? Uw : fma(Fw, Ub, Uw);
-      Fb = least(mul(Fb, Fw));
-    }
-    Vec<V> h;
-    if (size == 1) {
-      h = cut ? Ub : fma(Fb, carry, Ub);
-      carry = h;                                     // the next round's
+    for (int q = 0; q < WARPS - 1; q++) {
+      if (q >= warp) break;
+      const Vec<2 * V> m = sm.map[buf][q][lane];
+      Vec<V> Fq, Uq;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        if (w < warp) continue;
-        Vec<V> Fw, Uw;
-        slice_map(w, Fw, Uw);
-        carry = some && sm.starts[buf][w] != 0 ? Uw : fma(Fw, carry, Uw);
+      for (int k = 0; k < V; k++) { Fq.v[k] = m.v[k]; Uq.v[k] = m.v[V + k]; }
+      Ub = fma(Fq, Ub, Uq);
+      Fb = mul(Fb, Fq);
+      if (some && sm.starts[buf][q] != 0) {
+        cut = true;
+        Ub = Uq;
+      }
+    }
+    Fb = least(Fb);
+    Vec<V> enter = carry;
+    if (size == 1) {
+#pragma unroll
+      for (int q = 0; q < WARPS; q++) {
+        const Vec<2 * V> m = sm.map[buf][q][lane];
+        Vec<V> Fq, Uq;
+#pragma unroll
+        for (int k = 0; k < V; k++) { Fq.v[k] = m.v[k]; Uq.v[k] = m.v[V + k]; }
+        carry = fma(Fq, carry, Uq);
+        if (some && sm.starts[buf][q] != 0) carry = Uq;
       }
     } else {
       if (warp == WARPS - 1) {                       // it has the tile's map: to every block of the cluster
-        const Vec<V> Ut = starts ? U : fma(F, Ub, U), Ft = least(mul(Fb, F));
-        for (uint32_t b = 0; b < size; b++) put_remote(&sm.tile[buf][rank][lane], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
-        if (lane < size) put_remote(&sm.tile_starts[buf][rank], lane, (uint32_t)(cut || starts != 0));
+        const Vec<V> Ut = starts ? U : fma(F, Ub, U);
+        Vec<V> Ft = least(mul(Fb, F));
+        if (cut || starts) Ft = vec<V>(-1.0f);
+        for (uint32_t b = 0; b < size; b++) send(&sm.tile[buf][rank][lane], &sm.sent[buf], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
       }
-      cluster_arrive();
-      cluster_wait();
-      Vec<V> enter = carry;
+      if (!lost) lost = !bar_wait(&sm.sent[buf], round >> 1 & 1);
 #pragma unroll
       for (int b = 0; b < MAX_CLUSTER; b++) {
         if (b >= size) break;
         const float4 m = sm.tile[buf][b][lane];
-        Vec<V> Fw, Uw;
-        Fw.v[0] = m.x; Fw.v[V - 1] = m.y; Uw.v[0] = m.z; Uw.v[V - 1] = m.w;
+        Vec<V> Fq, Uq;
+        Fq.v[0] = m.x; Fq.v[V - 1] = m.y; Uq.v[0] = m.z; Uq.v[V - 1] = m.w;
         if (b == rank) enter = carry;
-        carry = sm.tile_starts[buf][b] != 0 ? Uw : fma(Fw, carry, Uw);
+        carry = pick(m.x < 0.0f, Uq, fma(Fq, carry, Uq));
       }
-      h = cut ? Ub : fma(Fb, enter, Ub);
     }
-    if (p.tiles != nullptr && warp % (GATED_SCAN_TILE / S) == 0 && mine && n > 0) {
+    Vec<V> h = cut ? Ub : fma(Fb, enter, Ub);
+    if (p.tiles != nullptr && warp == 0 && mine && n > 0) {
 #pragma unroll
-      for (int k = 0; k < V; k++) p.tiles[(t0 / GATED_SCAN_TILE) * p.C + c + k] = h.v[k];
+      for (int k = 0; k < V; k++) p.tiles[(long long)(t0 / TILE) * p.C + c + k] = h.v[k];
     }
-    Tokens& y = slice(slot, 0);
-    T* out = reinterpret_cast<T*>(p.out) + t0 * p.ldo + c;
-    auto token = [&](int s) {
-      if constexpr (ASYNC) y.row[s][lane] = pack<T, V>(h.v);
-      else if (mine) *out = from_float<T>(h.v[0]);
-      out += p.ldo;
-    };
-    if (!begins && n == S) {
-#pragma unroll
-      for (int s = 0; s < S; s++) {
-        h = fma(f[s], h, u[s]);
-        token(s);
-      }
-    } else {
+    T* out = reinterpret_cast<T*>(p.out) + (long long)t0 * p.ldo + c;
+    if (!plain && n > 0) {                           // token by token, with the ends of sequences
+      Vec<V> v = h;
 #pragma unroll
       for (int s = 0; s < S; s++) {
         if (s < n) {
-          if (begins && next <= t0 + s) {            // one of the entries may be this token
-            const int q = lower(p.seq, j, p.seq.N + 1, t0 + s);
-            if (q <= p.seq.N && cu_at(p.seq, q) == t0 + s) finish<V>(p, q, t0 + s, false, c, mine, h.v[0], h.v[V - 1]);
+          if (begins) {                              // one of the entries may be this token
+            const int q = lower(tables, 0, p.seq.N + 1, t0 + s);
+            if (q <= p.seq.N && tables.at(q) == t0 + s) finish<V>(p, tables, t0 + s, false, c, mine, v.v[0], v.v[V - 1]);
           }
-          h = pick(starts >> s & 1, u[s], fma(f[s], h, u[s]));
-          token(s);
+          v = pick(starts >> s & 1, u[s], fma(f[s], v, u[s]));
+          if (mine) *reinterpret_cast<Pack<T, V>*>(out + s * p.ldo) = pack<T, V>(v.v);
         }
       }
+      if (t0 + n == end) finish<V>(p, tables, end, false, c, mine, v.v[0], v.v[V - 1]);
+    }
+    if (!rejected) look(t0 + step, buf ^ 1);
+    // The round's outputs and the next one's gates together: what the exponentials' unit takes longest for lies beside the rest.  Outputs
+    // go through shared memory, in the places of the tokens that were read there.
+    Tokens &x = slice(round + 1 & 1, 0), &r = slice(round + 1 & 1, 1), &i = slice(round + 1 & 1, NT - 1);
+    if (ASYNC) {
+      copies_wait<1>();
+      __syncwarp();
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      h = fma(f[s], h, u[s]);
+      gates(s, x, r, i);
+      if constexpr (ASYNC) x.row[s][lane] = pack<T, V>(h.v);
+      else if (plain && mine) out[s * p.ldo] = from_float<T>(h.v[0]);
     }
     if constexpr (ASYNC) {
       __syncwarp();
-      y.store(p.out, p.ldo, t0, n, c0, p.C);
+      if (plain) Cursor<T, S>(p.out, p.ldo, t0, c0).store(x, g.y, S, chunk);
+      __syncwarp();
     }
-    if (!rejected && ((n > 0 && t0 + n == end) || (end == 0 && t0 == 0))) finish<V>(p, lower(p.seq, j, p.seq.N + 1, end), end, false, c, mine, h.v[0], h.v[V - 1]);
-    t0 += step;
-    slot = slot == DEPTH - 1 ? 0 : slot + 1;
+    if (plain && t0 + n == end) finish<V>(p, tables, end, false, c, mine, h.v[0], h.v[V - 1]);
+    ask(ASYNC ? 3 : 2, round + 1 & 1);
   }
-  if (rejected && rank == 0 && warp == 0) finish<V>(p, 1, 0, true, c, mine, 0.0f, 0.0f);
+  if (!rejected && end == 0 && rank == 0 && warp == 0) finish<V>(p, tables, 0, false, c, mine, 0.0f, 0.0f);
+  if (lost) report(p.seq.status, SEQ_LOST);
+  if (rejected && rank == 0 && warp == 0) finish<V>(p, tables, 0, true, c, mine, 0.0f, 0.0f);
   if (rejected || p.zero_pad) zero_rest<T, V>(p.out, p.ldo, end, p.seq.T, c, mine, rank, size);
 }
 
 template <typename T, bool ASYNC, bool POWER, bool GATED>
 cudaError_t launch_gates(const GatedScanParams& p, cudaStream_t stream) {
-  constexpr int V = CHANNELS<T, ASYNC>, S = TOKENS<T, ASYNC>;
+  constexpr int V = CHANNELS<T, ASYNC>, B = sizeof(T);
   const long long slabs = (p.C + 32 * V - 1) / (32 * V);
-  return launch_clusters(kda_gated_scan_kernel<T, ASYNC, POWER, GATED>, p, slabs, cluster_of(slabs, p.seq.T, WARPS * S),
-                         ASYNC ? DEPTH * WARPS * (GATED ? 3 : 2) * (int)sizeof(Slice<T, S>) : 0, stream);
+  constexpr int bytes = ASYNC ? DEPTH * WARPS * (GATED ? 3 : 2) * (int)sizeof(Slice<T, S>) : 0;
+  const auto kernel = kda_gated_scan_kernel<T, ASYNC, POWER, GATED>;
+  const int size = cluster_of(kernel, slabs, p.seq.T, TILE, THREADS, [](int) { return bytes; });
+  const Steps g = {4 * p.ldx * B, 4 * p.ldr * B, 4 * p.ldi * B, 4 * p.ldo * B};
+  return launch_clusters(kernel, slabs, size, THREADS, bytes, stream, p, g);
 }
 
 template <typename T, bool ASYNC>
@@ -316,7 +343,7 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_gated_scan_step_kernel(const
   for (int k = 0; k < VEC; k++) {
     rb[k] = mine ? bias_of<T>(p.r_bias, c + k) : 0.0f;
     ib[k] = mine && p.i != nullptr ? bias_of<T>(p.i_bias, c + k) : 0.0f;
-    k_[k] = POWER && mine ? decay_factor<T>(p.rate, c + k, p.rate_scale) : 0.0f;
+    k_[k] = POWER && mine ? decay_factor(p.rate, c + k, p.rate_scale) : 0.0f;
   }
   drop_repeats(p.seq, row0, slot);
   if (!mine) return;

@@ -15,15 +15,20 @@ namespace kda {
 
 namespace gscan {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int MAX_CLUSTER = 8;
-constexpr long long NEVER = 0x7fffffffffffffffLL;
+constexpr int MAX_CLUSTER = 8, MAX_DEVICES = 64;
+constexpr uint32_t WAIT_MS = 2000;
+constexpr uint32_t NEVER = 0xffffffffu;
 
 // A product of decays that underflows to zero is taken as the smallest positive number, so that an infinite state stays infinite, as it
 // does token by token (a finite one is not changed by that).  Where a decay is NaN, so is the map's constant.
 constexpr float LEAST = 1.4e-45f;
-constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
+constexpr float LOG2E_F = 1.4426950408889634f, LOG2E_REST = 1.925963033500e-8f, LN2_F = 0.6931471805599453f;
 
+__device__ __forceinline__ float sqrt_fast(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float rsqrt_fast(float x) {
   float y;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -40,22 +45,52 @@ __device__ __forceinline__ float bias_of(const float* p, int c) {
 // softplus in full precision, once a channel
 __device__ __forceinline__ float softplus_exact(float x) { return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))); }
 
-// The decay's factor in front of s: -c softplus(rate), for 16-bit tokens in powers of two; finite, since an infinite one times s = 0 would
+// The decay's factor in front of s, to base 2: -c softplus(rate) log2(e); finite, since an infinite one times s = 0 would
 // be NaN.
-template <typename T>
 __device__ __forceinline__ float decay_factor(const float* rate, int c, float scale) {
-  const float k = -scale * softplus_exact(rate[c]) * (sizeof(T) == 4 ? 1.0f : LOG2E_F);
+  const float k = -scale * softplus_exact(rate[c]) * LOG2E_F;
   return k < -3.0e38f ? -3.0e38f : k;
 }
 
 // ---- sequences
-// Called by a warp: the first of the entries [lo, hi) that is >= t, hi where none is.  32 entries are looked at at a time.
-__device__ __forceinline__ int lower(const SeqTable& s, int lo, int hi, long long t) {
+// A block's view of the tables: where they are short, copies in shared memory, so that a slice in which sequences meet does not wait for one
+// load after the other.  (The rounds of a cluster wait for its slowest block.)
+constexpr int TABLE = 256;
+template <bool SLOTS>
+struct Tables {
+  int cu[SLOTS ? TABLE : TABLE / 2], slot[SLOTS ? TABLE : 1];          // slot: -1 out of range
+};
+template <bool SLOTS>
+struct Layout {
+  const SeqTable& s;
+  const Tables<SLOTS>* copy;             // nullptr: read where they lie
+  __device__ __forceinline__ uint32_t at(int i) const { return copy != nullptr ? (uint32_t)copy->cu[i] : (uint32_t)cu_at(s, i); }
+  __device__ __forceinline__ int slot_of(int i) const {
+    if (SLOTS && copy != nullptr) return copy->slot[i];
+    const long long d = s.slots != nullptr ? table_at(s.slots, s.slots_is64, i) : i;
+    return d < 0 || d >= s.n_slots ? -1 : (int)d;
+  }
+};
+// Called by the whole block, which meets a barrier before it uses the copy.  Not for a layout that is rejected.
+template <bool SLOTS>
+__device__ __forceinline__ Layout<SLOTS> layout_of(const SeqTable& s, Tables<SLOTS>& copy) {
+  const Layout<SLOTS> direct = {s, nullptr};
+  if (s.N >= (int)(sizeof(copy.cu) / sizeof(int))) return direct;
+  for (int i = threadIdx.x; i <= s.N; i += blockDim.x) {
+    copy.cu[i] = (int)cu_at(s, i);
+    if (SLOTS) copy.slot[i] = i < s.N ? direct.slot_of(i) : -1;
+  }
+  return {s, &copy};
+}
+
+// Called by a warp: the first of the entries [lo, hi) of cu_seqlens that is >= t, hi where none is.  32 entries are looked at at a time.
+template <bool SLOTS>
+__device__ __forceinline__ int lower(const Layout<SLOTS>& l, int lo, int hi, uint32_t t) {
   const int lane = threadIdx.x % 32;
   while (lo < hi) {
     const int part = (hi - lo + 31) / 32;
     const long long at = (long long)lo + (long long)(lane + 1) * part - 1;
-    const unsigned found = __ballot_sync(0xffffffffu, cu_at(s, at < hi ? at : hi - 1) >= t);
+    const unsigned found = __ballot_sync(0xffffffffu, l.at(at < hi ? (int)at : hi - 1) >= t);
     if (found == 0) return hi;
     const int first = __ffs(found) - 1;
     hi = min(hi - 1, lo + (first + 1) * part - 1);
@@ -65,14 +100,15 @@ __device__ __forceinline__ int lower(const SeqTable& s, int lo, int hi, long lon
 }
 
 // Called by a warp: the slot of sequence i, or -1 where its entry is out of range or repeats an earlier one
-__device__ __forceinline__ long long claim(const SeqTable& s, int i) {
-  if (s.slots == nullptr) return i;
-  const long long d = table_at(s.slots, s.slots_is64, i);
-  int bad = d < 0 || d >= s.n_slots;
+template <bool SLOTS>
+__device__ __forceinline__ long long claim(const Layout<SLOTS>& l, int i) {
+  if (l.s.slots == nullptr) return i;
+  const int d = l.slot_of(i);
+  int bad = d < 0;
   for (int j = threadIdx.x % 32; j < i && !bad; j += 32)
-    if (table_at(s.slots, s.slots_is64, j) == d) bad = 1;
+    if (l.slot_of(j) == d) bad = 1;
   if (!__any_sync(0xffffffffu, bad)) return d;
-  if (threadIdx.x % 32 == 0) report(s.status, SEQ_BAD_SLOT);
+  if (threadIdx.x % 32 == 0) report(l.s.status, SEQ_BAD_SLOT);
   return -1;
 }
 
@@ -89,19 +125,45 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// at the address of `own` in another block
-__device__ __forceinline__ void put_remote(const void* own, uint32_t rank, float4 v) {
-  const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
-  asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.v4.f32 [t], {%2, %3, %4, %5};\n}" ::"r"(a), "r"(rank), "f"(v.x),
-               "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+// Values for another block, at the address of `own` there; they count towards the bytes that its barrier (at the address of `bar`) waits
+// for.  No fence: a barrier of the cluster with release would wait for the block's outputs to be in memory, 1.4 of 5 cycles a warp
+// spent per instruction.
+__device__ __forceinline__ void send(const void* own, const void* bar, uint32_t rank, float4 v) {
+  const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own)), b = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
+  asm volatile("{\n .reg .b32 t, u;\n mapa.shared::cluster.u32 t, %0, %2;\n mapa.shared::cluster.u32 u, %1, %2;\n"
+               " st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [t], {%3, %4, %5, %6}, [u];\n}" ::"r"(a), "r"(b), "r"(rank), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ void put_remote(const void* own, uint32_t rank, float v) {
   const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
   asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.f32 [t], %2;\n}" ::"r"(a), "r"(rank), "f"(v) : "memory");
 }
-__device__ __forceinline__ void put_remote(const void* own, uint32_t rank, uint32_t v) {
-  const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(own));
-  asm volatile("{\n .reg .b32 t;\n mapa.shared::cluster.u32 t, %0, %1;\n st.shared::cluster.u32 [t], %2;\n}" ::"r"(a), "r"(rank), "r"(v) : "memory");
+__device__ __forceinline__ void bar_init(const void* bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void bar_expect(const void* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(bar))), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_done(uint32_t b, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred q;\n mbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n selp.u32 %0, 1, 0, q;\n}" : "=r"(done) : "r"(b), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint32_t milliseconds() {     // about; wraps
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return (uint32_t)(t >> 20);
+}
+// False where two seconds ran out: what comes then is wrong, and ends
+__device__ __forceinline__ bool bar_wait(const void* bar, uint32_t parity) {
+  const uint32_t b = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
+  if (bar_done(b, parity)) return true;
+  const uint32_t begin = milliseconds();
+  while (!bar_done(b, parity))
+    if (milliseconds() - begin > WAIT_MS) return false;
+  return true;
 }
 
 // ---- one or two channels at once (two: one instruction)
@@ -156,41 +218,62 @@ template <typename T, bool ASYNC>
 constexpr int CHANNELS = ASYNC ? 4 / (int)sizeof(T) : 1;
 
 template <int S>
-__device__ __forceinline__ int count(long long t0, long long end) {        // tokens of the slice at t0
-  const long long n = end - t0;
-  return n < 0 ? 0 : (n > S ? S : (int)n);
+__device__ __forceinline__ int count(uint32_t t0, uint32_t end) {          // tokens of the slice at t0
+  return t0 >= end ? 0 : (end - t0 > S ? S : (int)(end - t0));
 }
 
-// A warp's slice of one tensor.  ASYNC: S rows of 128 bytes in shared memory, by copies of 16 bytes that are asked for rounds ahead;
-// places behind the last token or channel are zeros.  Otherwise S registers, asked for a round ahead.
+// A warp's slice of one tensor in shared memory: S rows of 128 bytes, which come and go in 16 bytes a lane.  Places behind the last token or
+// channel are zeros.
 template <typename T, int S>
 struct Slice {
   Pack<T, 4 / sizeof(T)> row[S][32];
+};
+// Strides in bytes that a launch works out for a tensor: of four rows, of a round
+struct Strides {
+  long long four, round;
+};
+inline Strides strides(long long ld, int size, long long round) { return {4 * ld * size, round * ld * size}; }
 
-  __device__ __forceinline__ void ask(const void* base, long long ld, long long t0, int n, int c0, int C) {
-    const int lane = threadIdx.x % 32, chunk = lane % 8;
-    const int c = c0 + chunk * (16 / (int)sizeof(T));
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(this)) + (uint32_t)(lane / 8 * 128 + chunk * 16);
-    const T* from = reinterpret_cast<const T*>(base) + (t0 + lane / 8) * ld + c;
+// Where a lane's 16 bytes of a slice lie in memory: a row's, four rows on, ...
+template <typename T, int S>
+struct Cursor {
+  const char* at;
+  __device__ __forceinline__ Cursor(const void* base, long long ld, long long t0, int c0) {
+    at = reinterpret_cast<const char*>(reinterpret_cast<const T*>(base) + (t0 + (int)(threadIdx.x % 32 / 8)) * ld + c0 + (int)(threadIdx.x % 8) * (16 / (int)sizeof(T)));
+  }
+  // n rows (`on`: the lane's channels exist) into a slice
+  __device__ __forceinline__ void ask(Slice<T, S>& to, long long four, int n, bool on, const void* valid) const {
+    const int row = threadIdx.x % 32 / 8;
+    const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(&to)) + (uint32_t)(threadIdx.x % 32 * 16);
+    const char* from = at;
+    if (n == S && on) {
 #pragma unroll
-    for (int q = 0; q < S / 4; q++) {
-      const bool on = c < C && lane / 8 + 4 * q < n;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + 512u * q), "l"(on ? (const void*)from : base), "r"(on ? 16 : 0) : "memory");
-      from += 4 * ld;
+      for (int q = 0; q < S / 4; q++) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a + 512u * q), "l"(from) : "memory");
+        from += four;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < S / 4; q++) {
+        const bool here = on && row + 4 * q < n;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a + 512u * q), "l"(here ? (const void*)from : valid), "r"(here ? 16 : 0) : "memory");
+        from += four;
+      }
     }
   }
-  // the first n rows to memory; the warp has written them
-  __device__ __forceinline__ void store(void* base, long long ld, long long t0, int n, int c0, int C) const {
-    const int lane = threadIdx.x % 32, chunk = lane % 8;
-    const int c = c0 + chunk * (16 / (int)sizeof(T));
-    T* to = reinterpret_cast<T*>(base) + (t0 + lane / 8) * ld + c;
+  // the first n rows of a slice, which the warp has written, to memory
+  __device__ __forceinline__ void store(const Slice<T, S>& from, long long four, int n, bool on) const {
+    const int row = threadIdx.x % 32 / 8;
+    const uint4* a = reinterpret_cast<const uint4*>(&from) + threadIdx.x % 32;
+    char* to = const_cast<char*>(at);
 #pragma unroll
     for (int q = 0; q < S / 4; q++) {
-      if (c < C && lane / 8 + 4 * q < n) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(this) + lane / 8 * 128 + chunk * 16 + 512 * q);
-      to += 4 * ld;
+      if (on && row + 4 * q < n) *reinterpret_cast<uint4*>(to) = a[32 * q];
+      to += four;
     }
   }
 };
+// One channel a lane, read one by one a round ahead
 template <typename T, int S>
 struct Registers {
   T row[S];
@@ -223,65 +306,107 @@ __device__ __forceinline__ Vec<V> values(const Pack<T, V>& p) {
   for (int k = 0; k < V; k++) r.v[k] = to_float(p.v[k]);
   return r;
 }
+template <>
+__device__ __forceinline__ Vec<2> values(const Pack<__nv_bfloat16, 2>& p) {      // one instruction each
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(&p);
+  return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
 
-// Of V channels: sigmoid and 1 minus it
-template <typename T, int V>
+// Of V channels: sigmoid and, with BOTH, 1 minus it, both to relative accuracy.  The approximate exponential and reciprocal are good to
+// 2^-22; for 32-bit tokens the exponential's argument is taken in two parts, since its rounding would be off by as much again for each unit of x.
+template <typename T, int V, bool BOTH = true>
 __device__ __forceinline__ void sigmoids(Vec<V> x, Vec<V> bias, Vec<V>& s, Vec<V>& n) {
-  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int k = 0; k < V; k++) sigmoid_pair<T>(x.v[k], bias.v[k], s.v[k], n.v[k]);
-  } else {
-    Vec<V> e = fma(x, vec<V>(-LOG2E_F), bias);
-#pragma unroll
-    for (int k = 0; k < V; k++) e.v[k] = ex2_fast(min_or_nan(e.v[k], 126.0f));
-    s = add(e, vec<V>(1.0f));
-#pragma unroll
-    for (int k = 0; k < V; k++) s.v[k] = rcp_fast(s.v[k]);
-    n = mul(e, s);
+  for (int k = 0; k < V; k++) {
+    float e;
+    if constexpr (sizeof(T) == 4) {
+      const float v = -(x.v[k] + bias.v[k]), hi = min_or_nan(v * LOG2E_F, 126.0f);
+      const float lo = fmaf(v, LOG2E_F, -hi) + v * LOG2E_REST;
+      e = ex2_fast(hi);
+      e = fabsf(hi) < 126.0f ? fmaf(e, lo * LN2_F, e) : e;
+    } else {
+      const float t = fmaf(x.v[k], -LOG2E_F, bias.v[k]);
+      e = ex2_fast(BOTH ? min_or_nan(t, 126.0f) : t);
+    }
+    s.v[k] = rcp_fast(e + 1.0f);
+    n.v[k] = BOTH ? e * s.v[k] : 0.0f;
   }
 }
 
-// A token's values.  `l` (POWER) is log f, natural for 32-bit tokens, else base 2; s, n: of the decay's gate; inv: 1 / gain.
+// 1 - f^2 for f = 2^l, l <= 0: near zero by a polynomial for (1 - 2^(2 l)) / l on [-0.36, 0] (relative minimax, found by linear programming, with
+// its roundings 1.9e-7 off in fp32), as the difference would lose its digits there
+template <int V>
+__device__ __forceinline__ Vec<V> one_minus_square(Vec<V> l, Vec<V> f) {
+  Vec<V> r;
+#pragma unroll
+  for (int k = 0; k < V; k++) {                      // single values: pairs of constants would take registers, or moves
+    const float a = l.v[k];
+    float q = fmaf(a, -0.03467162698507309f, -0.15143901109695435f);
+    q = fmaf(a, q, -0.44371989369392395f);
+    q = fmaf(a, q, -0.9608919620513916f);
+    q = fmaf(a, q, -1.3862942457199097f);
+    r.v[k] = a > -0.36f ? q * a : fmaf(-f.v[k], f.v[k], 1.0f);
+  }
+  return r;
+}
+
+// A token's values.  `l` (POWER) is log f to base 2; s, n: of the decay's gate; inv: 1 / gain.  What only gradients need comes with GRAD.
 template <int V>
 struct Gates {
   Vec<V> f, gain, s, n, l, inv;
 };
-template <typename T, bool POWER, int V>
+template <typename T, bool POWER, int V, bool GRAD = false>
 __device__ __forceinline__ Gates<V> decay(Vec<V> r, Vec<V> bias, Vec<V> k_) {
   Gates<V> a;
-  sigmoids<T, V>(r, bias, a.s, a.n);
+  sigmoids<T, V, GRAD || !POWER>(r, bias, a.s, a.n);
   if constexpr (!POWER) {
     a.f = a.s; a.gain = a.n; a.l = a.inv = vec<V>(0.0f);
   } else {
     a.l = mul(k_, a.s);
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int k = 0; k < V; k++) {
-        a.f.v[k] = expf(a.l.v[k]);
-        a.gain.v[k] = sqrtf(-expm1f(2.0f * a.l.v[k]));
-        a.inv.v[k] = 1.0f / fmaxf(a.gain.v[k], 1.0e-19f);
-      }
-    } else {
+    for (int k = 0; k < V; k++) a.f.v[k] = ex2_fast(a.l.v[k]);
+    const Vec<V> q = one_minus_square(a.l, a.f);
 #pragma unroll
-      for (int k = 0; k < V; k++) a.f.v[k] = ex2_fast(a.l.v[k]);
-      // 1 - f^2 = -(e^y - 1), y = 2 ln2 l <= 0: near zero by a polynomial for (e^y - 1) / y on [-1/2, 0] (relative minimax, found by linear
-      // programming, 1.0e-7 off in fp32), as the difference would lose its digits there
-      const Vec<V> y = mul(a.l, vec<V>(2.0f * LN2_F));
-      Vec<V> q = fma(y, vec<V>(0.006771687883883715f), vec<V>(0.0410030297935009f));
-      q = fma(y, q, vec<V>(0.1665491908788681f));
-      q = fma(y, q, vec<V>(0.4999926686286926f));
-      q = fma(y, q, vec<V>(0.9999999403953552f));
-      q = mul(q, y);
-      const Vec<V> d = fma(a.f, a.f, vec<V>(-1.0f));
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        const float m = y.v[k] > -0.5f ? -q.v[k] : -d.v[k];
-        a.inv.v[k] = rsqrt_fast(fmaxf(m, 1.0e-38f));     // l times it is 0 where l is
-        a.gain.v[k] = m * a.inv.v[k];
+    for (int k = 0; k < V; k++) {
+      if (GRAD) {
+        a.inv.v[k] = rsqrt_fast(fmaxf(q.v[k], 1.0e-38f));      // l times it is 0 where l is
+        a.gain.v[k] = q.v[k] * a.inv.v[k];
+      } else {
+        a.gain.v[k] = sqrt_fast(q.v[k]);
       }
     }
   }
   return a;
+}
+
+// A token's decay f and term u.  With both gates in 16 bits u = sqrt(q) / (1 + e^-i) x, q = 1 - f^2, takes one reciprocal root,
+// sqrt(q) / a = q rsqrt(q a^2): five operations of the special-function unit instead of six.  (An input gate below 2^-60 counts as that.)
+template <typename T, bool POWER, bool GATED, int V>
+__device__ __forceinline__ void token_terms(Vec<V> x, Vec<V> r, Vec<V> i, Vec<V> rb, Vec<V> ib, Vec<V> k_, Vec<V>& f, Vec<V>& u) {
+  if constexpr (POWER && GATED && sizeof(T) == 2) {
+    Vec<V> s, n;
+    sigmoids<T, V, false>(r, rb, s, n);
+    const Vec<V> l = mul(k_, s);
+#pragma unroll
+    for (int k = 0; k < V; k++) f.v[k] = ex2_fast(l.v[k]);
+    const Vec<V> q = one_minus_square(l, f);
+    Vec<V> w;
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+      const float a = ex2_fast(min_or_nan(fmaf(i.v[k], -LOG2E_F, ib.v[k]), 60.0f)) + 1.0f;
+      w.v[k] = rsqrt_fast(fmaf(q.v[k] * a, a, 1.0e-38f));
+    }
+    u = mul(mul(q, w), x);
+  } else {
+    const Gates<V> a = decay<T, POWER, V>(r, rb, k_);
+    f = a.f;
+    u = mul(a.gain, x);
+    if constexpr (GATED) {
+      Vec<V> g, n;
+      sigmoids<T, V, false>(i, ib, g, n);
+      u = mul(u, g);
+    }
+  }
 }
 
 // Rows [end, T) of an output are zeros, spread over the blocks of a cluster
@@ -291,36 +416,56 @@ __device__ __forceinline__ void zero_rest(void* out, long long ld, long long end
 #pragma unroll
   for (int k = 0; k < V; k++) zero.v[k] = from_float<T>(0.0f);
   if (mine)
-    for (long long t = end + rank * WARPS + threadIdx.x / 32; t < T_; t += size * WARPS)
+    for (long long t = end + rank * (blockDim.x / 32) + threadIdx.x / 32; t < T_; t += size * (blockDim.x / 32))
       *reinterpret_cast<Pack<T, V>*>(reinterpret_cast<T*>(out) + c + t * ld) = zero;
 }
 
-// Blocks along time: as many as give the card two blocks an SM, no more than the batch has tiles
-inline int cluster_of(long long slabs, long long T, int tile) {
-  int size = 1;
-  while (size < MAX_CLUSTER && slabs * size * 2 <= 2 * 148 && (long long)size * tile < T) size *= 2;
-  return size;
-}
-
-template <typename K, typename P>
-cudaError_t launch_clusters(K kernel, const P& p, long long slabs, int size, int bytes, cudaStream_t stream) {
-  if (slabs * size > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(slabs * size));
-  cfg.blockDim = dim3(THREADS);
+inline void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, long long blocks, int size, int threads, int bytes, cudaStream_t stream) {
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)bytes;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)size;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// Blocks along time: as many as the card holds at once for all slabs, no more than the batch has tiles.  A cluster lies within one of
+// the card's groups of SMs, so the sizes that fit are asked for (once for a kernel and device).
+template <typename K, typename B>
+int cluster_of(K kernel, long long slabs, long long T, int tile, int threads, B bytes) {
+  static int room[MAX_DEVICES][MAX_CLUSTER + 1];     // clusters of a size that run at once, plus one; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= MAX_DEVICES) return 1;
+  int best = 1;
+  for (int size = 2; size <= MAX_CLUSTER && (long long)(size - 1) * tile < T; size++) {
+    if (room[dev][size] == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      configure(cfg, attr, size, size, threads, bytes(size), nullptr);
+      int n = 0;
+      if (bytes(size) > 0) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(size));
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+      room[dev][size] = n + 1;
+    }
+    if (slabs <= room[dev][size] - 1) best = size;
+  }
+  return best;
+}
+
+template <typename K, typename... P>
+cudaError_t launch_clusters(K kernel, long long slabs, int size, int threads, int bytes, cudaStream_t stream, const P&... p) {
+  if (slabs * size > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (bytes > 0) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  configure(cfg, attr, slabs * size, size, threads, bytes, stream);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -15,314 +15,302 @@ namespace {
 
 using namespace gscan;
 
+constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int DEPTH = 2;                 // rounds of tokens on their way or worked on
-constexpr int S = 8, TILE = WARPS * S;   // tokens of a slice, of a block
+constexpr int S = 12, TILE = WARPS * S;  // tokens of a slice, of a block
 static_assert(TILE == GATED_SCAN_TILE, "the forward pass keeps the states in front of the tiles");
 
+// Two blocks an SM leave 17 KB beside the tokens of 16-bit calls.
 template <int V>
 struct Shared {
-  Vec<4> map[2][WARPS][V][32];           // {F, U, G, -} of a channel
-  float4 tile[2][MAX_CLUSTER][32];       // of the cluster's tiles, written by their blocks: {F, F, G, G}
-  uint32_t starts[2][WARPS], tile_starts[2][MAX_CLUSTER];
-  float tile_sums[3][MAX_CLUSTER][V][32];
+  Vec<V> F[2][WARPS][32], U[2][WARPS][32], G[2][WARPS][32];          // the maps of the block's slices
+  unsigned long long sent[2];            // barriers: the tiles' maps have arrived
+  uint32_t cuts[2][WARPS];               // tokens that start a sequence, from bit 16 on those that end one: the maps are constant
+  Tables<false> tables;
+};
+using Tile = float4[32];                 // of the cluster's tiles, sent by their blocks: {F, F, G, G}; F < 0: the map is constant
+
+struct Steps {             // bytes from a row to the fourth behind it
+  long long x, r, i, d, dx, dr, di;
 };
 
 template <typename T, bool ASYNC, bool POWER, bool GATED>
-__global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const __grid_constant__ GatedScanGradParams p) {
+__global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const __grid_constant__ GatedScanGradParams p, const __grid_constant__ Steps g) {
   constexpr int V = CHANNELS<T, ASYNC>, NT = GATED ? 4 : 3;
-  __shared__ Shared<V> sm;
-  extern __shared__ __align__(128) unsigned char raw[];              // ASYNC: [DEPTH][WARPS][NT] slices
   using Tokens = Slice<T, S>;
+  constexpr int RAW = ASYNC ? DEPTH * WARPS * NT * (int)sizeof(Tokens) : 0;
+  __shared__ Shared<V> sm;
+  extern __shared__ __align__(128) unsigned char raw[];              // ASYNC: [DEPTH][WARPS][NT] slices; then [2][blocks of the cluster] tiles
   const uint32_t rank = cluster_rank(), size = cluster_size();
+  Tile* const tiles = reinterpret_cast<Tile*>(raw + RAW);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int c0 = (int)(blockIdx.x / size) * 32 * V, c = c0 + lane * V;
-  const bool mine = c < p.C;
+  const bool mine = c < p.C, chunk = c0 + lane % 8 * (16 / (int)sizeof(T)) < p.C;
+  if (threadIdx.x == 0)
+    for (int b = 0; b < 2; b++) bar_init(&sm.sent[b]);
   if (size > 1) cluster_arrive();
   const bool rejected = cu_rejected(p.seq);
-  const long long end = rejected ? 0 : cu_at(p.seq, p.seq.N);
-  const long long step = (long long)size * TILE;
-  const int rounds = (int)((end + step - 1) / step);
+  const Layout<false> tables = rejected ? Layout<false>{p.seq, nullptr} : layout_of(p.seq, sm.tables);
+  const uint32_t end = rejected ? 0 : (uint32_t)cu_at(p.seq, p.seq.N);
+  const uint32_t step = size * TILE;
+  const int rounds = (int)(((long long)end + step - 1) / step);
+  __syncthreads();                                   // the copies of the tables
 
-  long long t0 = (rounds - 1) * step + (long long)rank * TILE + warp * S;
-  Registers<T, S> nx, nr, ni, nd;
+  uint32_t t0 = (uint32_t)(rounds - 1) * step + rank * TILE + warp * S;        // not used without rounds
+  Registers<T, S> rx, rr, ri, rd;
   Vec<V> next_enter = vec<V>(0.0f);
   auto slice = [&](int slot, int k) -> Tokens& { return reinterpret_cast<Tokens*>(raw)[(slot * WARPS + warp) * NT + k]; };
-  auto ask = [&](int ahead, int slot) {              // the tokens of a later round, which lie in front of this one's
-    const long long t = t0 - ahead * step;
-    const int m = t >= 0 ? count<S>(t, end) : 0;
+  auto ask = [&](int round, int slot) {              // the tokens of a round
+    const uint32_t t = (uint32_t)round * step + rank * TILE + warp * S;
+    const int m = round >= 0 ? count<S>(t, end) : 0;
     if constexpr (ASYNC) {
       if (m > 0) {
-        slice(slot, 0).ask(p.x, p.ldx, t, m, c0, p.C);
-        slice(slot, 1).ask(p.r, p.ldr, t, m, c0, p.C);
-        if (p.dy != nullptr) slice(slot, 2).ask(p.dy, p.lddy, t, m, c0, p.C);
-        if (GATED) slice(slot, 3).ask(p.i, p.ldi, t, m, c0, p.C);
+        Cursor<T, S>(p.x, p.ldx, t, c0).ask(slice(slot, 0), g.x, m, chunk, p.x);
+        Cursor<T, S>(p.r, p.ldr, t, c0).ask(slice(slot, 1), g.r, m, chunk, p.r);
+        if (p.dy != nullptr) Cursor<T, S>(p.dy, p.lddy, t, c0).ask(slice(slot, 2), g.d, m, chunk, p.dy);
+        if (GATED) Cursor<T, S>(p.i, p.ldi, t, c0).ask(slice(slot, 3), g.i, m, chunk, p.i);
       }
       copies_commit();
     } else if (m > 0) {
-      nx.ask(p.x, p.ldx, t, m, c, p.C);
-      nr.ask(p.r, p.ldr, t, m, c, p.C);
-      if (p.dy != nullptr) nd.ask(p.dy, p.lddy, t, m, c, p.C);
-      if (GATED) ni.ask(p.i, p.ldi, t, m, c, p.C);
+      rx.ask(p.x, p.ldx, t, m, c, p.C);
+      rr.ask(p.r, p.ldr, t, m, c, p.C);
+      if (p.dy != nullptr) rd.ask(p.dy, p.lddy, t, m, c, p.C);
+      if (GATED) ri.ask(p.i, p.ldi, t, m, c, p.C);
     }
-  };
-  auto ask_state = [&](int ahead) {                  // the state in front of the tile
-    const long long t = t0 - ahead * step;
 #pragma unroll
-    for (int k = 0; k < V; k++)
-      if (mine && t >= 0 && t < end) next_enter.v[k] = p.tiles[t / TILE * p.C + c + k];
+    for (int k = 0; k < V; k++)                      // the state in front of the tile
+      if (mine && m > 0) next_enter.v[k] = p.tiles[(long long)(t / TILE) * p.C + c + k];
   };
-#pragma unroll
-  for (int k = 0; k < (ASYNC ? DEPTH - 1 : 1); k++) ask(k, k);
-  ask_state(0);
+  ask(rounds - 1, 0);
   Vec<V> rb, ib, k_;
 #pragma unroll
   for (int k = 0; k < V; k++) {
     rb.v[k] = mine ? bias_of<T>(p.r_bias, c + k) : 0.0f;
     ib.v[k] = GATED && mine ? bias_of<T>(p.i_bias, c + k) : 0.0f;
-    k_.v[k] = POWER && mine ? decay_factor<T>(p.rate, c + k, p.rate_scale) : 0.0f;
+    k_.v[k] = POWER && mine ? decay_factor(p.rate, c + k, p.rate_scale) : 0.0f;
   }
   // the gradients of empty sequences' states pass through; a rejected layout has no others
   if (p.dsrc != nullptr && rank == 0) {
     for (int q = warp; q < p.seq.N; q += WARPS) {
-      if (!rejected && cu_at(p.seq, q) != cu_at(p.seq, q + 1)) continue;
+      if (!rejected && tables.at(q) != tables.at(q + 1)) continue;
 #pragma unroll
       for (int k = 0; k < V; k++)
         if (mine) p.dsrc[(long long)q * p.C + c + k] = p.dfinal != nullptr ? p.dfinal[(long long)q * p.C + c + k] : 0.0f;
     }
   }
-  int j = p.seq.N + 1;                               // first entry of cu_seqlens that is >= t0, once looked for
-  long long below = NEVER;                           // the entry in front of that one
+  auto state = [&](const float* table, uint32_t t) {  // of the sequence that token t belongs to; zeros without a table
+    Vec<V> h = vec<V>(0.0f);
+    if (table == nullptr) return h;
+    const int q = lower(tables, 0, p.seq.N + 1, t + 1) - 1;
+#pragma unroll
+    for (int k = 0; k < V; k++)
+      if (mine) h.v[k] = table[(long long)q * p.C + c + k];
+    return h;
+  };
+  uint32_t below = NEVER;                            // the last entry of cu_seqlens in front of the slices that are done
   Vec<V> carry = vec<V>(0.0f), sum_rate = vec<V>(0.0f), sum_r = vec<V>(0.0f), sum_i = vec<V>(0.0f);
+  bool lost = false;
   if (size > 1) cluster_wait();
 
-  int slot = 0;
-  for (int round = rounds - 1; round >= 0; round--) {
-    const int buf = round & 1, n = count<S>(t0, end);
-    // entries in [t0, t0 + n]: sequences end in front of them or start there
-    bool touched = false;
-    if (below >= t0) {
-      j = lower(p.seq, 0, j, t0);
-      below = j > 0 ? cu_at(p.seq, j - 1) : -1;
-      touched = n > 0 && j <= p.seq.N && cu_at(p.seq, j) <= t0 + n;
-    }
-    Registers<T, S> rx, rr, ri, rd;
+  for (int round = rounds - 1; round >= 0; round--, t0 -= step) {
+    const int use = rounds - 1 - round, buf = use & 1, n = count<S>(t0, end);
+    if (size > 1 && threadIdx.x == 0) bar_expect(&sm.sent[buf], size * 512);
+    Vec<V> h = next_enter;
     if constexpr (ASYNC) {
-      copies_wait<DEPTH - 2>();
+      copies_wait<0>();
       __syncwarp();
-      ask(DEPTH - 1, slot == 0 ? DEPTH - 1 : slot - 1);
-    } else {
-      rx = nx; rr = nr; ri = ni; rd = nd;
-      ask(1, 0);
+      ask(round - 1, buf ^ 1);
     }
-    Vec<V> enter = next_enter;
-    ask_state(1);
+    // entries in [t0, t0 + n]: sequences start there, or end in front of them
+    uint32_t starts = 0, ends = 0;
+    if (below >= t0) {
+      const int j = lower(tables, 0, p.seq.N + 1, t0);
+      below = j > 0 ? tables.at(j - 1) : 0;
+      if (j == 0) below = 0;
+      for (int q = j; q <= p.seq.N; q++) {
+        const uint32_t t = tables.at(q);
+        if (t > t0 + n) break;
+        if (t < t0 + n) starts |= 1u << (t - t0);
+        if (t > t0) ends |= 1u << (t - t0 - 1);
+      }
+    }
     auto token = [&](int k, int s) {                 // 0: x, 1: r, 2: dy, 3: i
-      if constexpr (ASYNC) return values(slice(slot, k).row[s][lane]);
+      if constexpr (ASYNC) return values(slice(buf, k).row[s][lane]);
       else return vec<V>(to_float(k == 0 ? rx.row[s] : k == 1 ? rr.row[s] : k == 2 ? rd.row[s] : ri.row[s]));
     };
-    Vec<V> f[S], u[S], d[S];                         // u: terms, then states in front of the tokens
+    auto gradient = [&](int s) { return p.dy != nullptr ? token(2, s) : vec<V>(0.0f); };
+    Vec<V> f[S], u[S];                               // decays; terms, then states in front of the tokens
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      const Gates<V> a = decay<T, POWER, V>(token(1, s), rb, k_);
-      f[s] = a.f;
-      u[s] = mul(a.gain, token(0, s));
-      if constexpr (GATED) {
-        Vec<V> g, ng;
-        sigmoids<T, V>(token(3, s), ib, g, ng);
-        u[s] = mul(u[s], g);
-      }
-      d[s] = p.dy != nullptr ? token(2, s) : vec<V>(0.0f);
-    }
-    if (n < S) {
-#pragma unroll
-      for (int s = 0; s < S; s++)
-        if (s >= n) { f[s] = vec<V>(1.0f); u[s] = d[s] = vec<V>(0.0f); }
-    }
-    // a sequence's final state is its last token's: so is the gradient
-    uint32_t starts = 0;
-    if (touched) {
-      for (int q = j; q <= p.seq.N; q++) {
-        const long long t = cu_at(p.seq, q);
-        if (t > t0 + n) break;
-        const int at = (int)(t - t0);
-        if (q > 0 && at > 0 && p.dfinal != nullptr && cu_at(p.seq, q - 1) < t) {
-          Vec<V> v = vec<V>(0.0f);
-#pragma unroll
-          for (int k = 0; k < V; k++)
-            if (mine) v.v[k] = p.dfinal[(long long)(q - 1) * p.C + c + k];
-#pragma unroll
-          for (int s = 0; s < S; s++)
-            if (s + 1 == at) d[s] = add(d[s], v);
-        }
-        if (at < n && q < p.seq.N && cu_at(p.seq, q + 1) > t) starts |= 1u << at;
-      }
-    }
-    auto entering = [&](int at, Vec<V>& h) {         // the initial state of the sequence that starts at that token
-      int q = lower(p.seq, j, p.seq.N + 1, t0 + at);
-      while (cu_at(p.seq, q + 1) == t0 + at) q++;
-#pragma unroll
-      for (int k = 0; k < V; k++) h.v[k] = mine && p.src != nullptr ? p.src[(long long)q * p.C + c + k] : 0.0f;
-      return q;
-    };
+    for (int s = 0; s < S; s++) token_terms<T, POWER, GATED, V>(token(0, s), token(1, s), token(3, s), rb, ib, k_, f[s], u[s]);
     // the slice's maps, forwards and backwards
     Vec<V> F = vec<V>(1.0f), U = vec<V>(0.0f), G = vec<V>(0.0f);
+    if (n == S && (starts | ends) == 0) {
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      if (starts >> s & 1) entering(s, U);
-      U = fma(f[s], U, u[s]);
-      F = mul(F, f[s]);
-    }
+      for (int s = 0; s < S; s++) {
+        U = fma(f[s], U, u[s]);
+        F = mul(F, f[s]);
+      }
 #pragma unroll
-    for (int s = S - 1; s >= 0; s--) {
-      G = mul(f[s], add(d[s], G));
-      if (starts >> s & 1) G = vec<V>(0.0f);
+      for (int s = S - 1; s >= 0; s--) G = mul(f[s], add(gradient(s), G));
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        if (s >= n) { f[s] = vec<V>(1.0f); u[s] = vec<V>(0.0f); }
+        if (starts >> s & 1) U = state(p.src, t0 + s);
+        U = fma(f[s], U, u[s]);
+        F = mul(F, f[s]);
+      }
+#pragma unroll
+      for (int s = S - 1; s >= 0; s--) {
+        if (ends >> s & 1) G = state(p.dfinal, t0 + s);
+        if (s < n) G = mul(f[s], add(gradient(s), G));
+      }
     }
     F = least(F);
-#pragma unroll
-    for (int k = 0; k < V; k++) sm.map[buf][warp][k][lane] = {F.v[k], U.v[k], G.v[k], 0.0f};
-    if (lane == 0) sm.starts[buf][warp] = starts;
-    const bool some = __syncthreads_or(starts != 0);
-    auto slice_map = [&](int w, Vec<V>& Fw, Vec<V>& Uw, Vec<V>& Gw) {
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        const Vec<4> m = sm.map[buf][w][k][lane];
-        Fw.v[k] = m.v[0]; Uw.v[k] = m.v[1]; Gw.v[k] = m.v[2];
-      }
-    };
-    Vec<V> h = enter, Fb = vec<V>(1.0f), Gb = vec<V>(0.0f);
+    sm.F[buf][warp][lane] = F;
+    sm.U[buf][warp][lane] = U;
+    sm.G[buf][warp][lane] = G;
+    if (lane == 0) sm.cuts[buf][warp] = starts | ends << 16;
+    const bool some = __syncthreads_or((starts | ends) != 0);
+    Vec<V> Fb = vec<V>(1.0f), Gb = vec<V>(0.0f);
     bool cut = false;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      if (w >= warp) break;
-      Vec<V> Fw, Uw, Gw;
-      slice_map(w, Fw, Uw, Gw);
-      h = some && sm.starts[buf][w] != 0 ? Uw : fma(Fw, h, Uw);
-    }
 #pragma unroll
     for (int w = WARPS - 1; w > 0; w--) {
       if (w <= warp) break;
-      Vec<V> Fw, Uw, Gw;
-      slice_map(w, Fw, Uw, Gw);
-      const bool constant = some && sm.starts[buf][w] != 0;
-      cut |= constant;
-      Gb = constant ? Gw : fma(Fw, Gb, Gw);
-      Fb = least(mul(Fb, Fw));
+      const Vec<V> Fw = sm.F[buf][w][lane], Gw = sm.G[buf][w][lane];
+      Gb = fma(Fw, Gb, Gw);
+      Fb = mul(Fb, Fw);
+      if (some && sm.cuts[buf][w] >> 16 != 0) {
+        cut = true;
+        Gb = Gw;
+      }
     }
-    Vec<V> e;                                        // what flows into the slice from behind
+    Fb = least(Fb);
+    Vec<V> e = carry;                                // what flows into the slice from behind
     if (size == 1) {
-      e = cut ? Gb : fma(Fb, carry, Gb);
-      carry = e;
 #pragma unroll
       for (int w = WARPS - 1; w >= 0; w--) {
-        if (w > warp) continue;
-        Vec<V> Fw, Uw, Gw;
-        slice_map(w, Fw, Uw, Gw);
-        carry = some && sm.starts[buf][w] != 0 ? Gw : fma(Fw, carry, Gw);
+        const Vec<V> Fw = sm.F[buf][w][lane], Gw = sm.G[buf][w][lane];
+        carry = fma(Fw, carry, Gw);
+        if (some && sm.cuts[buf][w] >> 16 != 0) carry = Gw;
       }
-    } else {
-      if (warp == 0) {                               // it has the tile's map: to every block of the cluster
-        const Vec<V> Gt = starts ? G : fma(F, Gb, G), Ft = least(mul(Fb, F));
-        for (uint32_t b = 0; b < size; b++) put_remote(&sm.tile[buf][rank][lane], b, make_float4(Ft.v[0], Ft.v[V - 1], Gt.v[0], Gt.v[V - 1]));
-        if (lane < size) put_remote(&sm.tile_starts[buf][rank], lane, (uint32_t)(cut || starts != 0));
-      }
-      cluster_arrive();
-      cluster_wait();
-      Vec<V> behind = carry;
-#pragma unroll
-      for (int b = MAX_CLUSTER - 1; b >= 0; b--) {
-        if (b >= size) continue;
-        const float4 m = sm.tile[buf][b][lane];
-        Vec<V> Fw, Gw;
-        Fw.v[0] = m.x; Fw.v[V - 1] = m.y; Gw.v[0] = m.z; Gw.v[V - 1] = m.w;
-        if (b == rank) behind = carry;
-        carry = sm.tile_starts[buf][b] != 0 ? Gw : fma(Fw, carry, Gw);
-      }
-      e = cut ? Gb : fma(Fb, behind, Gb);
+    } else if (warp == 0) {                          // it has the tile's map: to every block of the cluster
+      const Vec<V> Gt = ends ? G : fma(F, Gb, G);
+      Vec<V> Ft = least(mul(Fb, F));
+      if (cut || ends) Ft = vec<V>(-1.0f);
+      const float4 v = make_float4(Ft.v[0], Ft.v[V - 1], Gt.v[0], Gt.v[V - 1]);
+      for (uint32_t b = 0; b < size; b++) send(&tiles[buf * size + rank][lane], &sm.sent[buf], b, v);
     }
-    // the states in front of the tokens
+    // meanwhile the states in front of the tokens
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      if (w >= warp) break;
+      const Vec<V> Uw = sm.U[buf][w][lane];
+      h = fma(sm.F[buf][w][lane], h, Uw);
+      if (some && (sm.cuts[buf][w] & 0xffffu) != 0) h = Uw;
+    }
 #pragma unroll
     for (int s = 0; s < S; s++) {
-      if (starts >> s & 1) entering(s, h);
+      if (starts >> s & 1) h = state(p.src, t0 + s);
       const Vec<V> before = h;
       h = fma(f[s], h, u[s]);
       u[s] = before;
     }
-    T* dx = reinterpret_cast<T*>(p.dx) + (t0 + n - 1) * p.lddx + c;
-    T* dr = reinterpret_cast<T*>(p.dr) + (t0 + n - 1) * p.lddr + c;
-    T* di = reinterpret_cast<T*>(p.di) + (t0 + n - 1) * p.lddi + c;
+    if (size > 1) {
+      if (!lost) lost = !bar_wait(&sm.sent[buf], use >> 1 & 1);
+#pragma unroll
+      for (int b = MAX_CLUSTER - 1; b >= 0; b--) {
+        if (b >= size) continue;
+        const float4 m = tiles[buf * size + b][lane];
+        Vec<V> Fw, Gw;
+        Fw.v[0] = m.x; Fw.v[V - 1] = m.y; Gw.v[0] = m.z; Gw.v[V - 1] = m.w;
+        if (b == rank) e = carry;
+        carry = pick(m.x < 0.0f, Gw, fma(Fw, carry, Gw));
+      }
+    }
+    e = cut ? Gb : fma(Fb, e, Gb);
+    T* dx = reinterpret_cast<T*>(p.dx) + (long long)t0 * p.lddx + c;
+    T* dr = reinterpret_cast<T*>(p.dr) + (long long)t0 * p.lddr + c;
+    T* di = reinterpret_cast<T*>(p.di) + (long long)t0 * p.lddi + c;
 #pragma unroll
     for (int s = S - 1; s >= 0; s--) {
       if (s >= n) continue;
-      const Gates<V> a = decay<T, POWER, V>(token(1, s), rb, k_);
-      const Vec<V> dh = add(d[s], e);
+      if (ends >> s & 1) e = state(p.dfinal, t0 + s);
+      const Vec<V> dh = add(gradient(s), e);
+      Gates<V> a = decay<T, POWER, V, true>(token(1, s), rb, k_);
       Vec<V> b = mul(dh, token(0, s)), gx = mul(dh, a.gain), gr, gi = vec<V>(0.0f);
       if constexpr (GATED) {
-        Vec<V> g, ng;
-        sigmoids<T, V>(token(3, s), ib, g, ng);
-        b = mul(b, g);
-        gx = mul(gx, g);
+        Vec<V> gate, ng;
+        sigmoids<T, V>(token(3, s), ib, gate, ng);
+        b = mul(b, gate);
+        gx = mul(gx, gate);
         gi = mul(mul(b, a.gain), ng);
         sum_i = add(sum_i, gi);
       }
       if constexpr (POWER) {
-        const Vec<V> l = sizeof(T) == 4 ? a.l : mul(a.l, vec<V>(LN2_F));
-        // f (dh h l - b f (l / gain))
-        const Vec<V> m = mul(a.f, fma(mul(dh, u[s]), l, mul(mul(mul(b, vec<V>(-1.0f)), a.f), mul(l, a.inv))));
+        // l to base 2, whose ln 2 joins the sum at its end: f (dh h l - b f (l / gain))
+        Vec<V> bf = mul(b, a.f);
+#pragma unroll
+        for (int k = 0; k < V; k++) bf.v[k] = -bf.v[k];
+        const Vec<V> m = mul(a.f, fma(mul(dh, u[s]), a.l, mul(bf, mul(a.l, a.inv))));
         gr = mul(m, a.n);
+#pragma unroll
+        for (int k = 0; k < V; k++) gr.v[k] *= LN2_F;
         sum_rate = add(sum_rate, m);
       } else {
-        gr = mul(fma(dh, u[s], mul(b, vec<V>(-1.0f))), mul(a.s, a.n));
+        Vec<V> d = mul(dh, u[s]);
+#pragma unroll
+        for (int k = 0; k < V; k++) d.v[k] -= b.v[k];
+        gr = mul(d, mul(a.s, a.n));
       }
       sum_r = add(sum_r, gr);
       e = mul(a.f, dh);
       if constexpr (ASYNC) {                         // in the places of the inputs that they are the gradients of
-        slice(slot, 0).row[s][lane] = pack<T, V>(gx.v);
-        slice(slot, 1).row[s][lane] = pack<T, V>(gr.v);
-        if (GATED) slice(slot, 3).row[s][lane] = pack<T, V>(gi.v);
-      } else {
-        if (mine) {
-          *dx = from_float<T>(gx.v[0]);
-          *dr = from_float<T>(gr.v[0]);
-          if (GATED) *di = from_float<T>(gi.v[0]);
-        }
-        dx -= p.lddx;
-        dr -= p.lddr;
-        if (GATED) di -= p.lddi;
+        slice(buf, 0).row[s][lane] = pack<T, V>(gx.v);
+        slice(buf, 1).row[s][lane] = pack<T, V>(gr.v);
+        if (GATED) slice(buf, 3).row[s][lane] = pack<T, V>(gi.v);
+      } else if (mine) {
+        dx[s * p.lddx] = from_float<T>(gx.v[0]);
+        dr[s * p.lddr] = from_float<T>(gr.v[0]);
+        if (GATED) di[s * p.lddi] = from_float<T>(gi.v[0]);
       }
-      if (starts >> s & 1) {
-        Vec<V> unused;
-        const int q = entering(s, unused);
+      if ((starts >> s & 1) && p.dsrc != nullptr) {
+        const int q = lower(tables, 0, p.seq.N + 1, t0 + s + 1) - 1;
 #pragma unroll
         for (int k = 0; k < V; k++)
-          if (p.dsrc != nullptr && mine) p.dsrc[(long long)q * p.C + c + k] = e.v[k];
-        e = vec<V>(0.0f);
+          if (mine) p.dsrc[(long long)q * p.C + c + k] = e.v[k];
       }
     }
     if constexpr (ASYNC) {
       __syncwarp();
-      slice(slot, 0).store(p.dx, p.lddx, t0, n, c0, p.C);
-      slice(slot, 1).store(p.dr, p.lddr, t0, n, c0, p.C);
-      if (GATED) slice(slot, 3).store(p.di, p.lddi, t0, n, c0, p.C);
+      Cursor<T, S>(p.dx, p.lddx, t0, c0).store(slice(buf, 0), g.dx, n, chunk);
+      Cursor<T, S>(p.dr, p.lddr, t0, c0).store(slice(buf, 1), g.dr, n, chunk);
+      if (GATED) Cursor<T, S>(p.di, p.lddi, t0, c0).store(slice(buf, 3), g.di, n, chunk);
+    } else {
+      ask(round - 1, 0);                             // with a second set of registers, a round ahead, it spilled 100 to 800 bytes
     }
-    t0 -= step;
-    slot = slot == DEPTH - 1 ? 0 : slot + 1;
   }
+  if (lost) report(p.seq.status, SEQ_LOST);
   zero_rest<T, V>(p.dx, p.lddx, end, p.seq.T, c, mine, rank, size);
   zero_rest<T, V>(p.dr, p.lddr, end, p.seq.T, c, mine, rank, size);
   if (GATED) zero_rest<T, V>(p.di, p.lddi, end, p.seq.T, c, mine, rank, size);
 
-  // sums over the tokens: of the warps (in the places of the maps), then of the cluster's blocks
+  // sums over the tokens: of the warps (in the places of the maps), then of the cluster's blocks (in that of the tiles)
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < V; k++) sm.map[0][warp][k][lane] = {sum_rate.v[k], sum_r.v[k], sum_i.v[k], 0.0f};
+  sm.F[0][warp][lane] = sum_rate;
+  sm.U[0][warp][lane] = sum_r;
+  sm.G[0][warp][lane] = sum_i;
   __syncthreads();
-  float total[V];
+  if (size > 1) {                                    // no block reads tiles any more
+    cluster_arrive();
+    cluster_wait();
+  }
+  Vec<V> total = vec<V>(0.0f);
   if (warp < 3) {
+    for (int w = 0; w < WARPS; w++) total = add(total, warp == 0 ? sm.F[0][w][lane] : (warp == 1 ? sm.U[0][w][lane] : sm.G[0][w][lane]));
+    if (size > 1) {                                  // three rows of a block: rows 3 rank ... of the 2 size there are, of 4 values a lane
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-      total[k] = 0.0f;
-      for (int w = 0; w < WARPS; w++) total[k] += sm.map[0][w][k][lane].v[warp];
-      if (size > 1) put_remote(&sm.tile_sums[warp][rank][k][lane], 0, total[k]);
+      for (int k = 0; k < V; k++) put_remote(reinterpret_cast<float*>(tiles) + ((3 * rank + warp) * V + k) * 32 + lane, 0, total.v[k]);
     }
   }
   if (size > 1) {
@@ -335,24 +323,27 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
 #pragma unroll
     for (int k = 0; k < V; k++) {
       if (size > 1) {
-        total[k] = 0.0f;
-        for (uint32_t b = 0; b < size; b++) total[k] += sm.tile_sums[warp][b][k][lane];
+        total.v[k] = 0.0f;
+        for (uint32_t b = 0; b < size; b++) total.v[k] += reinterpret_cast<const float*>(tiles)[((3 * b + warp) * V + k) * 32 + lane];
       }
       if (warp == 0) {
         const float v = p.rate[c + k], soft = softplus_exact(v);
-        total[k] *= soft > 0.0f ? 1.0f / (1.0f + expf(-v)) / soft : 1.0f;      // 1 in the limit of low rates
+        total.v[k] *= LN2_F * (soft > 0.0f ? 1.0f / (1.0f + expf(-v)) / soft : 1.0f);      // 1 in the limit of low rates
       }
-      to[c + k] = total[k];
+      to[c + k] = total.v[k];
     }
   }
 }
 
 template <typename T, bool ASYNC, bool POWER, bool GATED>
 cudaError_t launch_gates(const GatedScanGradParams& p, cudaStream_t stream) {
-  constexpr int V = CHANNELS<T, ASYNC>;
+  constexpr int V = CHANNELS<T, ASYNC>, B = sizeof(T);
   const long long slabs = (p.C + 32 * V - 1) / (32 * V);
-  return launch_clusters(kda_gated_scan_grad_kernel<T, ASYNC, POWER, GATED>, p, slabs, cluster_of(slabs, p.seq.T, TILE),
-                         ASYNC ? DEPTH * WARPS * (GATED ? 4 : 3) * (int)sizeof(Slice<T, S>) : 0, stream);
+  const auto bytes = [](int size) { return (ASYNC ? DEPTH * WARPS * (GATED ? 4 : 3) * (int)sizeof(Slice<T, S>) : 0) + 2 * size * (int)sizeof(Tile); };
+  const auto kernel = kda_gated_scan_grad_kernel<T, ASYNC, POWER, GATED>;
+  const int size = cluster_of(kernel, slabs, p.seq.T, TILE, THREADS, bytes);
+  const Steps g = {4 * p.ldx * B, 4 * p.ldr * B, 4 * p.ldi * B, 4 * p.lddy * B, 4 * p.lddx * B, 4 * p.lddr * B, 4 * p.lddi * B};
+  return launch_clusters(kernel, slabs, size, THREADS, bytes(size), stream, p, g);
 }
 
 template <typename T, bool ASYNC>

@@ -8,7 +8,7 @@
 
 namespace kda {
 
-constexpr int SEQ_BAD_CU = 1, SEQ_BAD_SLOT = 2, SEQ_POOL_FULL = 32;      // KDA_STATUS_* of these operators
+constexpr int SEQ_BAD_CU = 1, SEQ_BAD_SLOT = 2, SEQ_POOL_FULL = 32, SEQ_LOST = 64;      // KDA_STATUS_* of these operators
 
 // Sequences of a packed batch and the slots of their states.  Without `cu` there is one sequence [0, T) (a step: T sequences
 // of one token); without `slots` sequence i uses slot i.
