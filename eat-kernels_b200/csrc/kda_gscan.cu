@@ -10,7 +10,7 @@ using namespace gscan;
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int DEPTH = 2;                 // rounds of tokens on their way or worked on
 constexpr int S = 12, TILE = WARPS * S;  // tokens of a slice, of a block: 16 a slice do not fit 128 registers with all that a ragged batch takes
-static_assert(TILE == GATED_SCAN_TILE, "the states that a training pass keeps are those in front of the tiles");
+static_assert(GATED_SCAN_TILE % S == 0 && TILE % GATED_SCAN_TILE == 0, "the states that a training pass keeps are those in front of slices");
 
 // One round's maps of the warps' slices, {F, U} of a lane's channels, double-buffered against warps (blocks) that are a round ahead.
 template <int V>
@@ -238,9 +238,9 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
       }
     }
     Vec<V> h = cut ? Ub : fma(Fb, enter, Ub);
-    if (p.tiles != nullptr && warp == 0 && mine && n > 0) {
+    if (p.tiles != nullptr && warp % (GATED_SCAN_TILE / S) == 0 && mine && n > 0) {
 #pragma unroll
-      for (int k = 0; k < V; k++) p.tiles[(long long)(t0 / TILE) * p.C + c + k] = h.v[k];
+      for (int k = 0; k < V; k++) p.tiles[(long long)(t0 / GATED_SCAN_TILE) * p.C + c + k] = h.v[k];
     }
     T* out = reinterpret_cast<T*>(p.out) + (long long)t0 * p.ldo + c;
     if (!plain && n > 0) {                           // token by token, with the ends of sequences

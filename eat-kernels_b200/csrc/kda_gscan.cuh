@@ -15,8 +15,8 @@ namespace kda {
 
 namespace gscan {
 
-constexpr int MAX_CLUSTER = 8, MAX_DEVICES = 64;
-constexpr uint32_t WAIT_MS = 2000;
+constexpr int MAX_CLUSTER = 16, MAX_DEVICES = 64;
+constexpr unsigned long long WAIT_NS = 2000000000ULL;
 constexpr uint32_t NEVER = 0xffffffffu;
 
 // A product of decays that underflows to zero is taken as the smallest positive number, so that an infinite state stays infinite, as it
@@ -151,19 +151,17 @@ __device__ __forceinline__ bool bar_done(uint32_t b, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-__device__ __forceinline__ uint32_t milliseconds() {     // about; wraps
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return (uint32_t)(t >> 20);
-}
-// False where two seconds ran out: what comes then is wrong, and ends
+// False where some two seconds ran out: what comes then is wrong, and ends
 __device__ __forceinline__ bool bar_wait(const void* bar, uint32_t parity) {
   const uint32_t b = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
-  if (bar_done(b, parity)) return true;
-  const uint32_t begin = milliseconds();
-  while (!bar_done(b, parity))
-    if (milliseconds() - begin > WAIT_MS) return false;
-  return true;
+  unsigned long long begin = 0, now;
+  do {
+    for (int i = 0; i < 4096; i++)
+      if (bar_done(b, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (begin == 0) begin = now;
+  } while (now - begin < WAIT_NS);
+  return false;
 }
 
 // ---- one or two channels at once (two: one instruction)
@@ -248,15 +246,15 @@ struct Cursor {
     const char* from = at;
     if (n == S && on) {
 #pragma unroll
-      for (int q = 0; q < S / 4; q++) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a + 512u * q), "l"(from) : "memory");
+      for (int q = 0; q < (S + 3) / 4; q++) {
+        if (4 * q + 3 < S || row + 4 * q < S) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a + 512u * q), "l"(from) : "memory");
         from += four;
       }
     } else {
 #pragma unroll
-      for (int q = 0; q < S / 4; q++) {
+      for (int q = 0; q < (S + 3) / 4; q++) {
         const bool here = on && row + 4 * q < n;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a + 512u * q), "l"(here ? (const void*)from : valid), "r"(here ? 16 : 0) : "memory");
+        if (4 * q + 3 < S || row + 4 * q < S) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(a + 512u * q), "l"(here ? (const void*)from : valid), "r"(here ? 16 : 0) : "memory");
         from += four;
       }
     }
@@ -267,7 +265,7 @@ struct Cursor {
     const uint4* a = reinterpret_cast<const uint4*>(&from) + threadIdx.x % 32;
     char* to = const_cast<char*>(at);
 #pragma unroll
-    for (int q = 0; q < S / 4; q++) {
+    for (int q = 0; q < (S + 3) / 4; q++) {
       if (on && row + 4 * q < n) *reinterpret_cast<uint4*>(to) = a[32 * q];
       to += four;
     }
@@ -446,8 +444,12 @@ int cluster_of(K kernel, long long slabs, long long T, int tile, int threads, B 
       cudaLaunchAttribute attr[1];
       configure(cfg, attr, size, size, threads, bytes(size), nullptr);
       int n = 0;
+      if (size > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (bytes(size) > 0) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(size));
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        n = 0;
+        cudaGetLastError();
+      }
       room[dev][size] = n + 1;
     }
     if (slabs <= room[dev][size] - 1) best = size;
@@ -460,6 +462,10 @@ cudaError_t launch_clusters(K kernel, long long slabs, int size, int threads, in
   if (slabs * size > 0x7fffffffLL) return cudaErrorInvalidValue;
   if (bytes > 0) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
+  if (size > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};

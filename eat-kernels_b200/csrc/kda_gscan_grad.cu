@@ -17,7 +17,7 @@ using namespace gscan;
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr int DEPTH = 2;                 // rounds of tokens on their way or worked on
-constexpr int S = 12, TILE = WARPS * S;  // tokens of a slice, of a block
+constexpr int S = 6, TILE = WARPS * S;   // tokens of a slice, of a block
 static_assert(TILE == GATED_SCAN_TILE, "the forward pass keeps the states in front of the tiles");
 
 // Two blocks an SM leave 17 KB beside the tokens of 16-bit calls.
@@ -143,16 +143,20 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
 #pragma unroll
     for (int s = 0; s < S; s++) token_terms<T, POWER, GATED, V>(token(0, s), token(1, s), token(3, s), rb, ib, k_, f[s], u[s]);
     // the slice's maps, forwards and backwards
-    Vec<V> F = vec<V>(1.0f), U = vec<V>(0.0f), G = vec<V>(0.0f);
-    if (n == S && (starts | ends) == 0) {
+    const bool plain = n == S && (starts | ends) == 0;
+    Vec<V> F = f[0], U = u[0], G;
+    if (plain) {
 #pragma unroll
-      for (int s = 0; s < S; s++) {
+      for (int s = 1; s < S; s++) {
         U = fma(f[s], U, u[s]);
         F = mul(F, f[s]);
       }
+      G = mul(f[S - 1], gradient(S - 1));
 #pragma unroll
-      for (int s = S - 1; s >= 0; s--) G = mul(f[s], add(gradient(s), G));
+      for (int s = S - 2; s >= 0; s--) G = mul(f[s], add(gradient(s), G));
     } else {
+      F = vec<V>(1.0f);
+      U = G = vec<V>(0.0f);
 #pragma unroll
       for (int s = 0; s < S; s++) {
         if (s >= n) { f[s] = vec<V>(1.0f); u[s] = vec<V>(0.0f); }
@@ -209,12 +213,21 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
       h = fma(sm.F[buf][w][lane], h, Uw);
       if (some && (sm.cuts[buf][w] & 0xffffu) != 0) h = Uw;
     }
+    if (starts == 0) {
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      if (starts >> s & 1) h = state(p.src, t0 + s);
-      const Vec<V> before = h;
-      h = fma(f[s], h, u[s]);
-      u[s] = before;
+      for (int s = 0; s < S; s++) {
+        const Vec<V> before = h;
+        h = fma(f[s], h, u[s]);
+        u[s] = before;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        if (starts >> s & 1) h = state(p.src, t0 + s);
+        const Vec<V> before = h;
+        h = fma(f[s], h, u[s]);
+        u[s] = before;
+      }
     }
     if (size > 1) {
       if (!lost) lost = !bar_wait(&sm.sent[buf], use >> 1 & 1);
@@ -232,39 +245,34 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
     T* dx = reinterpret_cast<T*>(p.dx) + (long long)t0 * p.lddx + c;
     T* dr = reinterpret_cast<T*>(p.dr) + (long long)t0 * p.lddr + c;
     T* di = reinterpret_cast<T*>(p.di) + (long long)t0 * p.lddi + c;
-#pragma unroll
-    for (int s = S - 1; s >= 0; s--) {
-      if (s >= n) continue;
-      if (ends >> s & 1) e = state(p.dfinal, t0 + s);
-      const Vec<V> dh = add(gradient(s), e);
-      Gates<V> a = decay<T, POWER, V, true>(token(1, s), rb, k_);
-      Vec<V> b = mul(dh, token(0, s)), gx = mul(dh, a.gain), gr, gi = vec<V>(0.0f);
+    auto gradients = [&](int s) {
+      const Vec<V> dh = add(gradient(s), e), x = token(0, s);
+      const Gates<V> a = decay<T, POWER, V, true>(token(1, s), rb, k_);
+      e = mul(f[s], dh);
+      Vec<V> b = mul(dh, x), gx = mul(dh, a.gain), gr, gi;
       if constexpr (GATED) {
         Vec<V> gate, ng;
         sigmoids<T, V>(token(3, s), ib, gate, ng);
         b = mul(b, gate);
         gx = mul(gx, gate);
-        gi = mul(mul(b, a.gain), ng);
+        gi = mul(mul(gx, x), ng);
         sum_i = add(sum_i, gi);
       }
       if constexpr (POWER) {
         // l to base 2, whose ln 2 joins the sum at its end: f (dh h l - b f (l / gain))
-        Vec<V> bf = mul(b, a.f);
+        Vec<V> m;
 #pragma unroll
-        for (int k = 0; k < V; k++) bf.v[k] = -bf.v[k];
-        const Vec<V> m = mul(a.f, fma(mul(dh, u[s]), a.l, mul(bf, mul(a.l, a.inv))));
-        gr = mul(m, a.n);
-#pragma unroll
-        for (int k = 0; k < V; k++) gr.v[k] *= LN2_F;
+        for (int k = 0; k < V; k++) {
+          const float w = a.l.v[k] * a.inv.v[k];
+          m.v[k] = f[s].v[k] * fmaf(dh.v[k] * u[s].v[k], a.l.v[k], -(b.v[k] * f[s].v[k] * w));
+          gr.v[k] = m.v[k] * (a.n.v[k] * LN2_F);
+        }
         sum_rate = add(sum_rate, m);
       } else {
-        Vec<V> d = mul(dh, u[s]);
 #pragma unroll
-        for (int k = 0; k < V; k++) d.v[k] -= b.v[k];
-        gr = mul(d, mul(a.s, a.n));
+        for (int k = 0; k < V; k++) gr.v[k] = fmaf(dh.v[k], u[s].v[k], -b.v[k]) * (a.s.v[k] * a.n.v[k]);
       }
       sum_r = add(sum_r, gr);
-      e = mul(a.f, dh);
       if constexpr (ASYNC) {                         // in the places of the inputs that they are the gradients of
         slice(buf, 0).row[s][lane] = pack<T, V>(gx.v);
         slice(buf, 1).row[s][lane] = pack<T, V>(gr.v);
@@ -274,11 +282,22 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
         dr[s * p.lddr] = from_float<T>(gr.v[0]);
         if (GATED) di[s * p.lddi] = from_float<T>(gi.v[0]);
       }
-      if ((starts >> s & 1) && p.dsrc != nullptr) {
-        const int q = lower(tables, 0, p.seq.N + 1, t0 + s + 1) - 1;
+    };
+    if (plain) {
 #pragma unroll
-        for (int k = 0; k < V; k++)
-          if (mine) p.dsrc[(long long)q * p.C + c + k] = e.v[k];
+      for (int s = S - 1; s >= 0; s--) gradients(s);
+    } else {
+#pragma unroll
+      for (int s = S - 1; s >= 0; s--) {
+        if (s >= n) continue;
+        if (ends >> s & 1) e = state(p.dfinal, t0 + s);
+        gradients(s);
+        if ((starts >> s & 1) && p.dsrc != nullptr) {
+          const int q = lower(tables, 0, p.seq.N + 1, t0 + s + 1) - 1;
+#pragma unroll
+          for (int k = 0; k < V; k++)
+            if (mine) p.dsrc[(long long)q * p.C + c + k] = e.v[k];
+        }
       }
     }
     if constexpr (ASYNC) {

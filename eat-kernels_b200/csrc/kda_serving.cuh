@@ -51,7 +51,7 @@ struct StepParams {
 };
 cudaError_t launch_kda_step(const StepParams& p, cudaStream_t stream);
 
-constexpr int GATED_SCAN_TILE = 96;      // a training pass keeps the states in front of every so many tokens
+constexpr int GATED_SCAN_TILE = 48;      // a training pass keeps the states in front of every so many tokens
 struct GatedScanParams {
   const void *x, *r, *i;   // [T][C]; i may be nullptr
   void* out;

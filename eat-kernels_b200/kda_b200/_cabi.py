@@ -22,7 +22,7 @@ EXPORTS = ["kda_prefill_workspace_bytes", "kda_prefill_workspace_bytes_cuts", "k
            "kda_group_norm_launch", "kda_group_norm_grad_launch"]
 TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
 SCAN_MAX_STATE, MAX_POOLS, MAX_TABLES = 128, 8, 8
-GATED_SCAN_TILE, GROUP_NORM_MAX_WIDTH = 96, 16384
+GATED_SCAN_TILE, GROUP_NORM_MAX_WIDTH = 48, 16384
 ACT_NONE, ACT_SILU, ACT_SIGMOID = 0, 1, 2
 
 

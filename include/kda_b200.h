@@ -334,14 +334,14 @@ typedef struct KdaGatedScanArgs {
   const float* i_bias;     /* [C] or NULL; only with i */
   const float* src;        /* [slot][C]; NULL = zeros */
   float* dst;              /* NULL = not stored; may be src.  A step needs src == dst */
-  float* tiles;            /* [(T + 95) / 96][C], packed: the states that a later kda_gated_scan_grad_launch starts from; or NULL.
+  float* tiles;            /* [(T + 47) / 48][C], packed: the states that a later kda_gated_scan_grad_launch starts from; or NULL.
                               Unused in a step */
   int64_t ldx, ldr, ldi, ldo, src_slot_stride, dst_slot_stride;
   KdaSequences seq;
   float rate_scale;
   int32_t C, type;
 } KdaGatedScanArgs;
-#define KDA_GATED_SCAN_TILE 96
+#define KDA_GATED_SCAN_TILE 48
 int kda_gated_scan_launch(const KdaGatedScanArgs* args, void* stream);
 int kda_gated_scan_step_launch(const KdaGatedScanArgs* args, void* stream);
 
