@@ -10,6 +10,7 @@
 // not depend on timing, nothing is kept in memory between blocks, and ragged batches cost what their tokens cost.
 #pragma once
 #include "kda_serving.cuh"
+#include <atomic>
 
 namespace kda {
 
@@ -367,7 +368,7 @@ __device__ __forceinline__ Gates<V> decay(Vec<V> r, Vec<V> bias, Vec<V> k_) {
 #pragma unroll
     for (int k = 0; k < V; k++) {
       if (GRAD) {
-        a.inv.v[k] = rsqrt_fast(fmaxf(q.v[k], 1.0e-38f));      // l times it is 0 where l is
+        a.inv.v[k] = rsqrt_fast(fmaxf(q.v[k], 2.0e-38f));      // l times it is 0 where l is
         a.gain.v[k] = q.v[k] * a.inv.v[k];
       } else {
         a.gain.v[k] = sqrt_fast(q.v[k]);
@@ -392,7 +393,7 @@ __device__ __forceinline__ void token_terms(Vec<V> x, Vec<V> r, Vec<V> i, Vec<V>
 #pragma unroll
     for (int k = 0; k < V; k++) {
       const float a = ex2_fast(min_or_nan(fmaf(i.v[k], -LOG2E_F, ib.v[k]), 60.0f)) + 1.0f;
-      w.v[k] = rsqrt_fast(fmaf(q.v[k] * a, a, 1.0e-38f));
+      w.v[k] = rsqrt_fast(fmaf(q.v[k] * a, a, 2.0e-38f));
     }
     u = mul(mul(q, w), x);
   } else {
@@ -434,7 +435,7 @@ inline void configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, long l
 // the card's groups of SMs, so the sizes that fit are asked for (once for a kernel and device).
 template <typename K, typename B>
 int cluster_of(K kernel, long long slabs, long long T, int tile, int threads, B bytes) {
-  static int room[MAX_DEVICES][MAX_CLUSTER + 1];     // clusters of a size that run at once, plus one; 0: not asked yet
+  static std::atomic<int> room[MAX_DEVICES][MAX_CLUSTER + 1];        // clusters of a size that run at once, plus one; 0: not asked yet
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= MAX_DEVICES) return 1;
   int best = 1;

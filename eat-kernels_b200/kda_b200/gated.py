@@ -5,7 +5,8 @@
     y, pool = gated_scan_step(x, r, i, rate, r_bias, i_bias, pool, slots)
     y = group_norm(x, groups, weight, bias, z, activation="silu")                                  # differentiable
 
-Tokens, sequences, slots, `out` and `status` are those of the operators in `serving.py`.  Gradients: with grad mode on, a call without
+Tokens, sequences, slots, `out` and `status` are those of the operators in `serving.py` (`status`: also the bit 64 = a wait inside
+the kernel ran out, results are wrong).  Gradients: with grad mode on, a call without
 `ssm_state_indices` and `out` whose tensors ask for some is recorded; calls that work on a pool or write the caller's `out` are serving
 calls and record nothing.  Backward passes return the same bits whenever they run, can be captured in a CUDA graph and are
 differentiable once."""
@@ -169,7 +170,7 @@ def _norm_inputs(x, groups, weight, bias, z, activation):
         if groups not in (None, x.shape[2]):
             raise _err(f"x [1, T, {x.shape[2]}, {x.shape[3]}] has {x.shape[2]} groups, got groups = {groups!r}")
         groups = x.shape[2]
-    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or channels % groups:
+    if groups is None or groups < 1 or channels % groups:
         raise _err(f"groups must divide the {channels} channels, got {groups!r}")
     width = channels // groups
     if width > _cabi.GROUP_NORM_MAX_WIDTH:
@@ -254,6 +255,8 @@ def group_norm(x, groups=None, weight=None, bias=None, z=None, *, activation=Non
     x, z [1, T, C] of one type (bf16, fp16 or fp32; any token strides) with `groups` dividing C, or [1, T, groups, D]; groups of up to
     16384 channels.  weight, bias fp32 with C entries, or with the C / groups that all groups share; each may be None.  activation
     "silu", "sigmoid" or None.  Returns y like x; without `out` it is differentiable with respect to all tensors."""
+    if groups is not None and (isinstance(groups, bool) or not isinstance(groups, int)):
+        raise _err(f"groups must be a whole number, got {groups!r}")
     eps = float(eps)
     if not (math.isfinite(eps) and eps >= 0.0):
         raise _err(f"eps must be a number of zero or more, got {eps!r}")

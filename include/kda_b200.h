@@ -242,7 +242,9 @@ enum { KDA_TYPE_BF16 = 0, KDA_TYPE_FP16 = 1, KDA_TYPE_FP32 = 2 };
 /* Further bits of `status` in these calls, which OR them in (the caller clears it): KDA_STATUS_BAD_CU (every sequence taken as
  * empty, all output rows zero), KDA_STATUS_BAD_SLOT (out of range or a repeat of an earlier entry: that sequence starts from
  * zeros and its state is not stored), and */
-enum { KDA_STATUS_POOL_FULL = 32 };   /* kda_pool_fork: no slot was left for some entry */
+enum { KDA_STATUS_POOL_FULL = 32,     /* kda_pool_fork: no slot was left for some entry */
+       KDA_STATUS_LOST = 64 };        /* kda_gated_scan(_grad): blocks of a cluster waited for one another for two seconds and went on;
+                                         the call's results are wrong */
 
 /* Sequences of a batch and the slots of their states. */
 typedef struct KdaSequences {
