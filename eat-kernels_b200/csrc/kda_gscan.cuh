@@ -332,21 +332,22 @@ __device__ __forceinline__ void sigmoids(Vec<V> x, Vec<V> bias, Vec<V>& s, Vec<V
   }
 }
 
-// 1 - f^2 for f = 2^l, l <= 0: near zero by a polynomial for (1 - 2^(2 l)) / l on [-0.36, 0] (relative minimax, found by linear programming, with
-// its roundings 1.9e-7 off in fp32), as the difference would lose its digits there
+// f = 2^l and q = 1 - f^2, l <= 0.  Near zero q comes from a polynomial for (1 - 2^(2 l)) / l on [-0.36, 0] (relative minimax, found by linear
+// programming, with its roundings 1.9e-7 off in fp32), as the difference d = 1 - f^2 would lose its digits there; and the approximate f,
+// which may be two steps off, is put right by what d misses of q (Newton's step on f^2 = 1 - q, 1 / f taken as 1).  A state that decays
+// slowly sums up that error 1 / (1 - f) times.
 template <int V>
-__device__ __forceinline__ Vec<V> one_minus_square(Vec<V> l, Vec<V> f) {
-  Vec<V> r;
+__device__ __forceinline__ void decay_pair(Vec<V> l, Vec<V>& f, Vec<V>& q) {
 #pragma unroll
   for (int k = 0; k < V; k++) {                      // single values: pairs of constants would take registers, or moves
-    const float a = l.v[k];
-    float q = fmaf(a, -0.03467162698507309f, -0.15143901109695435f);
-    q = fmaf(a, q, -0.44371989369392395f);
-    q = fmaf(a, q, -0.9608919620513916f);
-    q = fmaf(a, q, -1.3862942457199097f);
-    r.v[k] = a > -0.36f ? q * a : fmaf(-f.v[k], f.v[k], 1.0f);
+    const float a = l.v[k], e = ex2_fast(a), d = fmaf(-e, e, 1.0f);
+    float m = fmaf(a, -0.03467162698507309f, -0.15143901109695435f);
+    m = fmaf(a, m, -0.44371989369392395f);
+    m = fmaf(a, m, -0.9608919620513916f);
+    m = fmaf(a, m, -1.3862942457199097f);
+    q.v[k] = a > -0.36f ? m * a : d;
+    f.v[k] = fmaf(0.5f, d - q.v[k], e);
   }
-  return r;
 }
 
 // A token's values.  `l` (POWER) is log f to base 2; s, n: of the decay's gate; inv: 1 / gain.  What only gradients need comes with GRAD.
@@ -360,11 +361,13 @@ __device__ __forceinline__ Gates<V> decay(Vec<V> r, Vec<V> bias, Vec<V> k_) {
   sigmoids<T, V, GRAD || !POWER>(r, bias, a.s, a.n);
   if constexpr (!POWER) {
     a.f = a.s; a.gain = a.n; a.l = a.inv = vec<V>(0.0f);
+#pragma unroll
+    for (int k = 0; k < V; k++)                      // near one s is 1 - n to half a step
+      if (a.n.v[k] < 0.5f) a.f.v[k] = 1.0f - a.n.v[k];
   } else {
     a.l = mul(k_, a.s);
-#pragma unroll
-    for (int k = 0; k < V; k++) a.f.v[k] = ex2_fast(a.l.v[k]);
-    const Vec<V> q = one_minus_square(a.l, a.f);
+    Vec<V> q;
+    decay_pair(a.l, a.f, q);
 #pragma unroll
     for (int k = 0; k < V; k++) {
       if (GRAD) {
@@ -385,10 +388,8 @@ __device__ __forceinline__ void token_terms(Vec<V> x, Vec<V> r, Vec<V> i, Vec<V>
   if constexpr (POWER && GATED && sizeof(T) == 2) {
     Vec<V> s, n;
     sigmoids<T, V, false>(r, rb, s, n);
-    const Vec<V> l = mul(k_, s);
-#pragma unroll
-    for (int k = 0; k < V; k++) f.v[k] = ex2_fast(l.v[k]);
-    const Vec<V> q = one_minus_square(l, f);
+    Vec<V> q;
+    decay_pair(mul(k_, s), f, q);
     Vec<V> w;
 #pragma unroll
     for (int k = 0; k < V; k++) {
