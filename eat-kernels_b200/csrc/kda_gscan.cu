@@ -16,11 +16,11 @@ static_assert(GATED_SCAN_TILE % S == 0 && TILE % GATED_SCAN_TILE == 0, "the stat
 template <int V>
 struct Shared {
   Vec<2 * V> map[2][WARPS][32];
-  float4 tile[2][MAX_CLUSTER][32];       // of the cluster's tiles, sent by their blocks: {F, F, U, U}; F < 0: the map is constant
   unsigned long long sent[2];            // barriers: the tiles' maps have arrived
   uint32_t starts[2][WARPS];             // whether a sequence starts there: the map is constant
   Tables<true> tables;
 };
+using Tile = float4[32];                 // of the cluster's tiles, sent by their blocks: {F, F, U, U}; F < 0: the map is constant
 
 struct Steps {             // bytes from a row to the fourth behind it
   long long x, r, i, y;
@@ -48,9 +48,11 @@ template <typename T, bool ASYNC, bool POWER, bool GATED>
 __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid_constant__ GatedScanParams p, const __grid_constant__ Steps g) {
   constexpr int V = CHANNELS<T, ASYNC>, NT = GATED ? 3 : 2;
   __shared__ Shared<V> sm;
-  extern __shared__ __align__(128) unsigned char raw[];              // ASYNC: [DEPTH][WARPS][NT] slices
   using Tokens = Slice<T, S>;
+  constexpr int RAW = ASYNC ? DEPTH * WARPS * NT * (int)sizeof(Tokens) : 0;
+  extern __shared__ __align__(128) unsigned char raw[];              // ASYNC: [DEPTH][WARPS][NT] slices; then [2][blocks of the cluster] tiles
   const uint32_t rank = cluster_rank(), size = cluster_size();
+  Tile* const tiles = reinterpret_cast<Tile*>(raw + RAW);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int c0 = (int)(blockIdx.x / size) * 32 * V, c = c0 + lane * V;
   const bool mine = c < p.C, chunk = c0 + lane % 8 * (16 / (int)sizeof(T)) < p.C;
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
   for (int round = 0; round < rounds; round++, t0 += step) {
     const int buf = round & 1, n = count<S>(t0, end);
     if (size > 1 && threadIdx.x == 0) bar_expect(&sm.sent[buf], size * 512);
-    const bool begins = !rejected && next < t0 + n, plain = !begins && n == S;        // begins: some sequence starts in the slice
+    const bool begins = !rejected && next < t0 + n, plain = !begins && n == S && t0 + S != end;       // begins: some sequence starts in the slice
     Vec<V> F, U;                                     // the slice's map
     uint32_t starts = 0;
     if (plain) {
@@ -224,13 +226,13 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
         const Vec<V> Ut = starts ? U : fma(F, Ub, U);
         Vec<V> Ft = least(mul(Fb, F));
         if (cut || starts) Ft = vec<V>(-1.0f);
-        for (uint32_t b = 0; b < size; b++) send(&sm.tile[buf][rank][lane], &sm.sent[buf], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
+        for (uint32_t b = 0; b < size; b++) send(&tiles[buf * size + rank][lane], &sm.sent[buf], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
       }
       if (!lost) lost = !bar_wait(&sm.sent[buf], round >> 1 & 1);
 #pragma unroll
       for (int b = 0; b < MAX_CLUSTER; b++) {
         if (b >= size) break;
-        const float4 m = sm.tile[buf][b][lane];
+        const float4 m = tiles[buf * size + b][lane];
         Vec<V> Fq, Uq;
         Fq.v[0] = m.x; Fq.v[V - 1] = m.y; Uq.v[0] = m.z; Uq.v[V - 1] = m.w;
         if (b == rank) enter = carry;
@@ -243,20 +245,24 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
       for (int k = 0; k < V; k++) p.tiles[(long long)(t0 / GATED_SCAN_TILE) * p.C + c + k] = h.v[k];
     }
     T* out = reinterpret_cast<T*>(p.out) + (long long)t0 * p.ldo + c;
-    if (!plain && n > 0) {                           // token by token, with the ends of sequences
+    if (!plain && n > 0) {                           // token by token, with the ends of sequences; u becomes the states
       Vec<V> v = h;
 #pragma unroll
       for (int s = 0; s < S; s++) {
         if (s < n) {
-          if (begins) {                              // one of the entries may be this token
-            const int q = lower(tables, 0, p.seq.N + 1, t0 + s);
-            if (q <= p.seq.N && tables.at(q) == t0 + s) finish<V>(p, tables, t0 + s, false, c, mine, v.v[0], v.v[V - 1]);
-          }
           v = pick(starts >> s & 1, u[s], fma(f[s], v, u[s]));
+          u[s] = v;
           if (mine) *reinterpret_cast<Pack<T, V>*>(out + s * p.ldo) = pack<T, V>(v.v);
         }
       }
-      if (t0 + n == end) finish<V>(p, tables, end, false, c, mine, v.v[0], v.v[V - 1]);
+      // entries within the tokens start some sequence
+      for (uint32_t bits = starts | (t0 + n == end ? 1u << n : 0); bits != 0; bits &= bits - 1) {
+        const int at = __ffs(bits) - 1;
+        Vec<V> before = h;
+#pragma unroll
+        for (int s = 0; s < S; s++) before = pick(s + 1 == at, u[s], before);
+        finish<V>(p, tables, t0 + at, false, c, mine, before.v[0], before.v[V - 1]);
+      }
     }
     if (!rejected) look(t0 + step, buf ^ 1);
     // The round's outputs and the next one's gates together: what the exponentials' unit takes longest for lies beside the rest.  Outputs
@@ -278,7 +284,6 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
       if (plain) Cursor<T, S>(p.out, p.ldo, t0, c0).store(x, g.y, S, chunk);
       __syncwarp();
     }
-    if (plain && t0 + n == end) finish<V>(p, tables, end, false, c, mine, h.v[0], h.v[V - 1]);
     ask(ASYNC ? 3 : 2, round + 1 & 1);
   }
   if (!rejected && end == 0 && rank == 0 && warp == 0) finish<V>(p, tables, 0, false, c, mine, 0.0f, 0.0f);
@@ -291,11 +296,11 @@ template <typename T, bool ASYNC, bool POWER, bool GATED>
 cudaError_t launch_gates(const GatedScanParams& p, cudaStream_t stream) {
   constexpr int V = CHANNELS<T, ASYNC>, B = sizeof(T);
   const long long slabs = (p.C + 32 * V - 1) / (32 * V);
-  constexpr int bytes = ASYNC ? DEPTH * WARPS * (GATED ? 3 : 2) * (int)sizeof(Slice<T, S>) : 0;
+  const auto bytes = [](int size) { return (ASYNC ? DEPTH * WARPS * (GATED ? 3 : 2) * (int)sizeof(Slice<T, S>) : 0) + 2 * size * (int)sizeof(Tile); };
   const auto kernel = kda_gated_scan_kernel<T, ASYNC, POWER, GATED>;
-  const int size = cluster_of(kernel, slabs, p.seq.T, TILE, THREADS, [](int) { return bytes; });
+  const int size = cluster_of(kernel, slabs, p.seq.T, TILE, THREADS, bytes);
   const Steps g = {4 * p.ldx * B, 4 * p.ldr * B, 4 * p.ldi * B, 4 * p.ldo * B};
-  return launch_clusters(kernel, slabs, size, THREADS, bytes, stream, p, g);
+  return launch_clusters(kernel, slabs, size, THREADS, bytes(size), stream, p, g);
 }
 
 template <typename T, bool ASYNC>

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
       const Vec<V> dh = add(gradient(s), e), x = token(0, s);
       const Gates<V> a = decay<T, POWER, V, true>(token(1, s), rb, k_);
       e = mul(f[s], dh);
-      Vec<V> b = mul(dh, x), gx = mul(dh, a.gain), gr, gi;
+      Vec<V> b = mul(dh, x), gx = mul(dh, a.gain), gr, gi = vec<V>(0.0f);
       if constexpr (GATED) {
         Vec<V> gate, ng;
         sigmoids<T, V>(token(3, s), ib, gate, ng);
