@@ -34,6 +34,20 @@ struct Steps {             // bytes from a row to the fourth behind it
   long long x, r, i, d, dx, dr, di;
 };
 
+// The row [N][C] of a table that belongs to the sequence of token t; zeros without a table.  Not inlined: its two dozen places in the
+// kernel would not fit the instruction cache.
+__device__ __noinline__ float2 state_of(const float* table, const Layout<false> l, uint32_t t, int C, int c, bool mine, int channels) {
+  float2 h = make_float2(0.0f, 0.0f);
+  if (table == nullptr) return h;
+  const int q = lower(l, 0, l.s.N + 1, t + 1) - 1;
+  const float* row = table + (long long)q * C + c;
+  if (mine) {
+    h.x = row[0];
+    if (channels > 1) h.y = row[1];
+  }
+  return h;
+}
+
 template <typename T, bool ASYNC, bool POWER, bool GATED>
 __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const __grid_constant__ GatedScanGradParams p, const __grid_constant__ Steps g) {
   constexpr int V = CHANNELS<T, ASYNC>, NT = GATED ? 4 : 3;
@@ -98,13 +112,11 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
         if (mine) p.dsrc[(long long)q * p.C + c + k] = p.dfinal != nullptr ? p.dfinal[(long long)q * p.C + c + k] : 0.0f;
     }
   }
-  auto state = [&](const float* table, uint32_t t) {  // of the sequence that token t belongs to; zeros without a table
-    Vec<V> h = vec<V>(0.0f);
-    if (table == nullptr) return h;
-    const int q = lower(tables, 0, p.seq.N + 1, t + 1) - 1;
-#pragma unroll
-    for (int k = 0; k < V; k++)
-      if (mine) h.v[k] = table[(long long)q * p.C + c + k];
+  auto state = [&](const float* table, uint32_t t) {
+    Vec<V> h;
+    const float2 v = state_of(table, tables, t, p.C, c, mine, V);
+    h.v[0] = v.x;
+    h.v[V - 1] = V > 1 ? v.y : v.x;
     return h;
   };
   uint32_t below = NEVER;                            // the last entry of cu_seqlens in front of the slices that are done
