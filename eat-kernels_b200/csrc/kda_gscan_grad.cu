@@ -7,6 +7,9 @@
 // e runs backwards over the rounds by the same maps as h does forwards (e in front of a slice = F e behind it + G).  The states h
 // are computed again from those that the forward pass kept in front of each tile, inside the block, at the same barrier.  A cluster
 // has all tokens of its channels, so the sums over tokens are complete in its first block, always in the same order.
+// The gates are computed twice, once for the maps and once for the gradients: kept, they would take 48 registers more.
+// Measured in bf16, both gates: 8 ragged sequences, 10 245 tokens of 4096 channels, 273 us (2.2 TB/s); 8192 tokens in one sequence 202 us, with
+// 4095 channels 301; 16 384 tokens of 512 channels in fp32, the form without rate, 98 us.  Slices of 12 tokens (twice the code): 325 us for the first.
 #include "kda_gscan.cuh"
 
 namespace kda {
