@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
 
   for (int round = 0; round < rounds; round++, t0 += step) {
     const int buf = round & 1, n = count<S>(t0, end);
-    if (size > 1 && threadIdx.x == 0) bar_expect(&sm.sent[buf], size * 512);
+    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], size * 512);
     const bool begins = !rejected && next < t0 + n, plain = !begins && n == S && t0 + S != end;       // begins: some sequence starts in the slice
     Vec<V> F, U;                                     // the slice's map
     uint32_t starts = 0;
@@ -224,13 +224,13 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
         if (some && sm.starts[buf][q] != 0) carry = Uq;
       }
     } else {
-      if (warp == WARPS - 1) {                       // it has the tile's map: to every block of the cluster
+      if (warp == WARPS - 1 && !lost) {              // it has the tile's map: to every block of the cluster
         const Vec<V> Ut = starts ? U : fma(F, Ub, U);
         Vec<V> Ft = least(mul(Fb, F));
         if (cut || starts) Ft = vec<V>(-1.0f);
         for (uint32_t b = 0; b < size; b++) send(&tiles[buf * size + rank][lane], &sm.sent[buf], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
       }
-      if (!lost) lost = !bar_wait(&sm.sent[buf], round >> 1 & 1);
+      if (!lost) lost = bar_lost(&sm.sent[buf], round >> 1 & 1);
 #pragma unroll
       for (int b = 0; b < MAX_CLUSTER; b++) {
         if (b >= size) break;
@@ -289,7 +289,11 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
     ask(ASYNC ? 3 : 2, round + 1 & 1);
   }
   if (!rejected && end == 0 && rank == 0 && warp == 0) finish<V>(p, tables, 0, false, c, mine, 0.0f, 0.0f);
-  if (lost) report(p.seq.status, SEQ_LOST);
+  if (lost) {                                        // others may still send here: those that have not left
+    report(p.seq.status, SEQ_LOST);
+    cluster_arrive();
+    cluster_wait();
+  }
   if (rejected && rank == 0 && warp == 0) finish<V>(p, tables, 0, true, c, mine, 0.0f, 0.0f);
   if (rejected || p.zero_pad) zero_rest<T, V>(p.out, p.ldo, end, p.seq.T, c, mine, rank, size);
 }

@@ -159,17 +159,19 @@ __device__ __forceinline__ bool bar_done(uint32_t b, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-// False where some two seconds ran out: what comes then is wrong, and ends
-__device__ __forceinline__ bool bar_wait(const void* bar, uint32_t parity) {
+// Called by a warp: whether the wait for a phase ran out, after some two seconds.  A block that has lost its cluster goes on to its end
+// without barriers, and sends nothing, so that the others lose it too; its results are wrong, and it says so.
+__device__ __forceinline__ bool bar_lost(const void* bar, uint32_t parity) {
   const uint32_t b = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
   unsigned long long begin = 0, now;
+  bool done = false;
   do {
-    for (int i = 0; i < 4096; i++)
-      if (bar_done(b, parity)) return true;
+    for (int i = 0; i < 4096 && !done; i++) done = bar_done(b, parity);
+    if (done) break;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (begin == 0) begin = now;
   } while (now - begin < WAIT_NS);
-  return false;
+  return __any_sync(0xffffffffu, !done);
 }
 
 // ---- one or two channels at once (two: one instruction)

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
 
   for (int round = rounds - 1; round >= 0; round--, t0 -= step) {
     const int use = rounds - 1 - round, buf = use & 1, n = count<S>(t0, end);
-    if (size > 1 && threadIdx.x == 0) bar_expect(&sm.sent[buf], size * 512);
+    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], size * 512);
     Vec<V> h = next_enter;
     if constexpr (ASYNC) {
       copies_wait<0>();
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
         carry = fma(Fw, carry, Gw);
         if (some && sm.cuts[buf][w] >> 16 != 0) carry = Gw;
       }
-    } else if (warp == 0) {                          // it has the tile's map: to every block of the cluster
+    } else if (warp == 0 && !lost) {                 // it has the tile's map: to every block of the cluster
       const Vec<V> Gt = ends ? G : fma(F, Gb, G);
       Vec<V> Ft = least(mul(Fb, F));
       if (cut || ends) Ft = vec<V>(-1.0f);
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
       }
     }
     if (size > 1) {
-      if (!lost) lost = !bar_wait(&sm.sent[buf], use >> 1 & 1);
+      if (!lost) lost = bar_lost(&sm.sent[buf], use >> 1 & 1);
 #pragma unroll
       for (int b = MAX_CLUSTER - 1; b >= 0; b--) {
         if (b >= size) continue;
