@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
       for (int s = 0; s < S; s++)
         if (s >= n) { f[s] = vec<V>(1.0f); u[s] = vec<V>(0.0f); }
       // sequences that start in the slice: the state they enter with joins the first token's term
-      if (begins) copies_wait<0>();                  // of `look`
+      if (begins) asm volatile("cp.async.wait_all;" ::: "memory");          // of `look`, whether they have joined a group or not
       for (int q = begins ? lower(tables, 0, p.seq.N + 1, t0) : p.seq.N; q < p.seq.N; q++) {
         const uint32_t b = tables.at(q);
         if (b >= t0 + n) break;

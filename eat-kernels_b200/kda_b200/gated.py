@@ -8,8 +8,8 @@
 Tokens, sequences, slots, `out` and `status` are those of the operators in `serving.py` (`status`: also the bit 64 = a wait inside
 the kernel ran out, results are wrong).  Gradients: with grad mode on, a call without
 `ssm_state_indices` and `out` whose tensors ask for some is recorded; calls that work on a pool or write the caller's `out` are serving
-calls and record nothing.  Backward passes return the same bits whenever they run, can be captured in a CUDA graph and are
-differentiable once."""
+calls and record nothing.  Backward passes return the same bits whenever they run, can be captured in a CUDA graph (while no
+eager graph of the same leaves lives, as torch wants it) and are differentiable once."""
 from __future__ import annotations
 
 import math
