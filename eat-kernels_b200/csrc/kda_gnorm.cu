@@ -368,8 +368,9 @@ Shape shape_of(int G, int D, int vec) {
 template <typename T, int VEC, int CH, bool GRAD>
 cudaError_t launch_one(const GroupNormParams& p, const dim3& grid, cudaStream_t stream) {
   const int bytes = GRAD && p.partial != nullptr && (p.shared || p.G < THREADS / p.lanes) ? 2 * 4 * (p.shared ? p.D : p.G * p.D) : 0;
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kda_group_norm_kernel<T, VEC, CH, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  constexpr int most = 2 * 4 * THREADS * VEC * CH;   // whatever this call needs: another thread may be about to launch one that needs more
+  if (GRAD && most > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kda_group_norm_kernel<T, VEC, CH, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
   }
   kda_group_norm_kernel<T, VEC, CH, GRAD><<<grid, THREADS, bytes, stream>>>(p);
@@ -379,8 +380,8 @@ cudaError_t launch_one(const GroupNormParams& p, const dim3& grid, cudaStream_t 
 template <typename T, bool GRAD>
 cudaError_t launch_wide(const GroupNormParams& p, const dim3& grid, cudaStream_t stream) {
   const int bytes = GRAD && p.partial != nullptr ? 8 * p.D : 0;
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kda_group_norm_wide_kernel<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (GRAD) {
+    const cudaError_t e = cudaFuncSetAttribute(kda_group_norm_wide_kernel<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * GROUP_NORM_MAX_WIDTH);
     if (e != cudaSuccess) return e;
   }
   kda_group_norm_wide_kernel<T, GRAD><<<grid, THREADS, bytes, stream>>>(p);

@@ -306,7 +306,7 @@ cudaError_t launch_gates(const GatedScanParams& p, cudaStream_t stream) {
   const auto kernel = kda_gated_scan_kernel<T, ASYNC, POWER, GATED>;
   const int size = cluster_of(kernel, slabs, p.seq.T, TILE, THREADS, bytes);
   const Steps g = {4 * p.ldx * B, 4 * p.ldr * B, 4 * p.ldi * B, 4 * p.ldo * B};
-  return launch_clusters(kernel, slabs, size, THREADS, bytes(size), stream, p, g);
+  return launch_clusters(kernel, slabs, size, THREADS, bytes(size), bytes(MAX_CLUSTER), stream, p, g);
 }
 
 template <typename T, bool ASYNC>

@@ -456,7 +456,7 @@ int cluster_of(K kernel, long long slabs, long long T, int tile, int threads, B 
       configure(cfg, attr, size, size, threads, bytes(size), nullptr);
       int n = 0;
       if (size > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (bytes(size) > 0) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(size));
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(MAX_CLUSTER));
       if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
         n = 0;
         cudaGetLastError();
@@ -469,20 +469,19 @@ int cluster_of(K kernel, long long slabs, long long T, int tile, int threads, B 
 }
 
 template <typename K, typename... P>
-cudaError_t launch_clusters(K kernel, long long slabs, int size, int threads, int bytes, cudaStream_t stream, const P&... p) {
+cudaError_t launch_clusters(K kernel, long long slabs, int size, int threads, int bytes, int most, cudaStream_t stream, const P&... p) {
   if (slabs * size > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (bytes > 0) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-  }
+  // the same for all sizes: another thread may be about to launch a larger one
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e != cudaSuccess) return e;
   if (size > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   configure(cfg, attr, slabs * size, size, threads, bytes, stream);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);
+  e = cudaLaunchKernelEx(&cfg, kernel, p...);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 

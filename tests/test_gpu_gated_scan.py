@@ -264,6 +264,29 @@ def test_steps_with_repeats_without_slots_and_without_rows():
     assert y.shape == (1, 0, C) and torch.equal(final, pool[:3])
 
 
+def test_threads_with_calls_of_different_sizes():
+    """Clusters of different sizes of one kernel, launched side by side."""
+    import threading
+
+    import kda_b200
+    gen = generator(23)
+    args = [inputs(gen, T, 64, BF, "power", 1) for T in (40, 150, 700, 3000)]
+    want, got = [kda_b200.gated_scan(*a)[0] for a in args], [None] * 4
+    torch.cuda.synchronize()
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got[k] = kda_b200.gated_scan(*args[k])[0]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_prompt_then_steps_is_the_whole_prompt():
     import kda_b200
     gen, C = generator(22), 128
