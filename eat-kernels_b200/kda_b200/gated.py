@@ -6,10 +6,11 @@
     y = group_norm(x, groups, weight, bias, z, activation="silu")                                  # differentiable
 
 Tokens, sequences, slots, `out` and `status` are those of the operators in `serving.py` (`status`: also the bit 64 = a wait inside
-the kernel ran out, results are wrong).  Gradients: with grad mode on, a call without
-`ssm_state_indices` and `out` whose tensors ask for some is recorded; calls that work on a pool or write the caller's `out` are serving
-calls and record nothing.  Backward passes return the same bits whenever they run, can be captured in a CUDA graph (while no
-eager graph of the same leaves lives, as torch wants it) and are differentiable once."""
+the kernel ran out, results are wrong; a recorded call's backward pass reports into the same tensor, and without one nothing does).
+
+Gradients: with grad mode on, a call without `ssm_state_indices` and `out` whose tensors ask for some is recorded; calls that work on a
+pool or write the caller's `out` are serving calls and record nothing.  Backward passes return the same bits whenever they run, can be
+captured in a CUDA graph (while no eager graph of the same leaves lives, as torch wants it) and are differentiable once."""
 from __future__ import annotations
 
 import math
@@ -89,7 +90,7 @@ def _scan(x, r, i, rate, r_bias, i_bias, state, cu_seqlens, slots, out, status, 
     return _Ready(name, dev, args, given, fresh, result, [9, 10] + [6] * in_place, keep=(x, r, i, rate, r_bias, i_bias, src, cu, slots))
 
 
-def _scan_grad(x, r, i, rate, r_bias, i_bias, state, cu, tiles, dy, dfinal, rate_scale, wants):
+def _scan_grad(x, r, i, rate, r_bias, i_bias, state, cu, tiles, dy, dfinal, status, rate_scale, wants):
     T, dev, channels, rate, r_bias, i_bias = _gated_inputs(x, r, i, rate, r_bias, i_bias)
     N = 1 if cu is None else cu.numel() - 1
     cu, _ = _layout(dev, cu)
@@ -100,16 +101,19 @@ def _scan_grad(x, r, i, rate, r_bias, i_bias, state, cu, tiles, dy, dfinal, rate
     dy, lddy = _rows(dy) if dy is not None else (None, 0)
     sums = [torch.empty(channels, dtype=torch.float32, device=dev) if wanted else None for wanted in wants[:3]]
     dsrc = torch.empty((N, channels), dtype=torch.float32, device=dev) if wants[3] else None
+    if status is not None:
+        _reject_aliasing([_status(dev, status)], [("x", x), ("r", r), ("i", i), ("rate", rate), ("r_bias", r_bias), ("i_bias", i_bias),
+                                                  ("initial_state", state), ("cu_seqlens", cu), ("dy", dy), ("dfinal", dfinal)])
     args = _cabi.KdaGatedScanGradArgs(_ptr(x), _ptr(r), _ptr(i), _ptr(dy), _ptr(dx), _ptr(dr), _ptr(di), _ptr(rate), _ptr(r_bias), _ptr(i_bias),
                                       _ptr(tiles), _ptr(state), _ptr(dfinal), _ptr(dsrc), *map(_ptr, sums), ldx, ldr, ldi, lddy, channels, channels,
-                                      channels, _sequences(T, N, cu, None, N, None, 1), rate_scale, channels, TYPES[x.dtype])
-    given = {k: [f] for k, f in enumerate(("x", "r", "i", "rate", "r_bias", "i_bias", "src", "seq.cu_seqlens", "tiles", "dy", "dfinal"))}
+                                      channels, _sequences(T, N, cu, None, N, status, 1), rate_scale, channels, TYPES[x.dtype])
+    given = {k: [f] for k, f in enumerate(("x", "r", "i", "rate", "r_bias", "i_bias", "src", "seq.cu_seqlens", "tiles", "dy", "dfinal", "seq.status"))}
     fresh, result = [], []
     for t, field in ((dx, "dx"), (dr, "dr"), (di, "di"), *zip(sums, ("drate", "dr_bias", "di_bias")), (dsrc, "dsrc")):
         if t is not None:
             fresh.append((t, [field]))
             result.append(-len(fresh))
-    return _Ready("kda_gated_scan_grad_launch", dev, args, given, fresh, tuple(result), keep=(x, r, i, rate, r_bias, i_bias, state, cu, tiles, dy, dfinal))
+    return _Ready("kda_gated_scan_grad_launch", dev, args, given, fresh, tuple(result), [11], keep=(x, r, i, rate, r_bias, i_bias, state, cu, tiles, dy, dfinal))
 
 
 class _GatedScan(torch.autograd.Function):
@@ -117,7 +121,7 @@ class _GatedScan(torch.autograd.Function):
     def forward(ctx, x, r, i, rate, r_bias, i_bias, state, cu_seqlens, status, rate_scale):
         y, final, tiles = _call(_scan, (x, r, i, rate, r_bias, i_bias, state, cu_seqlens, None, None, status), rate_scale, False, True)
         ctx.set_materialize_grads(False)
-        ctx.rate_scale = rate_scale
+        ctx.rate_scale, ctx.status = rate_scale, status          # not a saved tensor: calls write it
         ctx.save_for_backward(x, r, i, rate, r_bias, i_bias, state, cu_seqlens, tiles)
         return y, final
 
@@ -128,7 +132,7 @@ class _GatedScan(torch.autograd.Function):
         if dy is None and dfinal is None:
             return (None,) * 10
         wants = (need[3], need[4], need[5], need[6])
-        grads = iter(_call(_scan_grad, (*tensors, dy, dfinal), ctx.rate_scale, wants))
+        grads = iter(_call(_scan_grad, (*tensors, dy, dfinal, ctx.status), ctx.rate_scale, wants))
         dx, dr = next(grads), next(grads)
         di = next(grads) if tensors[2] is not None else None
         params = [next(grads).view_as(tensors[3 + k]) if wants[k] else None for k in range(3)]
