@@ -28,7 +28,7 @@ struct Steps {             // bytes from a row to the fourth behind it
   long long x, r, i, y;
 };
 
-// Stores the final states of the sequences that end at t.  h: the state in front of t.
+// Stores the final states of the sequences that end at t, where they change.  h: the state in front of t.
 template <int V>
 __device__ __forceinline__ void finish(const GatedScanParams& p, const Layout<true> l, uint32_t t, bool all_empty, int c, bool mine, float h0, float h1) {
   if (p.dst == nullptr) return;
@@ -37,9 +37,8 @@ __device__ __forceinline__ void finish(const GatedScanParams& p, const Layout<tr
     if (!all_empty && l.at(j) != t) return;
     if (j == 0) continue;
     const bool empty = all_empty || l.at(j - 1) == t;
-    if (empty && p.src == p.dst) continue;
-    const long long slot = claim(l, j - 1);
-    if (slot < 0 || !mine) continue;
+    const long long slot = claim(l, j - 1);          // of an empty one too: a bad entry is reported
+    if (slot < 0 || !mine || (empty && p.src == p.dst)) continue;
 #pragma unroll
     for (int k = 0; k < V; k++)
       p.dst[slot * p.dst_stride + c + k] = !empty ? h[k] : (p.src != nullptr ? p.src[slot * p.src_stride + c + k] : 0.0f);

@@ -1,8 +1,9 @@
-"""What the gated linear recurrence reports through `status` from its backward passes."""
+"""What the gated linear recurrence reports through `status` from its backward passes and of empty sequences."""
 import pytest
 import torch
 
-from serving_testlib import DEV, cu_of
+from serving_testlib import DEV, cu_of, generator, randn
+from test_gpu_gated_scan import inputs
 from test_gpu_gated_scan_grad import case, leaves
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,29 @@ def test_backward_passes_report_into_the_calls_status(dtype):
         out = kda_b200.gated_scan(*v, cu_of([30, 50]), status=status)
         torch.autograd.grad(out, v, (dy, dfinal))
         assert int(status) == 0
+
+
+def test_slots_of_empty_sequences_are_checked():
+    """As by the convolution and the selective scan: out of range or a repeat is reported whether the sequence has tokens or not, and
+    whether the layout is rejected or not; a sequence that names the slot of an empty one is a repeat."""
+    import kda_b200
+    gen, C = generator(32), 64
+    for lens, slots, bits in (([3, 0], [0, 99], 2), ([3, 0], [1, 1], 2), ([0, 3], [1, 1], 2), ([0, 3, 0], [-1, 2, 3], 2), ([0, 0], [4, 4], 2), ([0, 0], [4, 5], 0),
+                              ([0, 3, 0, 200, 0], [3, 0, 2, 1, 4], 0), ([0, 3, 0, 200, 0], [3, 0, 3, 1, 4], 2)):
+        x, r, i, rate, rb, ib = inputs(gen, sum(lens), C, F32, "power", 1)
+        pool, table = randn(gen, 6, C), torch.tensor(slots, device=DEV)
+        before, status = pool.clone(), fresh_status()
+        kda_b200.gated_scan(x, r, i, rate, rb, ib, pool, cu_of(lens), ssm_state_indices=table, status=status)
+        assert int(status) == bits, (lens, slots)
+        kept = [s for s in range(6) if s not in [s for s, n in zip(slots, lens) if n > 0]]
+        assert torch.equal(pool[kept], before[kept])
+        other, word = randn(gen, 6, 3, C), fresh_status()
+        kda_b200.short_conv(x, torch.ones(C, 4, device=DEV), None, other, cu_of(lens), ssm_state_indices=table, status=word)
+        assert int(word) == bits
+    x, r, i, rate, rb, ib = inputs(gen, 8, C, F32, "power", 1)
+    for slots, bits in (([0, 1], 1), ([0, 6], 3), ([2, 2], 3)):
+        pool, table, status, word = randn(gen, 6, C), torch.tensor(slots, device=DEV), fresh_status(), fresh_status()
+        before = pool.clone()
+        kda_b200.gated_scan(x, r, i, rate, rb, ib, pool, torch.tensor([0, 9, 8], device=DEV), ssm_state_indices=table, status=status)
+        kda_b200.short_conv(x, torch.ones(C, 4, device=DEV), None, randn(gen, 6, 3, C), torch.tensor([0, 9, 8], device=DEV), ssm_state_indices=table, status=word)
+        assert int(status) == bits and int(word) == bits and torch.equal(pool, before)
