@@ -441,7 +441,7 @@ int kda_prefill_plan_counts(const KdaPrefillArgs* a, int32_t* counts, void* stre
 }
 
 int kda_debug_configure(int64_t wait_limit_us, int32_t flags, void* prof_counters) {
-  if (wait_limit_us < 0 || (flags & ~(kda::DBG_STALL_V_STREAM | kda::DBG_FORCE_CAND_MASK))) return KDA_ERR_ARG;
+  if (wait_limit_us < 0 || (flags & ~(kda::DBG_STALL_V_STREAM | kda::DBG_MORE_MAPS | kda::DBG_FORCE_CAND_MASK))) return KDA_ERR_ARG;
   g_wait_limit_ns = (unsigned long long)wait_limit_us * 1000ull;
   g_debug_flags = flags;
   g_prof = reinterpret_cast<unsigned long long*>(prof_counters);
@@ -538,6 +538,13 @@ int scan_launch(const KdaScanArgs* a, bool step, void* stream) {
 
 static_assert(KDA_GATED_SCAN_TILE == kda::GATED_SCAN_TILE && KDA_GROUP_NORM_MAX_WIDTH == kda::GROUP_NORM_MAX_WIDTH, "limits as documented");
 
+// Waits of the gated scan: two seconds, or what kda_debug_configure says
+template <typename P>
+void bound_waits(P& p) {
+  p.wait_ns = g_wait_limit_ns != 0 ? g_wait_limit_ns : 2000000000ull;
+  p.more_maps = (g_debug_flags & kda::DBG_MORE_MAPS) != 0;
+}
+
 int gated_scan_launch(const KdaGatedScanArgs* a, bool step, void* stream) {
   if (a == nullptr || a->C < 1 || !known_type(a->type)) return KDA_ERR_ARG;
   const int rc = check_sequences(a->seq, step);
@@ -557,6 +564,7 @@ int gated_scan_launch(const KdaGatedScanArgs* a, bool step, void* stream) {
   p.seq = seq_table(a->seq);
   p.ldx = a->ldx; p.ldr = a->ldr; p.ldi = a->i ? a->ldi : 0; p.ldo = a->ldo; p.src_stride = a->src_slot_stride; p.dst_stride = a->dst_slot_stride;
   p.rate_scale = a->rate_scale; p.C = a->C; p.zero_pad = a->seq.zero_rest != 0;
+  bound_waits(p);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return launched(step ? kda::launch_gated_scan_step(p, a->type, s) : kda::launch_gated_scan(p, a->type, s));
 }
@@ -687,6 +695,7 @@ int kda_gated_scan_grad_launch(const KdaGatedScanGradArgs* a, void* stream) {
   p.seq = seq_table(seq);
   p.ldx = a->ldx; p.ldr = a->ldr; p.ldi = a->i ? a->ldi : 0; p.lddy = a->dy ? a->lddy : 0; p.lddx = a->lddx; p.lddr = a->lddr; p.lddi = a->i ? a->lddi : 0;
   p.rate_scale = a->rate_scale; p.C = a->C;
+  bound_waits(p);
   return launched(kda::launch_gated_scan_grad(p, a->type, reinterpret_cast<cudaStream_t>(stream)));
 }
 

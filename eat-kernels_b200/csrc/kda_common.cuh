@@ -68,8 +68,9 @@ struct ChunkParams {
   unsigned long long* prof;           // cycle counters of profiling builds (KDA_PROF), else unused
 };
 
-// Diagnostic switches of the tcgen05 kernel (set only through kda_debug_configure).
+// Diagnostic switches of the tcgen05 kernel and of the gated scan (set only through kda_debug_configure).
 constexpr int DBG_STALL_V_STREAM = 1;  // the v tiles never count as arrived: their waiters run into the bound
+constexpr int DBG_MORE_MAPS = 2;       // gated scan: blocks wait for a map that nobody sends and run into the bound
 // bits 8-11: k + 1 makes the device planner take candidate k of its piece lengths (a tuning aid for the cost model)
 constexpr int DBG_FORCE_CAND_SHIFT = 8, DBG_FORCE_CAND_MASK = 0xf00;
 

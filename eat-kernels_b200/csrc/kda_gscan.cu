@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
 
   for (int round = 0; round < rounds; round++, t0 += step) {
     const int buf = round & 1, n = count<S>(t0, end);
-    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], size * 512);
+    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], (size + p.more_maps) * 512);
     const bool begins = !rejected && next < t0 + n, plain = !begins && n == S && t0 + S != end;       // begins: some sequence starts in the slice
     Vec<V> F, U;                                     // the slice's map
     uint32_t starts = 0;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_kernel(const __grid
         if (cut || starts) Ft = vec<V>(-1.0f);
         for (uint32_t b = 0; b < size; b++) send(&tiles[buf * size + rank][lane], &sm.sent[buf], b, make_float4(Ft.v[0], Ft.v[V - 1], Ut.v[0], Ut.v[V - 1]));
       }
-      if (!lost) lost = bar_lost(&sm.sent[buf], round >> 1 & 1);
+      if (!lost) lost = bar_lost(&sm.sent[buf], round >> 1 & 1, p.wait_ns);
 #pragma unroll
       for (int b = 0; b < MAX_CLUSTER; b++) {
         if (b >= size) break;

@@ -24,7 +24,6 @@ namespace kda {
 namespace gscan {
 
 constexpr int MAX_CLUSTER = 16, MAX_DEVICES = 64;
-constexpr unsigned long long WAIT_NS = 2000000000ULL;
 constexpr uint32_t NEVER = 0xffffffffu;
 
 // A product of decays that underflows to zero is taken as the smallest positive number, so that an infinite state stays infinite, as it
@@ -159,18 +158,18 @@ __device__ __forceinline__ bool bar_done(uint32_t b, uint32_t parity) {
                : "memory");
   return done != 0;
 }
-// Called by a warp: whether the wait for a phase ran out, after some two seconds.  A block that has lost its cluster goes on to its end
+// Called by a warp: whether the wait for a phase ran out, after `limit` ns.  A block that has lost its cluster goes on to its end
 // without barriers, and sends nothing, so that the others lose it too; its results are wrong, and it says so.
-__device__ __forceinline__ bool bar_lost(const void* bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_lost(const void* bar, uint32_t parity, unsigned long long limit) {
   const uint32_t b = static_cast<uint32_t>(__cvta_generic_to_shared(bar));
   unsigned long long begin = 0, now;
   bool done = false;
   do {
-    for (int i = 0; i < 4096 && !done; i++) done = bar_done(b, parity);
+    for (int i = 0; i < 64 && !done; i++) done = bar_done(b, parity);
     if (done) break;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (begin == 0) begin = now;
-  } while (now - begin < WAIT_NS);
+  } while (now - begin < limit);
   return __any_sync(0xffffffffu, !done);
 }
 

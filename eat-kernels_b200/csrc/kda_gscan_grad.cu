@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
 
   for (int round = rounds - 1; round >= 0; round--, t0 -= step) {
     const int use = rounds - 1 - round, buf = use & 1, n = count<S>(t0, end);
-    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], size * 512);
+    if (size > 1 && threadIdx.x == 0 && !lost) bar_expect(&sm.sent[buf], (size + p.more_maps) * 512);
     Vec<V> h = next_enter;
     if constexpr (ASYNC) {
       copies_wait<0>();
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 2) kda_gated_scan_grad_kernel(const _
       }
     }
     if (size > 1) {
-      if (!lost) lost = bar_lost(&sm.sent[buf], use >> 1 & 1);
+      if (!lost) lost = bar_lost(&sm.sent[buf], use >> 1 & 1, p.wait_ns);
 #pragma unroll
       for (int b = MAX_CLUSTER - 1; b >= 0; b--) {
         if (b >= size) continue;

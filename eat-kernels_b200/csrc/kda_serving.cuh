@@ -64,6 +64,8 @@ struct GatedScanParams {
   float rate_scale;
   int C, zero_pad;
   int tile;                // step: rows of a block, set by the launcher
+  int more_maps;           // diagnostic: 1 = blocks wait for a map that nobody sends
+  unsigned long long wait_ns;            // bound of a wait for maps
 };
 cudaError_t launch_gated_scan(const GatedScanParams& p, int type, cudaStream_t stream);
 cudaError_t launch_gated_scan_step(const GatedScanParams& p, int type, cudaStream_t stream);
@@ -81,6 +83,8 @@ struct GatedScanGradParams {
   long long ldx, ldr, ldi, lddy, lddx, lddr, lddi;
   float rate_scale;
   int C;
+  int more_maps;           // as above
+  unsigned long long wait_ns;
 };
 cudaError_t launch_gated_scan_grad(const GatedScanGradParams& p, int type, cudaStream_t stream);
 

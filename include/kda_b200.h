@@ -440,11 +440,13 @@ const char* kda_version(void);
 
 /* Diagnostics for tests and profiling runs; process-wide, not thread-safe, never needed by a product call.  No
  * counterpart in the reference (whose waits trap after 60 s, kda/b200/README.md:169-171).
- *   wait_limit_us  bound of every wait inside the tcgen05 kernel (0 = the built-in two seconds).  When a wait runs out
- *                  the kernel finishes its control flow, waits for its own copies and tensor-core work, frees tensor
- *                  memory and writes a code to status[2].
+ *   wait_limit_us  bound of every wait inside the tcgen05 kernel and of the gated scan's and its gradients' waits for the
+ *                  other blocks of a cluster (0 = the built-in two seconds).  When a wait runs out the tcgen05 kernel finishes
+ *                  its control flow, waits for its own copies and tensor-core work, frees tensor memory and writes a code
+ *                  to status[2]; the gated scan goes on to its end and reports KDA_STATUS_LOST.
  *   flags          bit 0: the arrival of the v tiles is never signalled to their consumers, so that a waiter runs into
  *                  the bound (used to test the give-up path without faulting or hanging anything); 0 = normal.
+ *                  bit 1: the same for the gated scan: the blocks of a cluster wait for one message more than is sent.
  *                  bits 8-11: k + 1 makes the device planner cut with candidate k of its piece lengths (the longest
  *                  sequence in 2, 3, 4, 6, 8, 12, 16, 24, 32 pieces) instead of asking its cost model (tuning aid).
  *   prof_counters  device uint64[1024] receiving per-role cycle counters in builds compiled with -DKDA_PROF; NULL else. */

@@ -57,3 +57,35 @@ def test_slots_of_empty_sequences_are_checked():
         kda_b200.gated_scan(x, r, i, rate, rb, ib, pool, torch.tensor([0, 9, 8], device=DEV), ssm_state_indices=table, status=status)
         kda_b200.short_conv(x, torch.ones(C, 4, device=DEV), None, randn(gen, 6, 3, C), torch.tensor([0, 9, 8], device=DEV), ssm_state_indices=table, status=word)
         assert int(status) == bits and int(word) == bits and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("C", [64, 33], ids=["copies", "one by one"])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_a_wait_that_runs_out_is_reported(dtype, C):
+    """The blocks of a cluster wait for each other's maps.  With the diagnostic switch under which they wait for one more than is sent,
+    all run into the (shortened) bound: the call still ends, says so, and the next one is right.  Nothing faults or hangs."""
+    import kda_b200
+    from kda_b200 import _cabi
+    lens = [1700, 1, 1299]
+    tensors, dy, dfinal = case(lens, C, dtype, "power", 1, 33)
+    v, cu, status = leaves(*tensors), cu_of(lens), fresh_status()
+    want = kda_b200.gated_scan(*v, cu, status=status)
+    grads = torch.autograd.grad(want, v, (dy, dfinal), retain_graph=True)
+    assert int(status) == 0
+    for back in (False, True):
+        status.zero_()
+        torch.cuda.synchronize()
+        assert _cabi.lib().kda_debug_configure(200, 2, None) == 0             # 200 us
+        try:
+            if back:
+                torch.autograd.grad(want, v, (dy, dfinal), retain_graph=True)
+            else:
+                kda_b200.gated_scan(*tensors, cu, status=status)
+            torch.cuda.synchronize()
+        finally:
+            assert _cabi.lib().kda_debug_configure(0, 0, None) == 0
+        assert int(status) == 64
+    status.zero_()
+    again = kda_b200.gated_scan(*v, cu, status=status)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, v, (dy, dfinal)), grads)) and int(status) == 0
