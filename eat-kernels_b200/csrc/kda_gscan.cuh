@@ -321,13 +321,14 @@ __device__ __forceinline__ Vec<2> values(const Pack<__nv_bfloat16, 2>& p) {     
 
 // Of V channels: sigmoid and, with BOTH, 1 minus it, both to relative accuracy.  The approximate exponential and reciprocal are good to
 // 2^-22; for 32-bit tokens the exponential's argument is taken in two parts, since its rounding would be off by as much again for each unit of x.
+// Alone, the sigmoid of an infinitely low x is zero; with the other one it stays at 2^-126, so that the product that makes that one is 1.
 template <typename T, int V, bool BOTH = true>
 __device__ __forceinline__ void sigmoids(Vec<V> x, Vec<V> bias, Vec<V>& s, Vec<V>& n) {
 #pragma unroll
   for (int k = 0; k < V; k++) {
     float e;
     if constexpr (sizeof(T) == 4) {
-      const float v = -(x.v[k] + bias.v[k]), hi = min_or_nan(v * LOG2E_F, 126.0f);
+      const float v = -(x.v[k] + bias.v[k]), hi = BOTH ? min_or_nan(v * LOG2E_F, 126.0f) : v * LOG2E_F;
       const float lo = fmaf(v, LOG2E_F, -hi) + v * LOG2E_REST;
       e = ex2_fast(hi);
       e = fabsf(hi) < 126.0f ? fmaf(e, lo * LN2_F, e) : e;
@@ -390,7 +391,8 @@ __device__ __forceinline__ Gates<V> decay(Vec<V> r, Vec<V> bias, Vec<V> k_) {
 }
 
 // A token's decay f and term u.  With both gates in 16 bits u = sqrt(q) / (1 + e^-i) x, q = 1 - f^2, takes one reciprocal root,
-// sqrt(q) / a = q rsqrt(q a^2): five operations of the special-function unit instead of six.  (An input gate below 2^-60 counts as that.)
+// sqrt(q) / a = q rsqrt(q a^2): five operations of the special-function unit instead of six.  (An input gate below 2^-64 counts as shut:
+// the square is infinite, a itself is not, so that q = 0 stays 0.)
 template <typename T, bool POWER, bool GATED, int V>
 __device__ __forceinline__ void token_terms(Vec<V> x, Vec<V> r, Vec<V> i, Vec<V> rb, Vec<V> ib, Vec<V> k_, Vec<V>& f, Vec<V>& u) {
   if constexpr (POWER && GATED && sizeof(T) == 2) {
@@ -401,7 +403,7 @@ __device__ __forceinline__ void token_terms(Vec<V> x, Vec<V> r, Vec<V> i, Vec<V>
     Vec<V> w;
 #pragma unroll
     for (int k = 0; k < V; k++) {
-      const float a = ex2_fast(min_or_nan(fmaf(i.v[k], -LOG2E_F, ib.v[k]), 60.0f)) + 1.0f;
+      const float a = ex2_fast(min_or_nan(fmaf(i.v[k], -LOG2E_F, ib.v[k]), 126.0f)) + 1.0f;
       w.v[k] = rsqrt_fast(fmaf(q.v[k] * a, a, 2.0e-38f));
     }
     u = mul(mul(q, w), x);

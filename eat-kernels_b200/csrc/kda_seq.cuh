@@ -180,18 +180,19 @@ __device__ __forceinline__ float min_or_nan(float a, float b) {       // NaN if 
 }
 
 // sigmoid(x + bias) and 1 minus it, both to relative accuracy.  16-bit tokens: the approximate exponential and reciprocal, some
-// 2^-21 off, with `bias` scaled by -log2(e).  e^-x stops at 2^126, behind which the sigmoid is 2^-126 and its product with e^-x still 1.
+// 2^-21 off, with `bias` scaled by -log2(e).  Where e^-x leaves 2^126 behind, 1 minus the sigmoid is 1, and an infinitely low x has
+// the sigmoid zero.
 template <typename T>
 __device__ __forceinline__ void sigmoid_pair(float x, float bias, float& s, float& n) {
   float e;
   if constexpr (sizeof(T) == 4) {
-    e = expf(min_or_nan(-(x + bias), 87.0f));
+    e = expf(-(x + bias));
     s = 1.0f / (1.0f + e);
   } else {
-    e = ex2_fast(min_or_nan(fmaf(x, -1.4426950408889634f, bias), 126.0f));
+    e = ex2_fast(fmaf(x, -1.4426950408889634f, bias));
     s = rcp_fast(1.0f + e);
   }
-  n = e * s;
+  n = e >= 0x1p126f ? 1.0f : e * s;
 }
 
 }  // namespace kda
