@@ -545,8 +545,12 @@ void bound_waits(P& p) {
   p.more_maps = (g_debug_flags & kda::DBG_MORE_MAPS) != 0;
 }
 
+// Channels whose blocks, of up to 128 channels on top, are still counted in 32 bits
+constexpr int GATED_SCAN_MAX_CHANNELS = 0x7fffffff / 2;
+
 int gated_scan_launch(const KdaGatedScanArgs* a, bool step, void* stream) {
   if (a == nullptr || a->C < 1 || !known_type(a->type)) return KDA_ERR_ARG;
+  if (a->C > GATED_SCAN_MAX_CHANNELS) return KDA_ERR_LIMIT;
   const int rc = check_sequences(a->seq, step);
   if (rc != KDA_OK) return rc;
   if (!whole(a->type, a->x, a->r, a->i, a->out)) return KDA_ERR_ARG;
@@ -675,6 +679,7 @@ int kda_gated_scan_step_launch(const KdaGatedScanArgs* a, void* stream) { return
 
 int kda_gated_scan_grad_launch(const KdaGatedScanGradArgs* a, void* stream) {
   if (a == nullptr || a->C < 1 || !known_type(a->type) || a->seq.slots) return KDA_ERR_ARG;
+  if (a->C > GATED_SCAN_MAX_CHANNELS) return KDA_ERR_LIMIT;
   KdaSequences seq = a->seq;
   seq.n_slots = seq.N;                               // one state a sequence
   const int rc = check_sequences(seq, false);

@@ -35,6 +35,8 @@ def _gated_inputs(x, r, i, rate, r_bias, i_bias):
     dev, channels = x.device, x.shape[2]
     if x.dtype not in TYPES:
         raise _err(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    if channels > INT32_MAX // 2:
+        raise _err(f"x has more than {INT32_MAX // 2} channels")
     if r is None:
         raise _err("r is required")
     if i_bias is not None and i is None:

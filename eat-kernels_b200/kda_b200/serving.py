@@ -177,6 +177,8 @@ def _lead(t, name, width_dims):
         raise _err(f"{name} must be a packed token tensor [1, T{', .' * width_dims}], got {list(t.shape)}")
     if t.shape[1] > INT32_MAX:
         raise _err(f"{name} has more than 2^31 - 1 tokens")
+    if t.shape[2:].numel() > INT32_MAX:                # argument blocks hold 32 bits
+        raise _err(f"{name} has more than 2^31 - 1 channels")
     return t.shape[1]
 
 

@@ -341,7 +341,7 @@ typedef struct KdaGatedScanArgs {
   int64_t ldx, ldr, ldi, ldo, src_slot_stride, dst_slot_stride;
   KdaSequences seq;
   float rate_scale;
-  int32_t C, type;
+  int32_t C, type;         /* C < 2^30 */
 } KdaGatedScanArgs;
 #define KDA_GATED_SCAN_TILE 48
 int kda_gated_scan_launch(const KdaGatedScanArgs* args, void* stream);

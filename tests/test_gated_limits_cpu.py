@@ -1,0 +1,20 @@
+"""Arguments of the gated linear recurrence and the group norm that 32-bit fields of the entry points cannot hold."""
+import pytest
+import torch
+
+from test_gated_cpu import _grad, _scan, _seq, lib  # noqa: F401
+
+
+def test_channels_that_index_arithmetic_cannot_hold(lib):  # noqa: F811
+    """Refused before anything is launched: blocks and channels are counted in 32 bits, with a block's width on top."""
+    wide = 1 << 31
+    for make, names in ((_scan, ["kda_gated_scan_launch", "kda_gated_scan_step_launch"]), (_grad, ["kda_gated_scan_grad_launch"])):
+        for name in names:
+            for C in ((1 << 30) + 1, (1 << 31) - 1):
+                a = make()
+                a.C = C
+                for field, _ in a._fields_:
+                    if field.startswith("ld") or field.endswith("_stride"):
+                        setattr(a, field, wide)
+                a.seq = _seq(2, 2) if "step" in name else a.seq
+                assert getattr(lib, name)(a, None) == -4, (name, C)
