@@ -48,10 +48,13 @@ def _gated_inputs(x, r, i, rate, r_bias, i_bias):
     return T, dev, channels, _vector(rate, "rate", channels), _vector(r_bias, "r_bias", channels), _vector(i_bias, "i_bias", channels)
 
 
+F32 = torch.finfo(torch.float32)
+
+
 def _scale(rate_scale):
     scale = float(rate_scale)
-    if not (math.isfinite(scale) and scale > 0.0):
-        raise _err(f"rate_scale must be a positive number, got {rate_scale!r}")
+    if not F32.tiny <= scale <= F32.max:               # the kernels take it in 32 bits
+        raise _err(f"rate_scale must be a positive number of fp32's range, got {rate_scale!r}")
     return scale
 
 
@@ -264,8 +267,8 @@ def group_norm(x, groups=None, weight=None, bias=None, z=None, *, activation=Non
     if groups is not None and (isinstance(groups, bool) or not isinstance(groups, int)):
         raise _err(f"groups must be a whole number, got {groups!r}")
     eps = float(eps)
-    if not (math.isfinite(eps) and eps >= 0.0):
-        raise _err(f"eps must be a number of zero or more, got {eps!r}")
+    if not 0.0 <= eps <= F32.max:
+        raise _err(f"eps must be a number of zero or more in fp32's range, got {eps!r}")
     if out is None and _recorded(x, weight, bias, z):
         return _GroupNorm.apply(x, weight, bias, z, groups, activation, eps, bool(center))
     return _call(_norm, (x, weight, bias, z, out), groups, activation, eps, bool(center))[0]

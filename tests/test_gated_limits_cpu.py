@@ -18,3 +18,16 @@ def test_channels_that_index_arithmetic_cannot_hold(lib):  # noqa: F811
                         setattr(a, field, wide)
                 a.seq = _seq(2, 2) if "step" in name else a.seq
                 assert getattr(lib, name)(a, None) == -4, (name, C)
+
+
+def test_numbers_that_32_bits_do_not_hold():
+    """A positive number must still be one in 32 bits: 1e39 would be infinite there and 1e-50 zero."""
+    import kda_b200
+    x = torch.zeros(1, 4, 64)
+    for bad in (1e39, 1e-50):
+        with pytest.raises(ValueError, match="rate_scale"):
+            kda_b200.gated_scan(x, x, rate_scale=bad)
+        with pytest.raises(ValueError, match="rate_scale"):
+            kda_b200.gated_scan_step(x, x, None, None, None, None, x[0], rate_scale=bad)
+    with pytest.raises(ValueError, match="eps"):
+        kda_b200.group_norm(x, 4, eps=1e39)
