@@ -10,12 +10,14 @@ the kernel ran out, results are wrong; a recorded call's backward pass reports i
 
 Gradients: with grad mode on, a call without `ssm_state_indices` and `out` whose tensors ask for some is recorded; calls that work on a
 pool or write the caller's `out` are serving calls and record nothing.  Backward passes return the same bits whenever they run, can be
-captured in a CUDA graph (while no eager graph of the same leaves lives, as torch wants it) and are differentiable once."""
+captured in a CUDA graph (while no eager graph of the same leaves lives, as torch wants it) and are differentiable once.  Forward-mode
+derivatives are refused."""
 from __future__ import annotations
 
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi, _err, _reject_aliasing
 from .serving import (INT32_MAX, TYPES, _call, _cuda, _is, _layout, _lead, _out, _pool_rows, _ptr, _Ready, _rows, _sequences, _states, _status,
@@ -26,6 +28,12 @@ ACTIVATIONS = {None: _cabi.ACT_NONE, "silu": _cabi.ACT_SILU, "sigmoid": _cabi.AC
 
 def _recorded(*tensors):
     return torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in tensors)
+
+
+def _no_tangents(*tensors):
+    """A launch by address would lose the tangents of forward-mode derivatives, which counts as zero."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _err("forward-mode derivatives are not supported")
 
 
 # ------------------------------------------------------------------------------------------------ gated linear recurrence
@@ -153,6 +161,7 @@ def gated_scan(x, r, i=None, rate=None, r_bias=None, i_bias=None, initial_state=
     fp32: a pool [P, C] with `ssm_state_indices`, else [N, C].  Returns (y, pool or final state); without pool and `out` both are
     differentiable with respect to everything but cu_seqlens (rows behind the last sequence get zero gradients)."""
     scale = _scale(rate_scale)
+    _no_tangents(x, r, i, rate, r_bias, i_bias, initial_state)
     if ssm_state_indices is None and out is None and _recorded(x, r, i, rate, r_bias, i_bias, initial_state):
         return _GatedScan.apply(x, r, i, rate, r_bias, i_bias, initial_state, cu_seqlens, status, scale)
     return _call(_scan, (x, r, i, rate, r_bias, i_bias, initial_state, cu_seqlens, ssm_state_indices, out, status), scale, False, False)
@@ -160,6 +169,7 @@ def gated_scan(x, r, i=None, rate=None, r_bias=None, i_bias=None, initial_state=
 
 def gated_scan_step(x, r, i, rate, r_bias, i_bias, pool, ssm_state_indices=None, *, rate_scale=8.0, out=None, status=None):
     """The recurrence of the next token of each row, x, r, i [1, N, C]; records no gradients.  Returns (y, pool)."""
+    _no_tangents(x, r, i, rate, r_bias, i_bias, pool)
     return _call(_scan, (x, r, i, rate, r_bias, i_bias, pool, None, ssm_state_indices, out, status), _scale(rate_scale), True, False)
 
 
@@ -269,6 +279,7 @@ def group_norm(x, groups=None, weight=None, bias=None, z=None, *, activation=Non
     eps = float(eps)
     if not 0.0 <= eps <= F32.max:
         raise _err(f"eps must be a number of zero or more in fp32's range, got {eps!r}")
+    _no_tangents(x, weight, bias, z)
     if out is None and _recorded(x, weight, bias, z):
         return _GroupNorm.apply(x, weight, bias, z, groups, activation, eps, bool(center))
     return _call(_norm, (x, weight, bias, z, out), groups, activation, eps, bool(center))[0]
