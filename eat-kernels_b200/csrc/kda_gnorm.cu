@@ -353,11 +353,13 @@ struct Shape {
     return n < 1 ? 1 : (n > 65535 ? 65535 : n);
   }
 };
-// `vec` values an access: two of those a lane at most, in gradients four, of single values 32.  Groups of 1024 in bf16: 20 000 rows of four forward 367 us
-// with four a lane, 254 as a block's work; gradients of 4096 rows of four 97 and 258 us.  (Single values: groups of 127 take 240 us where 128 take 99.)
+// `vec` values an access.  Forward a lane has 16 values at most, in gradients four accesses, of single values 32.  Forward, eight gated groups a row:
+// 15 625 rows of 320 in fp32 166 us with 16 values a lane, 595 as a block's work, 9765 of 512 119 and 398; in bf16 13 020 rows of 768 385 with
+// 32 a lane, 360 as a block's work, 9765 of 1024 367 and 291.  Gradients of 4096 rows of four groups of 1024 in bf16 97 and 258 us.  (Single values:
+// groups of 127 take 240 us where 128 take 99.)
 Shape shape_of(int G, int D, int vec, bool grad) {
   Shape s = {1, 4, 0};
-  const int need = (D + vec - 1) / vec, most = vec > 1 ? (grad ? 4 : 2) : 32;
+  const int need = (D + vec - 1) / vec, most = vec > 1 ? (grad ? 4 : 16 / vec) : 32;
   while (s.lanes < 32 && s.lanes < need) s.lanes *= 2;
   while (s.ch <= most && s.ch * s.lanes < need) s.ch *= 2;
   if (s.ch > most) s.ch = 0;
@@ -403,7 +405,7 @@ cudaError_t launch_type(GroupNormParams p, cudaStream_t stream) {
   if (p.T == 0) e = cudaSuccess;
   else if (s.ch == 0) e = launch_wide<T, GRAD>(p, grid, stream);
   else if (wide && s.ch <= 2) e = s.ch == 1 ? launch_one<T, VEC, 1, GRAD>(p, grid, stream) : launch_one<T, VEC, 2, GRAD>(p, grid, stream);
-  else if (wide) e = launch_one<T, VEC, 4, true>(p, grid, stream);         // gradients only
+  else if (wide) e = launch_one<T, VEC, 4, GRAD || VEC == 8>(p, grid, stream);       // 16 bits: gradients only
   else if (s.ch <= 4) e = launch_one<T, 1, 4, GRAD>(p, grid, stream);
   else if (s.ch <= 8) e = launch_one<T, 1, 8, GRAD>(p, grid, stream);
   else if (s.ch <= 16) e = launch_one<T, 1, 16, GRAD>(p, grid, stream);
