@@ -5,7 +5,10 @@
 // Bound by memory: x, z (and dy) are read once and stay in registers, mean and squares are taken of the values there.  A group lies
 // in `lanes` neighbouring lanes; a thread keeps its channels for all the rows that it goes over, so that weights are read and their
 // gradients summed in registers.  Measured in bf16: 20 000 rows of 32 groups of 128, gated, one weight for all, 99 us (5.0 TB/s); 8192 rows of
-// 16 groups of 256 with all gradients 176 us for both passes (3.0 TB/s).  Groups wider than a warp holds are a block's work, which reads them again out of the caches.
+// 16 groups of 256 with all gradients 176 us for both passes (3.0 TB/s), in fp32 76 us forward and 112 for the gradients (5.3 and 6.0 TB/s).  Groups wider
+// than a warp holds are a block's work, which reads them again out of the caches: 16 384 rows of 4096 channels as one group 169 us forward (2.4 TB/s),
+// 1069 for the gradients.  Lanes of a group are a power of two: widths of 80, 160 and 320 leave three eighths of them idle (176, 179 and 255 us where
+// 128 takes 116).  Gradients with 32 single values a lane take 255 registers and spill 64 (fp32) or 112 bytes.
 #include "kda_serving.cuh"
 
 namespace kda {

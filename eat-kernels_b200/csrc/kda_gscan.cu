@@ -1,6 +1,7 @@
 // Gated linear recurrence over packed sequences, forward, and its step for single tokens (formulas and layout: kda_gscan.cuh).
-// Measured in bf16, both gates: 20 ragged prompts, 29 814 tokens of 4096 channels, 340 us (2.9 TB/s); 8192 tokens of 4096 channels in one
-// sequence 99 us, of 2560 74, with 4095 channels (read one by one) 137, in fp32 133; 65 537 tokens of 1024 channels in fp16, one gate, 160 us.
+// Measured in bf16, both gates: 20 ragged prompts, 29 814 tokens of 4096 channels, 333 us (2.9 TB/s); 8192 tokens of 4096 channels in one
+// sequence 93 us, of 2560 68, with 4095 channels (read one by one) 133, in fp32 129; 65 537 tokens of 1024 channels in fp16, one gate, 157 us.
+// A slab of channels has 16 blocks along time at most, so 65 536 tokens of 64 channels take 138 us, as long as 256 channels do.
 #include "kda_gscan.cuh"
 
 namespace kda {
@@ -325,7 +326,8 @@ cudaError_t launch_type(const GatedScanParams& p, cudaStream_t stream) {
 // ---- one token a row
 constexpr int STEP_THREADS = 128, STEP_ROWS = 4;
 
-// VEC channels a thread, up to STEP_ROWS rows a block; the rows' states and tokens are asked for before repeats are looked for.
+// VEC channels a thread, up to STEP_ROWS rows a block; the rows' states and tokens are asked for before repeats are looked for.  The input gate
+// of 32-bit tokens takes the exact exponential here and the approximate one in prompts: the two differ in last digits.
 template <typename T, int VEC, bool POWER>
 __global__ void __launch_bounds__(STEP_THREADS) kda_gated_scan_step_kernel(const GatedScanParams p) {
   using P = Pack<T, VEC>;

@@ -7,9 +7,11 @@
 // e runs backwards over the rounds by the same maps as h does forwards (e in front of a slice = F e behind it + G).  The states h
 // are computed again from those that the forward pass kept in front of each tile, inside the block, at the same barrier.  A cluster
 // has all tokens of its channels, so the sums over tokens are complete in its first block, always in the same order.
-// The gates are computed twice, once for the maps and once for the gradients: kept, they would take 48 registers more.
-// Measured in bf16, both gates: 8 ragged sequences, 10 245 tokens of 4096 channels, 273 us (2.2 TB/s); 8192 tokens in one sequence 202 us, with
-// 4095 channels 301; 16 384 tokens of 512 channels in fp32, the form without rate, 98 us.  Slices of 12 tokens (twice the code): 325 us for the first.
+// The gates are computed twice, once for the maps and once for the gradients: kept in registers, they would take 48 more.  (In shared memory
+// they would fit; that is not done.)  In fp32, read one by one, with both gates, the kernel spills 124 bytes, without rate 4; the others spill none.
+// Measured in bf16, both gates: 8 ragged sequences, 10 245 tokens of 4096 channels, 271 us (2.2 TB/s); 8192 tokens in one sequence 199 us, with
+// 4095 channels 300, in fp32 292; 16 384 tokens of 512 channels in fp32, the form without rate, 94 us.  Slices of 12 tokens (twice the code): 325 us
+// for the first.
 #include "kda_gscan.cuh"
 
 namespace kda {
@@ -23,7 +25,7 @@ constexpr int DEPTH = 2;                 // rounds of tokens on their way or wor
 constexpr int S = 6, TILE = WARPS * S;   // tokens of a slice, of a block
 static_assert(TILE == GATED_SCAN_TILE, "the forward pass keeps the states in front of the tiles");
 
-// Two blocks an SM leave 17 KB beside the tokens of 16-bit calls.
+// With 48 KB of tokens (16 bits, both gates) and 16 KB of tiles (16 blocks a cluster) some 77 KB a block: two an SM leave 36 KB each.
 template <int V>
 struct Shared {
   Vec<V> F[2][WARPS][32], U[2][WARPS][32], G[2][WARPS][32];          // the maps of the block's slices

@@ -155,7 +155,9 @@ class _GatedScan(torch.autograd.Function):
 def gated_scan(x, r, i=None, rate=None, r_bias=None, i_bias=None, initial_state=None, cu_seqlens=None, *, rate_scale=8.0,
                ssm_state_indices=None, out=None, status=None):
     """Gated linear recurrence over prompts: per channel h = f h + gain g x, y = h, with s = sigmoid(r + r_bias), g = sigmoid(i + i_bias)
-    (1 without i) and, with `rate`, f = exp(-rate_scale softplus(rate) s), gain = sqrt(1 - f^2); without it f = s, gain = 1 - s.
+    (1 without i) and, with `rate`, f = exp(-rate_scale softplus(rate) s), gain = sqrt(1 - f^2); without it f = s, gain = 1 - s.  The gain
+    holds for every token, a sequence's first one too: models that leave it out there (gain 1 behind a reset) get another first state.
+    Of 16-bit tokens an input gate below 2^-64 counts as shut.
 
     x, r, i [1, T, C] of one type (bf16, fp16 or fp32; any token strides); rate, r_bias, i_bias [C] fp32, each may be None.  State
     fp32: a pool [P, C] with `ssm_state_indices`, else [N, C].  Returns (y, pool or final state); without pool and `out` both are
@@ -168,7 +170,8 @@ def gated_scan(x, r, i=None, rate=None, r_bias=None, i_bias=None, initial_state=
 
 
 def gated_scan_step(x, r, i, rate, r_bias, i_bias, pool, ssm_state_indices=None, *, rate_scale=8.0, out=None, status=None):
-    """The recurrence of the next token of each row, x, r, i [1, N, C]; records no gradients.  Returns (y, pool)."""
+    """The recurrence of the next token of each row, x, r, i [1, N, C]; records no gradients; equal to a prompt's tokens but for last digits.
+    Returns (y, pool)."""
     _no_tangents(x, r, i, rate, r_bias, i_bias, pool)
     return _call(_scan, (x, r, i, rate, r_bias, i_bias, pool, None, ssm_state_indices, out, status), _scale(rate_scale), True, False)
 
