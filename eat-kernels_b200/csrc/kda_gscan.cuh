@@ -321,20 +321,22 @@ __device__ __forceinline__ Vec<2> values(const Pack<__nv_bfloat16, 2>& p) {     
 
 // Of V channels: sigmoid and, with BOTH, 1 minus it, both to relative accuracy.  The approximate exponential and reciprocal are good to
 // 2^-22; for 32-bit tokens the exponential's argument is taken in two parts, since its rounding would be off by as much again for each unit of x.
-// Alone, the sigmoid of an infinitely low x is zero; with the other one it stays at 2^-126, so that the product that makes that one is 1.
-template <typename T, int V, bool BOTH = true>
+// Alone, the sigmoid of an infinitely low x is zero; with the other one it stays at 2^-126, so that the product that makes that one is 1, or, with
+// SHUTS, both become zero (the reciprocal of 2^127 does), for uses where the other one only stands in products with the first.
+template <typename T, int V, bool BOTH = true, bool SHUTS = false>
 __device__ __forceinline__ void sigmoids(Vec<V> x, Vec<V> bias, Vec<V>& s, Vec<V>& n) {
 #pragma unroll
   for (int k = 0; k < V; k++) {
+    constexpr float MOST = SHUTS ? 127.0f : 126.0f;
     float e;
     if constexpr (sizeof(T) == 4) {
-      const float v = -(x.v[k] + bias.v[k]), hi = BOTH ? min_or_nan(v * LOG2E_F, 126.0f) : v * LOG2E_F;
+      const float v = -(x.v[k] + bias.v[k]), hi = BOTH ? min_or_nan(v * LOG2E_F, MOST) : v * LOG2E_F;
       const float lo = fmaf(v, LOG2E_F, -hi) + v * LOG2E_REST;
       e = ex2_fast(hi);
       e = fabsf(hi) < 126.0f ? fmaf(e, lo * LN2_F, e) : e;
     } else {
       const float t = fmaf(x.v[k], -LOG2E_F, bias.v[k]);
-      e = ex2_fast(BOTH ? min_or_nan(t, 126.0f) : t);
+      e = ex2_fast(BOTH ? min_or_nan(t, MOST) : t);
     }
     s.v[k] = rcp_fast(e + 1.0f);
     n.v[k] = BOTH ? e * s.v[k] : 0.0f;

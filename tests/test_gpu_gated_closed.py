@@ -58,3 +58,23 @@ def test_a_shut_output_gate_gives_zeros(dtype):
         y = kda_b200.group_norm(x, G, None, None, z, activation="sigmoid")
         open_, dz = kda_b200.group_norm(x, G, None, None, z.detach().masked_fill(shut, 0.5), activation="sigmoid"), torch.autograd.grad(y, z, dy)[0]
         assert (y[shut] == 0).all() and (dz[shut] == 0).all() and torch.equal(y[~shut], open_[~shut])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("form", ["power", "logistic"])
+def test_nothing_flows_back_through_a_shut_input_gate(dtype, form):
+    """Its token gets zeros and so does the gate; everything else is as for a token of zeros there."""
+    import kda_b200
+    for C in (64, 33):
+        gen, lens = generator(45 + C), [30, 1, 160]
+        x, r, i, rate, rb, ib = inputs(gen, sum(lens), C, dtype, form, 1)
+        shut = torch.rand(i.shape, generator=gen, device=DEV) < 0.3
+        states, dy, dfinal, got = randn(gen, 3, C), randn(gen, *x.shape, dtype=dtype), randn(gen, 3, C), []
+        for xs, gate in ((x, i.masked_fill(shut, LOW)), (x.masked_fill(shut, 0.0), i)):
+            v = [t.detach().requires_grad_() for t in (xs, r, gate, *(t for t in (rate, rb, ib, states) if t is not None))]
+            it = iter(v[3:])
+            out = kda_b200.gated_scan(*v[:3], next(it) if rate is not None else None, *it, cu_of(lens))
+            got.append(torch.autograd.grad(out, v, (dy, dfinal)))
+        masked, none = got
+        assert (masked[0][shut] == 0).all() and (masked[2][shut] == 0).all()
+        assert torch.equal(masked[0][~shut], none[0][~shut]) and all(torch.equal(a, b) for a, b in zip(masked[1:], none[1:]))
