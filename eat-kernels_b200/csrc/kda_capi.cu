@@ -545,7 +545,7 @@ void bound_waits(P& p) {
   p.more_maps = (g_debug_flags & kda::DBG_MORE_MAPS) != 0;
 }
 
-// Channels whose blocks, of up to 128 channels on top, are still counted in 32 bits
+// Channels whose blocks, with up to 512 channels on top, are still counted in 32 bits
 constexpr int GATED_SCAN_MAX_CHANNELS = 0x7fffffff / 2;
 
 int gated_scan_launch(const KdaGatedScanArgs* a, bool step, void* stream) {

@@ -8,7 +8,7 @@
 // are computed again from those that the forward pass kept in front of each tile, inside the block, at the same barrier.  A cluster
 // has all tokens of its channels, so the sums over tokens are complete in its first block, always in the same order.
 // The gates are computed twice, once for the maps and once for the gradients: kept in registers, they would take 48 more.  (In shared memory
-// they would fit; that is not done.)  The kernel for fp32 tokens read one by one, with an input gate and no rate, spills 4 bytes, the others none.
+// they would fit; that is not done.)  The kernel for fp32 tokens read one by one, with rate and input gate, spills 4 bytes, the others none.
 // Measured in bf16, both gates: 8 ragged sequences, 10 245 tokens of 4096 channels, 271 us (2.2 TB/s); 8192 tokens in one sequence 199 us, with
 // 4095 channels 300, in fp32 292; 16 384 tokens of 512 channels in fp32, the form without rate, 94 us.  Slices of 12 tokens (twice the code): 325 us
 // for the first.
